@@ -1,7 +1,8 @@
 """gsplat_b200: B200-native (sm_100a) Gaussian-splatting training hot path.
 
 Drop-in for the reference gsplat Python API of that path: ``rasterization``,
-the ``gsplat.cuda._wrapper`` operators and ``gsplat.optimizers.SelectiveAdam``.
+the ``gsplat.cuda._wrapper`` operators and ``gsplat.optimizers.SelectiveAdam``; next to
+them ``orthogonalize`` and the ``Muon`` optimizer for parameters that are matrices.
 All compute runs in the hand-written kernels of ``libgsplat_b200.so`` (C ABI in
 ``include/gsplat_b200.h``); there is no CPU fallback.
 """
@@ -19,6 +20,8 @@ from .cuda._wrapper import (
     has_reloc,
     isect_offset_encode,
     isect_tiles,
+    muon,
+    orthogonalize,
     persp_proj,
     proj,
     quat_scale_to_covar_preci,
@@ -27,13 +30,14 @@ from .cuda._wrapper import (
     spherical_harmonics,
     world_to_cam,
 )
-from .optimizers import SelectiveAdam
+from .optimizers import Muon, SelectiveAdam
 from .rendering import RasterizeMode, RenderMode, rasterization
 
 __version__ = "0.1.0"
 
 __all__ = [
     "CameraModel",
+    "Muon",
     "RasterizeMode",
     "RenderMode",
     "SelectiveAdam",
@@ -48,6 +52,8 @@ __all__ = [
     "has_reloc",
     "isect_offset_encode",
     "isect_tiles",
+    "muon",
+    "orthogonalize",
     "persp_proj",
     "proj",
     "quat_scale_to_covar_preci",

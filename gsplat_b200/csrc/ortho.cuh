@@ -1,0 +1,145 @@
+// Shared declarations of the matrix-orthogonalising operators (orthogonalize.cu,
+// ortho_thin.cu, ortho_gemm.cu).
+//
+// X0 = U / max(|U|_F, eps), then for every step (a, b, c)
+//     A = X X^T,  B = b A + c A A,  X <- a X + B X
+// on the orientation whose rows are the shorter side (a tall U is transposed:
+// the iteration commutes with transposition).
+#pragma once
+
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "common.cuh"
+#include "gsb_internal.h"
+
+namespace gsb {
+
+enum OrthoDtype : int { kOrthoF32 = 0, kOrthoBF16 = 1, kOrthoF16 = 2 };
+
+constexpr int kOrthoMaxSteps = 32;
+constexpr int kOrthoMaxTensors = 32; // tensors of one launch
+
+struct OrthoCoefficients {
+    int steps;
+    float c[kOrthoMaxSteps][3];
+};
+
+template <typename T> __device__ __forceinline__ float to_f32(T v);
+template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <> __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+
+// One value of a type known at run time (uniform over the launch).
+__device__ __forceinline__ float load_as_f32(const void *p, size_t i, int dtype) {
+    if (dtype == kOrthoF32) return static_cast<const float *>(p)[i];
+    if (dtype == kOrthoBF16) return to_f32(static_cast<const __nv_bfloat16 *>(p)[i]);
+    return to_f32(static_cast<const __half *>(p)[i]);
+}
+__device__ __forceinline__ void store_from_f32(void *p, size_t i, int dtype, float v) {
+    if (dtype == kOrthoF32) static_cast<float *>(p)[i] = v;
+    else if (dtype == kOrthoBF16) static_cast<__nv_bfloat16 *>(p)[i] = from_f32<__nv_bfloat16>(v);
+    else static_cast<__half *>(p)[i] = from_f32<__half>(v);
+}
+
+// Momentum and the matrix that is orthogonalised, in 32 bits: m <- m + (1 - mu)(g - m),
+// u = g + mu (m - g) (Nesterov) or m.
+__device__ __forceinline__ float muon_momentum(float g, float m, float one_minus_mu) {
+    return fmaf(one_minus_mu, g - m, m);
+}
+__device__ __forceinline__ float muon_update(float g, float m_new, float mu, int nesterov) {
+    return nesterov ? fmaf(mu, m_new - g, g) : m_new;
+}
+__device__ __forceinline__ float muon_param(float p, float o, float lr, float decay) {
+    return fmaf(-lr, o, p * decay);
+}
+
+// The tensors of one Muon step that share a shape: [batch_t, rows, cols] each.
+// Matrix b of the launch belongs to the tensor t with first[t] <= b < first[t + 1].
+struct MuonTable {
+    int n;
+    int dtype, state_dtype, nesterov;
+    float mu, one_minus_mu;
+    const bool *valid; // per leading row of every tensor, or NULL
+    void *param[kOrthoMaxTensors];
+    const void *grad[kOrthoMaxTensors];
+    void *momentum[kOrthoMaxTensors];
+    float lr[kOrthoMaxTensors], decay[kOrthoMaxTensors]; // decay = 1 - lr * weight_decay
+    int inner[kOrthoMaxTensors];         // matrices per leading row
+    long long skipped[kOrthoMaxTensors]; // the tensor's matrices before its first one here
+    long long first[kOrthoMaxTensors + 1];
+};
+
+__device__ __forceinline__ int muon_tensor_of(const MuonTable &t, long long b) {
+    int i = 0;
+    while (i + 1 < t.n && b >= t.first[i + 1]) ++i;
+    return i;
+}
+__device__ __forceinline__ bool muon_visible(const MuonTable &t, int i, long long b) {
+    return t.valid == nullptr || t.valid[(b - t.first[i] + t.skipped[i]) / t.inner[i]];
+}
+
+// --- thin matrices (ortho_thin.cu) -----------------------------------------
+// short side <= 4 and long side <= 128: a few lanes hold one matrix.
+bool ortho_is_thin(int rows, int cols);
+int ortho_thin_fwd(long long batch, int rows, int cols, int dtype, const void *x, void *y,
+                   const OrthoCoefficients &co, float eps, cudaStream_t stream);
+int ortho_thin_bwd(long long batch, int rows, int cols, int dtype, const void *x, const void *v_y, void *v_x,
+                   const OrthoCoefficients &co, float eps, cudaStream_t stream);
+int ortho_thin_muon(const MuonTable &table, int rows, int cols, const OrthoCoefficients &co, float eps,
+                    cudaStream_t stream);
+
+// --- tiled products (ortho_gemm.cu) ----------------------------------------
+// A matrix of the iteration: value = scale * (hi + lo), both fp16, so 22
+// significand bits. Row-major, rows of `ld` elements (a multiple of 8), one
+// matrix after `stride` elements.
+struct OrthoPlanes {
+    __half *hi, *lo;
+    int ld;
+    long long stride;
+};
+
+enum OrthoEpilogue : int {
+    kEpiGram,   // A: off-diagonal part and its diagonal
+    kEpiSquare, // B from A A
+    kEpiApply,  // X <- a X + B X
+    kEpiOut,    // the last step, to the caller's tensor
+    kEpiMuon,   // the last step, into the parameters
+    kEpiSym,    // S = G X^T + X G^T
+    kEpiAnti,   // T = b S + c (S A + A S)
+};
+
+// C[b] = sum over pairs p of P_p[b] Q_p[b] (M x N, contraction K), then the epilogue,
+// with e the element-wise operand, D = diag_in and d = c the constants:
+//   kEpiGram    i != j: out = c0 C, i == j: diag_out = c1 C, out = 0
+//   kEpiSquare  i != j: out = (c0 + c1 (D_i + D_j)) e + c2 C
+//               i == j: diag_out = c3 D + c4 D D + c5 C, out = 0
+//   kEpiApply   out = ((c0 + D_i) e + c1 C) c2, kEpiOut and kEpiMuon likewise
+//   kEpiSym     out = c0 C
+//   kEpiAnti    out = (c0 + c1 (D_i + D_j)) e + c2 C
+struct OrthoGemm {
+    long long batch;
+    int M, N, K;
+    int pairs;      // 1 or 2
+    int q_k_major;  // Q stored [N, K] (1) or [K, N] (0)
+    int symmetric;  // only tiles on and below the diagonal, mirrored when written
+    int split;      // products of hi + lo (three products); else of hi alone
+    OrthoPlanes p[2], q[2];
+    int epilogue;
+    float c[6];
+    OrthoPlanes e, out;      // the element-wise operand and the result
+    const float *diag_in;    // [batch, M]
+    float *diag_out;         // [batch, M]
+    void *y;                 // kEpiOut: [batch, rows, cols] of `dtype`
+    int dtype, transposed;   // transposed: y / param are [N, M] in memory
+};
+
+int ortho_gemm(const OrthoGemm &g, const MuonTable *table, cudaStream_t stream);
+
+} // namespace gsb

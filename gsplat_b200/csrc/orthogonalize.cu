@@ -1,0 +1,677 @@
+// Newton-Schulz orthogonalisation of matrices, its backward pass and the Muon
+// step: the entry points, and the passes before and after the tiled products.
+//
+// Numbers of the tiled path. Every matrix of the iteration is kept as
+// scale * (hi + lo), both fp16 (22 significand bits), with power-of-two scales
+// from bounds on its values, so that nothing overflows and little is subnormal:
+// X <= s_max, the largest singular value that the polynomials reach from [0, 1];
+// A <= s_max^2; B <= max |b t + c t^2| over t <= s_max^2. The diagonals of A and B are kept
+// apart in 32 bits: near convergence A is close to a multiple of the identity, and
+// rounding its diagonal would cost more than all of its other entries together.
+// With A = D + O (D diagonal) the products are
+//     A A = O O + D O + O D + D D,   B X = O_B X + D_B X,
+// and the terms with a diagonal are element-wise, in the epilogue.
+// Products are of hi + lo, in three matrix products (lo lo is below 2^-22). Those of
+// bfloat16 matrices (8 bits) are of hi alone, with its 11 bits, while X itself goes from
+// step to step with hi and lo: a X + B X is where small singular values would lose theirs.
+// The result is then 0.0005 to 0.001 off (2-norm), against the type's own rounding of 0.0017.
+// float16 results would be off by three times their rounding that way, and backward passes by the
+// sum of theirs, so they take hi + lo as float32 does; so do matrices of at most 128 x 128, whose
+// calls are bound by latency.
+#include <algorithm>
+#include <cmath>
+
+#include "ortho.cuh"
+
+namespace gsb {
+
+// --- norms and the split into planes ----------------------------------------
+constexpr int kNormThreads = 256;
+constexpr long long kNormChunk = 16384; // elements a block
+constexpr int kSplitTile = 64;
+
+struct OrthoSource { // what is read: x, or the Muon update of its matrix
+    const void *x;
+    int dtype;
+};
+
+__device__ __forceinline__ float source_at(const OrthoSource &s, const MuonTable &tab, int t, long long b, size_t numel,
+                                           size_t e, bool write_momentum) {
+    if (tab.n == 0) return load_as_f32(s.x, (size_t)b * numel + e, s.dtype);
+    const size_t at = (size_t)(b - tab.first[t]) * numel + e;
+    const float g = load_as_f32(tab.grad[t], at, tab.dtype);
+    const float m = muon_momentum(g, load_as_f32(tab.momentum[t], at, tab.state_dtype), tab.one_minus_mu);
+    if (write_momentum) store_from_f32(tab.momentum[t], at, tab.state_dtype, m);
+    return muon_update(g, m, tab.mu, tab.nesterov);
+}
+
+__device__ __forceinline__ double block_sum(double v) {
+    __shared__ double part[kNormThreads / 32];
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x / 32] = v;
+    __syncthreads();
+    v = 0.0;
+    for (int w = 0; w < kNormThreads / 32; ++w) v += part[w];
+    return v;
+}
+
+// Sums of squares of the chunks of each matrix, in 64 bits and a fixed order.
+__global__ void __launch_bounds__(kNormThreads)
+    ortho_norm_kernel(OrthoSource src, const __grid_constant__ MuonTable tab, size_t numel, int chunks, double *partial) {
+    const long long b = blockIdx.x / chunks;
+    const int chunk = (int)(blockIdx.x % chunks);
+    const int t = tab.n > 0 ? muon_tensor_of(tab, b) : 0;
+    if (tab.n > 0 && !muon_visible(tab, t, b)) return;
+    const size_t first = (size_t)chunk * kNormChunk, last = min(numel, first + (size_t)kNormChunk);
+    double s = 0.0;
+    for (size_t e = first + threadIdx.x; e < last; e += kNormThreads) {
+        const double v = source_at(src, tab, t, b, numel, e, false);
+        s = fma(v, v, s);
+    }
+    s = block_sum(s);
+    if (threadIdx.x == 0) partial[blockIdx.x] = s;
+}
+
+__device__ __forceinline__ double sum_partials(const double *partial, long long b, int chunks) {
+    double s = 0.0;
+    for (int c = threadIdx.x; c < chunks; c += kNormThreads) s += partial[b * chunks + c];
+    return block_sum(s);
+}
+
+// planes <- factor * source, in the orientation whose rows are the shorter side.
+// eps > 0: factor = scale / max(norm, eps), and norm_out gets the norm, negated
+// below eps. eps = 0: factor = the power of two that brings the norm to (scale / 2, scale], and
+// norm_out gets the factor.
+__global__ void __launch_bounds__(kNormThreads)
+    ortho_split_kernel(OrthoSource src, const __grid_constant__ MuonTable tab, int rows, int cols, int transposed,
+                       const double *partial, int chunks, float scale, float eps, float *norm_out, OrthoPlanes out,
+                       int tiles_r, int tiles_c) {
+    __shared__ float tile[kSplitTile][kSplitTile + 1];
+    const long long per = (long long)tiles_r * tiles_c;
+    const long long b = blockIdx.x / per;
+    const int ti = (int)(blockIdx.x % per);
+    const int r0 = (ti / tiles_c) * kSplitTile, c0 = (ti % tiles_c) * kSplitTile;
+    const int t = tab.n > 0 ? muon_tensor_of(tab, b) : 0;
+    if (tab.n > 0 && !muon_visible(tab, t, b)) return;
+    const float norm = (float)sqrt(sum_partials(partial, b, chunks));
+    float div, mul;
+    if (eps > 0.f) {
+        div = norm < eps ? eps : norm;
+        mul = scale;
+        if (ti == 0 && threadIdx.x == 0) norm_out[b] = norm < eps ? -1.f : norm;
+    } else {
+        const int e = norm > 0.f && norm < INFINITY ? min(max(ilogb(norm) + 1, -100), 126) : 0;
+        div = 1.f;
+        mul = scale * exp2f((float)-e);
+        if (ti == 0 && threadIdx.x == 0) norm_out[b] = mul;
+    }
+    const size_t numel = (size_t)rows * cols;
+    const int cx = threadIdx.x % kSplitTile, ry = threadIdx.x / kSplitTile;
+    for (int r = ry; r < kSplitTile; r += kNormThreads / kSplitTile)
+        if (r0 + r < rows && c0 + cx < cols)
+            tile[r][cx] = source_at(src, tab, t, b, numel, (size_t)(r0 + r) * cols + c0 + cx, true) / div * mul;
+    __syncthreads();
+    for (int r = ry; r < kSplitTile; r += kNormThreads / kSplitTile) {
+        const int i = transposed ? c0 + r : r0 + r, j = transposed ? r0 + cx : c0 + cx;
+        if (i < (transposed ? cols : rows) && j < (transposed ? rows : cols)) {
+            const float v = transposed ? tile[cx][r] : tile[r][cx];
+            const __half h = __float2half_rn(v);
+            const size_t at = (size_t)b * out.stride + (size_t)i * out.ld + j;
+            out.hi[at] = h;
+            out.lo[at] = __float2half_rn(v - __half2float(h));
+        }
+    }
+}
+
+// Partial sums of <G, X> over the rows of each matrix (32-bit products of planes).
+__global__ void __launch_bounds__(kNormThreads)
+    ortho_dot_kernel(OrthoPlanes g, OrthoPlanes x, int m, int n, int chunks, double *partial) {
+    const long long b = blockIdx.x / chunks;
+    const int chunk = (int)(blockIdx.x % chunks);
+    double s = 0.0;
+    for (int i = chunk; i < m; i += chunks)
+        for (int j = threadIdx.x; j < n; j += kNormThreads) {
+            const size_t gi = (size_t)b * g.stride + (size_t)i * g.ld + j, xi = (size_t)b * x.stride + (size_t)i * x.ld + j;
+            s += (double)(__half2float(g.hi[gi]) + __half2float(g.lo[gi])) *
+                 (double)(__half2float(x.hi[xi]) + __half2float(x.lo[xi]));
+        }
+    s = block_sum(s);
+    if (threadIdx.x == 0) partial[blockIdx.x] = s;
+}
+
+// G's planes brought back to a norm in (scale / 2, scale] by a power of two, which its
+// factor takes too. <G, G> in `partial`.
+__global__ void __launch_bounds__(kNormThreads)
+    ortho_rescale_kernel(OrthoPlanes g, int m, int n, int chunks, const double *partial, float scale, const float *factor_in,
+                         float fallen, float *factor_out) {
+    const long long b = blockIdx.x / chunks;
+    const int chunk = (int)(blockIdx.x % chunks);
+    const float norm = (float)sqrt(sum_partials(partial, b, chunks));
+    const int e = norm > 0.f && norm < INFINITY ? min(max(ilogb(norm) + 1, -100), 126) : ilogb(scale);
+    const float mul = scale * exp2f((float)-e);
+    if (chunk == 0 && threadIdx.x == 0) factor_out[b] = factor_in[b] * fallen * mul;
+    for (int i = chunk; i < m; i += chunks)
+        for (int j = threadIdx.x; j < n; j += kNormThreads) {
+            const size_t at = (size_t)b * g.stride + (size_t)i * g.ld + j;
+            const float v = (__half2float(g.hi[at]) + __half2float(g.lo[at])) * mul;
+            const __half h = __float2half_rn(v);
+            g.hi[at] = h;
+            g.lo[at] = __float2half_rn(v - __half2float(h));
+        }
+}
+
+// v_x = (G - X0 <G, X0>) / norm, or G / eps for a matrix whose norm is below eps.
+__global__ void __launch_bounds__(kNormThreads)
+    ortho_grad_out_kernel(OrthoPlanes g, OrthoPlanes x, int rows, int cols, int transposed, const double *partial,
+                          int chunks, const float *norms, const float *g_factor, float g_scale, float x_scale, float eps,
+                          void *v_x, int dtype, int tiles_r, int tiles_c) {
+    __shared__ float tile[kSplitTile][kSplitTile + 1];
+    const long long per = (long long)tiles_r * tiles_c;
+    const long long b = blockIdx.x / per;
+    const int ti = (int)(blockIdx.x % per);
+    const int r0 = (ti / tiles_c) * kSplitTile, c0 = (ti % tiles_c) * kSplitTile; // of v_x
+    const double dot = sum_partials(partial, b, chunks);
+    const float norm = norms[b];
+    const bool small = norm < 0.f;
+    const float along = small ? 0.f : (float)(dot / ((double)x_scale * x_scale));
+    const float div = small ? eps : norm;
+    // g_factor and g_scale are powers of two; one after the other keeps both in range
+    const float f = g_factor[b];
+    const int cx = threadIdx.x % kSplitTile, ry = threadIdx.x / kSplitTile;
+    for (int r = ry; r < kSplitTile; r += kNormThreads / kSplitTile) {
+        const int i = transposed ? c0 + r : r0 + r, j = transposed ? r0 + cx : c0 + cx;
+        if (i < (transposed ? cols : rows) && j < (transposed ? rows : cols)) {
+            const size_t gi = (size_t)b * g.stride + (size_t)i * g.ld + j, xi = (size_t)b * x.stride + (size_t)i * x.ld + j;
+            const float gv = __half2float(g.hi[gi]) + __half2float(g.lo[gi]);
+            const float xv = __half2float(x.hi[xi]) + __half2float(x.lo[xi]);
+            const float v = fmaf(-xv, along, gv) / g_scale / f / div;
+            if (transposed) tile[cx][r] = v;
+            else tile[r][cx] = v;
+        }
+    }
+    __syncthreads();
+    for (int r = ry; r < kSplitTile; r += kNormThreads / kSplitTile)
+        if (r0 + r < rows && c0 + cx < cols)
+            store_from_f32(v_x, (size_t)b * rows * cols + (size_t)(r0 + r) * cols + c0 + cx, dtype, tile[r][cx]);
+}
+
+// --- the plan of one call -----------------------------------------------------
+constexpr double kPlaneTop = 16384.0; // bound on scaled values: a factor of four below fp16's largest
+
+static double pow2_floor(double v) { return std::exp2(std::floor(std::log2(v))); }
+
+struct OrthoScales {
+    double x, a, b;           // of X, A, B
+    double top, top_b, slope; // bounds: singular values, |B|, |p'|
+    double worst_t;           // |b| 2 top + 4 |c| top^3 over the steps: of T for a G of norm 1
+};
+
+// Bounds over [0, 1] under the steps' polynomials p(s) = a s + b s^3 + c s^5.
+static OrthoScales ortho_scales(const OrthoCoefficients &co) {
+    OrthoScales r = {};
+    double m = 1.0, top = 1.0;
+    r.slope = 1.0;
+    for (int k = 0; k < co.steps; ++k) {
+        const double a = co.c[k][0], b = co.c[k][1], c = co.c[k][2];
+        auto p = [&](double s) { return std::fabs(s * (a + s * s * (b + s * s * c))); };
+        auto dp = [&](double t) { return std::fabs(a + t * (3 * b + t * 5 * c)); }; // t = s^2
+        auto q = [&](double t) { return std::fabs(t * (b + t * c)); };
+        double next = p(m), slope = std::fmax(dp(0.0), dp(m * m)), qb = q(m * m);
+        // interior extrema: p' = 0 at t = (-3b +- sqrt(9 b^2 - 20 a c)) / (10 c); p'' = 0 at t = -3b / (10 c); q' = 0 at -b / 2c
+        auto at = [&](double t) { if (t > 0 && t < m * m) next = std::fmax(next, p(std::sqrt(t))); };
+        if (c != 0.0) {
+            const double disc = 9 * b * b - 20 * a * c;
+            if (disc >= 0) {
+                at((-3 * b + std::sqrt(disc)) / (10 * c));
+                at((-3 * b - std::sqrt(disc)) / (10 * c));
+            }
+            const double ti = -3 * b / (10 * c), tq = -b / (2 * c);
+            if (ti > 0 && ti < m * m) slope = std::fmax(slope, dp(ti));
+            if (tq > 0 && tq < m * m) qb = std::fmax(qb, q(tq));
+        } else if (b != 0.0) {
+            at(-a / (3 * b));
+        }
+        r.slope = std::fmax(r.slope, slope);
+        r.top_b = std::fmax(r.top_b, qb);
+        r.worst_t = std::fmax(r.worst_t, 2 * m * (std::fabs(b) + 2 * std::fabs(c) * m * m));
+        m = next;
+        top = std::fmax(top, m);
+    }
+    r.top = top;
+    return r;
+}
+
+constexpr double kOrthoMaxTop = 16.0; // larger singular values would leave the planes' range
+
+struct OrthoPlan {
+    int rows, cols, m, n, transposed, steps;
+    bool split, backward;
+    int chunks;
+    OrthoScales s;
+    int ldx, lda;
+    long long px, pa; // elements of one matrix's plane
+    size_t per_matrix; // scratch bytes a matrix
+    size_t fixed;      // and for alignment
+};
+
+static size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
+
+static OrthoPlan ortho_plan(int rows, int cols, int dtype, const OrthoCoefficients &co, bool backward) {
+    OrthoPlan p = {};
+    p.rows = rows;
+    p.cols = cols;
+    p.transposed = rows > cols;
+    p.m = p.transposed ? cols : rows;
+    p.n = p.transposed ? rows : cols;
+    p.steps = co.steps;
+    p.backward = backward;
+    p.split = dtype != kOrthoBF16 || backward || p.n <= 128;
+    p.chunks = (int)(((long long)rows * cols + kNormChunk - 1) / kNormChunk);
+    p.s = ortho_scales(co);
+    p.ldx = (p.n + 7) / 8 * 8;
+    p.lda = (p.m + 7) / 8 * 8;
+    p.px = (long long)p.m * p.ldx;
+    p.pa = (long long)p.m * p.lda;
+    const int kept = backward ? co.steps : 1;
+    const size_t halves = 2 * sizeof(__half);
+    size_t bytes = 0;
+    bytes += (backward ? kept : 2) * halves * p.px;        // X
+    bytes += 2 * kept * halves * p.pa;                     // O_A, O_B
+    bytes += 2 * kept * sizeof(float) * p.m;               // diagonals
+    bytes += sizeof(double) * (size_t)p.chunks + 3 * sizeof(float);
+    if (backward) bytes += 2 * halves * p.px + 2 * halves * p.pa; // G twice, S, T
+    p.per_matrix = bytes;
+    p.fixed = 256 * (size_t)(8 * kept + 24);
+    return p;
+}
+
+constexpr size_t kScratchBudget = (size_t)1 << 30;
+
+static long long ortho_chunk(const OrthoPlan &p, long long batch) {
+    long long n = (long long)(kScratchBudget / p.per_matrix);
+    // one launch's grid holds a chunk's tiles
+    const long long tiles = (long long)((p.rows + 63) / 64) * ((p.cols + 63) / 64) + p.chunks;
+    if (n > 0x3fffffffll / tiles) n = 0x3fffffffll / tiles;
+    if (n < 1) n = 1;
+    return n < batch ? n : batch;
+}
+
+struct Carver {
+    char *p;
+    template <typename T> T *take(size_t n) {
+        T *r = reinterpret_cast<T *>(p);
+        p += align256(n * sizeof(T));
+        return r;
+    }
+    OrthoPlanes planes(long long batch, long long size, int ld) {
+        OrthoPlanes o;
+        o.hi = take<__half>((size_t)batch * size);
+        o.lo = take<__half>((size_t)batch * size);
+        o.ld = ld;
+        o.stride = size;
+        return o;
+    }
+};
+
+struct OrthoBuffers {
+    OrthoPlanes x[kOrthoMaxSteps], a[kOrthoMaxSteps], b[kOrthoMaxSteps];
+    float *da[kOrthoMaxSteps], *db[kOrthoMaxSteps];
+};
+
+static int run_split(const OrthoPlan &p, long long nb, const OrthoSource &src, const MuonTable &tab, float scale,
+                     float eps, float *norm_out, double *partial, const OrthoPlanes &out, cudaStream_t stream) {
+    ortho_norm_kernel<<<(unsigned)(nb * p.chunks), kNormThreads, 0, stream>>>(src, tab, (size_t)p.rows * p.cols,
+                                                                             p.chunks, partial);
+    if (int e = check_launch("ortho_norm_kernel")) return e;
+    const int tr = (p.rows + kSplitTile - 1) / kSplitTile, tc = (p.cols + kSplitTile - 1) / kSplitTile;
+    ortho_split_kernel<<<(unsigned)(nb * tr * tc), kNormThreads, 0, stream>>>(
+        src, tab, p.rows, p.cols, p.transposed, partial, p.chunks, scale, eps, norm_out, out, tr, tc);
+    return check_launch("ortho_split_kernel");
+}
+
+static OrthoGemm gemm_base(const OrthoPlan &p, long long nb) {
+    OrthoGemm g = {};
+    g.batch = nb;
+    g.pairs = 1;
+    g.split = p.split;
+    g.transposed = p.transposed;
+    return g;
+}
+
+// A and its polynomial B of step k, from X_k.
+static int run_poly(const OrthoPlan &p, long long nb, const float c[3], double sb, const OrthoPlanes &x,
+                    const OrthoPlanes &a, const OrthoPlanes &b, float *da, float *db, const MuonTable *tab,
+                    cudaStream_t stream) {
+    OrthoGemm g = gemm_base(p, nb);
+    g.M = g.N = p.m;
+    g.K = p.n;
+    g.q_k_major = g.symmetric = 1;
+    g.p[0] = g.q[0] = x;
+    g.epilogue = kEpiGram;
+    g.c[0] = (float)(p.s.a / (p.s.x * p.s.x));
+    g.c[1] = (float)(1.0 / (p.s.x * p.s.x));
+    g.out = a;
+    g.diag_out = da;
+    if (int e = ortho_gemm(g, tab, stream)) return e;
+    g.K = p.m;
+    g.p[0] = g.q[0] = g.e = a;
+    g.epilogue = kEpiSquare;
+    g.c[0] = (float)(c[1] * sb / p.s.a);
+    g.c[1] = (float)(c[2] * sb / p.s.a);
+    g.c[2] = (float)(c[2] * sb / (p.s.a * p.s.a));
+    g.c[3] = c[1];
+    g.c[4] = c[2];
+    g.c[5] = (float)(c[2] / (p.s.a * p.s.a));
+    g.out = b;
+    g.diag_in = da;
+    g.diag_out = db;
+    return ortho_gemm(g, tab, stream);
+}
+
+static OrthoGemm apply_gemm(const OrthoPlan &p, long long nb, float a, double sb, const OrthoPlanes &x,
+                            const OrthoPlanes &b, const float *db) {
+    OrthoGemm g = gemm_base(p, nb);
+    g.M = g.K = p.m;
+    g.N = p.n;
+    g.p[0] = b;
+    g.q[0] = g.e = x;
+    g.diag_in = db;
+    g.epilogue = kEpiApply;
+    g.c[0] = a;
+    g.c[1] = (float)(1.0 / sb);
+    g.c[2] = 1.f;
+    return g;
+}
+
+static int ortho_tiled_fwd(const OrthoPlan &p, const OrthoCoefficients &co, long long nb, const OrthoSource &src,
+                           void *y, int dtype, const MuonTable &tab, float eps, char *scratch, cudaStream_t stream) {
+    Carver ws{scratch};
+    OrthoPlanes x[2] = {ws.planes(nb, p.px, p.ldx), ws.planes(nb, p.px, p.ldx)};
+    const OrthoPlanes a = ws.planes(nb, p.pa, p.lda), b = ws.planes(nb, p.pa, p.lda);
+    float *da = ws.take<float>((size_t)nb * p.m), *db = ws.take<float>((size_t)nb * p.m);
+    double *partial = ws.take<double>((size_t)nb * p.chunks);
+    float *norms = ws.take<float>(nb);
+    const MuonTable *t = tab.n > 0 ? &tab : nullptr;
+    if (int e = run_split(p, nb, src, tab, (float)p.s.x, eps, norms, partial, x[0], stream)) return e;
+    for (int k = 0; k < co.steps; ++k) {
+        const OrthoPlanes &from = x[k & 1];
+        if (int e = run_poly(p, nb, co.c[k], p.s.b, from, a, b, da, db, t, stream)) return e;
+        OrthoGemm g = apply_gemm(p, nb, co.c[k][0], p.s.b, from, b, db);
+        if (k + 1 < co.steps) {
+            g.out = x[(k + 1) & 1];
+        } else {
+            g.epilogue = t ? kEpiMuon : kEpiOut;
+            g.c[2] = (float)(1.0 / p.s.x);
+            g.y = y;
+            g.dtype = dtype;
+        }
+        if (int e = ortho_gemm(g, t, stream)) return e;
+    }
+    return kOk;
+}
+
+// The steps again, each one's X, A and B kept, and then back through them:
+//     S = G X^T + X G^T,  T = b S + c (S A + A S),  G <- a G + B G + T X.
+// G's scale falls by the power of two above the largest slope |p'| at each
+// step, which bounds how far its norm can grow; it is measured anew before
+// that has cost it its low bits.
+static int ortho_tiled_bwd(const OrthoPlan &p, const OrthoCoefficients &co, long long nb, const OrthoSource &src,
+                           const OrthoSource &v, void *v_x, int dtype, float eps, char *scratch, cudaStream_t stream) {
+    const int K = co.steps;
+    Carver ws{scratch};
+    OrthoBuffers w;
+    for (int k = 0; k < K; ++k) {
+        w.x[k] = ws.planes(nb, p.px, p.ldx);
+        w.a[k] = ws.planes(nb, p.pa, p.lda);
+        w.b[k] = ws.planes(nb, p.pa, p.lda);
+        w.da[k] = ws.take<float>((size_t)nb * p.m);
+        w.db[k] = ws.take<float>((size_t)nb * p.m);
+    }
+    OrthoPlanes gr[2] = {ws.planes(nb, p.px, p.ldx), ws.planes(nb, p.px, p.ldx)};
+    const OrthoPlanes s = ws.planes(nb, p.pa, p.lda), t = ws.planes(nb, p.pa, p.lda);
+    double *partial = ws.take<double>((size_t)nb * p.chunks);
+    float *norms = ws.take<float>(nb), *factor[2] = {ws.take<float>(nb), ws.take<float>(nb)};
+    const MuonTable none = {};
+    const double shrink = std::exp2(std::ceil(std::log2(p.s.slope)));
+    // both products of G's step accumulate together: (B's scale)(G's) = (T's)(X's).
+    // With |G| scaled to at most kPlaneTop, T's scaled bound is worst_t kPlaneTop sb / sx.
+    const double sb = std::fmin(p.s.b, pow2_floor(p.s.x / p.s.worst_t));
+    if (int e = run_split(p, nb, src, none, (float)p.s.x, eps, norms, partial, w.x[0], stream)) return e;
+    for (int k = 0; k < K; ++k) {
+        if (int e = run_poly(p, nb, co.c[k], sb, w.x[k], w.a[k], w.b[k], w.da[k], w.db[k], nullptr, stream)) return e;
+        if (k + 1 == K) break;
+        OrthoGemm g = apply_gemm(p, nb, co.c[k][0], sb, w.x[k], w.b[k], w.db[k]);
+        g.out = w.x[k + 1];
+        if (int e = ortho_gemm(g, nullptr, stream)) return e;
+    }
+    if (int e = run_split(p, nb, v, none, (float)kPlaneTop, 0.f, factor[0], partial, gr[K & 1], stream)) return e;
+    double grown = 1.0; // G's scale has fallen by this
+    for (int k = K - 1; k >= 0; --k) {
+        const OrthoPlanes &from = gr[(k + 1) & 1], &to = gr[k & 1];
+        // scaled G is at most kPlaneTop, so S is at most 2 top kPlaneTop sx before its own scale
+        const double ss = pow2_floor(1.0 / (2.0 * p.s.top));      // S's scale for G's scaled values
+        const double st = sb / p.s.x;                             // T's
+        OrthoGemm g = gemm_base(p, nb);
+        g.pairs = 2;
+        g.M = g.N = p.m;
+        g.K = p.n;
+        g.q_k_major = g.symmetric = 1;
+        g.p[0] = g.q[1] = from;
+        g.q[0] = g.p[1] = w.x[k];
+        g.epilogue = kEpiSym;
+        g.c[0] = (float)(ss / p.s.x);
+        g.out = s;
+        if (int e = ortho_gemm(g, nullptr, stream)) return e;
+        g.K = p.m;
+        g.p[0] = g.q[1] = g.e = s;
+        g.q[0] = g.p[1] = w.a[k];
+        g.epilogue = kEpiAnti;
+        g.diag_in = w.da[k];
+        g.c[0] = (float)(co.c[k][1] * st / ss);
+        g.c[1] = (float)(co.c[k][2] * st / ss);
+        g.c[2] = (float)(co.c[k][2] * st / (ss * p.s.a));
+        g.out = t;
+        if (int e = ortho_gemm(g, nullptr, stream)) return e;
+        OrthoGemm h = apply_gemm(p, nb, co.c[k][0], sb, from, w.b[k], w.db[k]);
+        h.pairs = 2;
+        h.p[1] = t;
+        h.q[1] = w.x[k];
+        h.c[2] = (float)(1.0 / shrink);
+        h.out = to;
+        if (int e = ortho_gemm(h, nullptr, stream)) return e;
+        grown /= shrink;
+        if (grown < 1.0 / 256 && k > 0) { // the bound is far off by now: measure the norm
+            ortho_dot_kernel<<<(unsigned)(nb * p.chunks), kNormThreads, 0, stream>>>(to, to, p.m, p.n, p.chunks, partial);
+            if (int e = check_launch("ortho_dot_kernel")) return e;
+            ortho_rescale_kernel<<<(unsigned)(nb * p.chunks), kNormThreads, 0, stream>>>(
+                to, p.m, p.n, p.chunks, partial, (float)kPlaneTop, factor[0], (float)grown, factor[1]);
+            if (int e = check_launch("ortho_rescale_kernel")) return e;
+            std::swap(factor[0], factor[1]);
+            grown = 1.0;
+        }
+    }
+    ortho_dot_kernel<<<(unsigned)(nb * p.chunks), kNormThreads, 0, stream>>>(gr[0], w.x[0], p.m, p.n, p.chunks, partial);
+    if (int e = check_launch("ortho_dot_kernel")) return e;
+    const int tr = (p.rows + kSplitTile - 1) / kSplitTile, tc = (p.cols + kSplitTile - 1) / kSplitTile;
+    ortho_grad_out_kernel<<<(unsigned)(nb * tr * tc), kNormThreads, 0, stream>>>(
+        gr[0], w.x[0], p.rows, p.cols, p.transposed, partial, p.chunks, norms, factor[0], (float)grown, (float)p.s.x, eps,
+        v_x, dtype, tr, tc);
+    return check_launch("ortho_grad_out_kernel");
+}
+
+static int check_common(const char *what, long long batch, int rows, int cols, int dtype, int steps,
+                        const float *coefficients, float eps, OrthoCoefficients *co) {
+    if (batch < 0 || rows < 0 || cols < 0) return set_error(kErrInvalidArgument, "%s: negative size", what);
+    if (dtype < kOrthoF32 || dtype > kOrthoF16) return set_error(kErrUnsupported, "%s: dtype %d", what, dtype);
+    if (steps < 1 || steps > kOrthoMaxSteps)
+        return set_error(kErrInvalidArgument, "%s: steps must be 1 to %d, got %d", what, kOrthoMaxSteps, steps);
+    if (coefficients == nullptr) return set_error(kErrInvalidArgument, "%s: no coefficients", what);
+    if (!(eps > 0.f)) return set_error(kErrInvalidArgument, "%s: eps must be positive", what);
+    co->steps = steps;
+    for (int k = 0; k < steps; ++k)
+        for (int j = 0; j < 3; ++j) {
+            co->c[k][j] = coefficients[3 * k + j];
+            if (!std::isfinite(co->c[k][j])) return set_error(kErrInvalidArgument, "%s: coefficient not finite", what);
+        }
+    const OrthoScales s = ortho_scales(*co);
+    if (!(s.top <= kOrthoMaxTop))
+        return set_error(kErrInvalidArgument, "%s: the polynomials take a singular value of 1 or less to %g; at most %g is held",
+                         what, s.top, kOrthoMaxTop);
+    return kOk;
+}
+
+static void finish_scales(OrthoPlan *p) {
+    OrthoScales &s = p->s;
+    s.x = pow2_floor(kPlaneTop / s.top);
+    s.a = pow2_floor(kPlaneTop / (s.top * s.top));
+    s.b = pow2_floor(kPlaneTop / std::fmax(s.top_b, 1.0));
+}
+
+static OrthoPlan make_plan(int rows, int cols, int dtype, const OrthoCoefficients &co, bool backward) {
+    OrthoPlan p = ortho_plan(rows, cols, dtype, co, backward);
+    finish_scales(&p);
+    return p;
+}
+
+static size_t plan_bytes(const OrthoPlan &p, long long batch) {
+    return (size_t)ortho_chunk(p, batch) * p.per_matrix + p.fixed;
+}
+
+} // namespace gsb
+
+using namespace gsb;
+
+extern "C" size_t gsb_orthogonalize_scratch_bytes(long long batch, int rows, int cols, int dtype, int steps, int backward) {
+    if (batch <= 0 || rows <= 0 || cols <= 0 || steps < 1 || steps > kOrthoMaxSteps || ortho_is_thin(rows, cols)) return 0;
+    OrthoCoefficients co = {};
+    co.steps = steps;
+    return plan_bytes(ortho_plan(rows, cols, dtype, co, backward != 0), batch);
+}
+
+static const char *at_matrix(const void *p, long long b, int rows, int cols, int dtype) {
+    return static_cast<const char *>(p) + (size_t)b * rows * cols * (dtype == kOrthoF32 ? 4 : 2);
+}
+
+extern "C" int gsb_orthogonalize_fwd(long long batch, int rows, int cols, int dtype, const void *x, void *y, int steps,
+                                     const float *coefficients, float eps, void *scratch, size_t scratch_bytes,
+                                     cudaStream_t stream) {
+    OrthoCoefficients co = {};
+    if (int e = check_common("orthogonalize", batch, rows, cols, dtype, steps, coefficients, eps, &co)) return e;
+    if (batch == 0 || rows == 0 || cols == 0) return kOk;
+    if (ortho_is_thin(rows, cols)) return ortho_thin_fwd(batch, rows, cols, dtype, x, y, co, eps, stream);
+    const OrthoPlan p = make_plan(rows, cols, dtype, co, false);
+    if (scratch == nullptr || scratch_bytes < plan_bytes(p, batch))
+        return set_error(kErrInvalidArgument, "orthogonalize: %zu scratch bytes are needed", plan_bytes(p, batch));
+    const long long chunk = ortho_chunk(p, batch);
+    const MuonTable none = {};
+    for (long long b = 0; b < batch; b += chunk) {
+        const OrthoSource src = {at_matrix(x, b, rows, cols, dtype), dtype};
+        if (int e = ortho_tiled_fwd(p, co, std::min(chunk, batch - b), src,
+                                    const_cast<char *>(at_matrix(y, b, rows, cols, dtype)), dtype, none, eps,
+                                    static_cast<char *>(scratch), stream))
+            return e;
+    }
+    return kOk;
+}
+
+extern "C" int gsb_orthogonalize_bwd(long long batch, int rows, int cols, int dtype, const void *x, const void *v_y,
+                                     void *v_x, int steps, const float *coefficients, float eps, void *scratch,
+                                     size_t scratch_bytes, cudaStream_t stream) {
+    OrthoCoefficients co = {};
+    if (int e = check_common("orthogonalize", batch, rows, cols, dtype, steps, coefficients, eps, &co)) return e;
+    if (batch == 0 || rows == 0 || cols == 0) return kOk;
+    if (ortho_is_thin(rows, cols)) return ortho_thin_bwd(batch, rows, cols, dtype, x, v_y, v_x, co, eps, stream);
+    const OrthoPlan p = make_plan(rows, cols, dtype, co, true);
+    if (scratch == nullptr || scratch_bytes < plan_bytes(p, batch))
+        return set_error(kErrInvalidArgument, "orthogonalize: %zu scratch bytes are needed", plan_bytes(p, batch));
+    const long long chunk = ortho_chunk(p, batch);
+    for (long long b = 0; b < batch; b += chunk) {
+        const OrthoSource src = {at_matrix(x, b, rows, cols, dtype), dtype}, v = {at_matrix(v_y, b, rows, cols, dtype), dtype};
+        if (int e = ortho_tiled_bwd(p, co, std::min(chunk, batch - b), src, v,
+                                    const_cast<char *>(at_matrix(v_x, b, rows, cols, dtype)), dtype, eps,
+                                    static_cast<char *>(scratch), stream))
+            return e;
+    }
+    return kOk;
+}
+
+// The matrices [from, from + n) of a table.
+static MuonTable table_part(const MuonTable &all, long long from, long long n, int rows, int cols) {
+    MuonTable t = all;
+    t.n = 0;
+    for (int i = 0; i < all.n; ++i) {
+        const long long lo = std::max(all.first[i], from), hi = std::min(all.first[i + 1], from + n);
+        if (lo >= hi) continue;
+        const long long skip = lo - all.first[i];
+        t.param[t.n] = const_cast<char *>(at_matrix(all.param[i], skip, rows, cols, all.dtype));
+        t.grad[t.n] = at_matrix(all.grad[i], skip, rows, cols, all.dtype);
+        t.momentum[t.n] = const_cast<char *>(at_matrix(all.momentum[i], skip, rows, cols, all.state_dtype));
+        t.lr[t.n] = all.lr[i];
+        t.decay[t.n] = all.decay[i];
+        t.inner[t.n] = all.inner[i];
+        t.skipped[t.n] = all.skipped[i] + skip;
+        t.first[t.n] = lo - from;
+        ++t.n;
+    }
+    t.first[t.n] = n;
+    return t;
+}
+
+extern "C" int gsb_muon(int n_tensors, const GsbMuonTensor *tensors, int rows, int cols, int dtype, int state_dtype,
+                        const bool *valid, float momentum, int nesterov, int steps, const float *coefficients, float eps,
+                        void *scratch, size_t scratch_bytes, cudaStream_t stream) {
+    OrthoCoefficients co = {};
+    if (int e = check_common("muon", 0, rows, cols, dtype, steps, coefficients, eps, &co)) return e;
+    if (state_dtype != dtype && state_dtype != kOrthoF32)
+        return set_error(kErrUnsupported, "muon: the momentum buffer has the parameter's type or float32");
+    if (n_tensors < 0) return set_error(kErrInvalidArgument, "muon: negative tensor count");
+    if (n_tensors > 0 && tensors == nullptr) return set_error(kErrInvalidArgument, "muon: no tensor list");
+    long long total = 0;
+    for (int i = 0; i < n_tensors; ++i) {
+        if (tensors[i].batch < 0 || tensors[i].inner < 1)
+            return set_error(kErrInvalidArgument, "muon: tensor %d: batch %lld, inner %d", i, tensors[i].batch, tensors[i].inner);
+        total += tensors[i].batch;
+    }
+    if (total == 0 || rows == 0 || cols == 0) return kOk;
+    const bool thin = ortho_is_thin(rows, cols);
+    OrthoPlan p = {};
+    if (!thin) {
+        p = make_plan(rows, cols, dtype, co, false);
+        if (scratch == nullptr || scratch_bytes < plan_bytes(p, total))
+            return set_error(kErrInvalidArgument, "muon: %zu scratch bytes are needed", plan_bytes(p, total));
+    }
+    for (int at = 0; at < n_tensors; at += kOrthoMaxTensors) {
+        MuonTable t = {};
+        t.dtype = dtype;
+        t.state_dtype = state_dtype;
+        t.nesterov = nesterov;
+        t.mu = momentum;
+        t.one_minus_mu = (float)(1.0 - (double)momentum);
+        t.valid = valid;
+        for (int i = at; i < n_tensors && i < at + kOrthoMaxTensors; ++i) {
+            if (tensors[i].batch == 0) continue;
+            t.param[t.n] = tensors[i].param;
+            t.grad[t.n] = tensors[i].grad;
+            t.momentum[t.n] = tensors[i].momentum_buffer;
+            t.lr[t.n] = tensors[i].lr;
+            t.decay[t.n] = tensors[i].decay;
+            t.inner[t.n] = tensors[i].inner;
+            t.first[t.n + 1] = t.first[t.n] + tensors[i].batch;
+            ++t.n;
+        }
+        if (t.n == 0) continue;
+        if (thin) {
+            if (int e = ortho_thin_muon(t, rows, cols, co, eps, stream)) return e;
+            continue;
+        }
+        const long long here = t.first[t.n], chunk = ortho_chunk(p, total);
+        for (long long b = 0; b < here; b += chunk) {
+            const long long n = std::min(chunk, here - b);
+            if (int e = ortho_tiled_fwd(p, co, n, OrthoSource{nullptr, dtype}, nullptr, dtype,
+                                        table_part(t, b, n, rows, cols), eps, static_cast<char *>(scratch), stream))
+                return e;
+        }
+    }
+    return kOk;
+}

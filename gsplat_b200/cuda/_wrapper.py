@@ -12,6 +12,7 @@ tests written against the reference run unchanged. Every op launches the
 hand-written sm_100a kernels of ``gsplat_b200/csrc``; there is no CPU path.
 """
 
+import ctypes
 import math
 import warnings
 from typing import Optional, Tuple
@@ -21,7 +22,7 @@ from torch import Tensor
 from typing_extensions import Literal
 
 from . import _backend as _B
-from ._backend import call, check_cuda, device_guard, ptr, stream_of
+from ._backend import call, check_cuda, device_guard, lib, ptr, stream_of
 
 CameraModel = Literal["pinhole", "ortho", "fisheye", "ftheta", "lidar"]
 _CAMERA_IDS = {"pinhole": 0, "ortho": 1, "fisheye": 2}
@@ -102,6 +103,181 @@ def adam_multi(groups, valid: Optional[Tensor], b1: float, b2: float) -> None:
     check_cuda("valid", valid)
     with device_guard(dev):
         call("gsb_adam_multi", len(groups), arr, ptr(valid), b1, b2, stream_of(groups[0][0]))
+
+
+# ---------------------------------------------------------------------------
+# Orthogonalised matrices and the Muon step
+# ---------------------------------------------------------------------------
+#: The polynomial a s + b s^3 + c s^5 of the Muon optimiser: steep at 0, so that five steps take
+#: singular values down to about 0.003 into [0.7, 1.2].
+MUON_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+_ORTHO_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _ortho_dtype(name: str, t: Tensor) -> int:
+    if t.dtype not in _ORTHO_DTYPES:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    return _ORTHO_DTYPES[t.dtype]
+
+
+def _ortho_coefficients(coefficients, steps: int):
+    """``coefficients`` (one (a, b, c) for every step, or a list of them) as a C array of steps triples."""
+    if not 1 <= steps <= 32:
+        raise ValueError(f"steps must be 1 to 32, got {steps}")
+    triples = list(coefficients)
+    if len(triples) == 3 and not any(isinstance(v, (list, tuple)) for v in triples):
+        triples = [triples] * steps
+    if len(triples) != steps or any(len(t) != 3 for t in triples):
+        raise ValueError(f"coefficients must be (a, b, c) or a list of steps = {steps} such triples")
+    flat = [float(v) for t in triples for v in t]
+    return (ctypes.c_float * len(flat))(*flat)
+
+
+def _ortho_scratch(batch: int, rows: int, cols: int, dtype: int, steps: int, backward: bool, device) -> Tensor:
+    size = lib().gsb_orthogonalize_scratch_bytes(batch, rows, cols, dtype, steps, int(backward))
+    return torch.empty(size, dtype=torch.uint8, device=device)
+
+
+def orthogonalize(
+    x: Tensor,  # [..., M, N]
+    steps: int = 5,
+    coefficients=MUON_COEFFICIENTS,
+    eps: float = 1e-7,
+) -> Tensor:
+    """Orthogonalises each matrix by Newton-Schulz steps (no counterpart in the reference).
+
+    X = x / max(|x|_F, eps), then ``steps`` (1 to 32) times A = X X^T, X = a X + (b A + c A A) X:
+    every singular value s becomes p(...p(s)) with p(s) = a s + b s^3 + c s^5. The default
+    coefficients bring all but the smallest near 1 in five steps; (1.5, -0.5, 0) converges to the orthogonal
+    factor itself. ``coefficients`` may also be a list with a triple for each step. Matrices are multiplied
+    with 22 significand bits, bfloat16 ones with a side above 128 with 11; the result has x's shape and type. Differentiable (once); a matrix with a NaN or an infinity becomes NaN, others of the batch are not touched
+    by it. Polynomials that take a singular value in [0, 1] above 16 are refused.
+    """
+    if x.dim() < 2:
+        raise ValueError(f"x must be [..., M, N], got {tuple(x.shape)}")
+    _ortho_dtype("x", x)
+    if not eps > 0:
+        raise ValueError(f"eps must be positive, got {eps}")
+    return _Orthogonalize.apply(x.contiguous(), steps, _ortho_coefficients(coefficients, steps), eps)
+
+
+class _Orthogonalize(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x: Tensor, steps: int, coefficients, eps: float) -> Tensor:
+        check_cuda("x", x)
+        rows, cols = x.shape[-2:]
+        batch = math.prod(x.shape[:-2])
+        dtype = _ORTHO_DTYPES[x.dtype]
+        y = torch.empty_like(x)
+        with device_guard(x.device):
+            scratch = _ortho_scratch(batch, rows, cols, dtype, steps, False, x.device)
+            call("gsb_orthogonalize_fwd", batch, rows, cols, dtype, ptr(x), ptr(y), steps, coefficients, eps,
+                 ptr(scratch), scratch.numel(), stream_of(x))
+        ctx.save_for_backward(x)
+        ctx.steps, ctx.coefficients, ctx.eps = steps, coefficients, eps
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, v_y: Tensor):
+        (x,) = ctx.saved_tensors
+        v_y = v_y.contiguous()
+        check_cuda("v_y", v_y)
+        rows, cols = x.shape[-2:]
+        batch = math.prod(x.shape[:-2])
+        dtype = _ORTHO_DTYPES[x.dtype]
+        v_x = torch.empty_like(x)
+        with device_guard(x.device):
+            scratch = _ortho_scratch(batch, rows, cols, dtype, ctx.steps, True, x.device)
+            call("gsb_orthogonalize_bwd", batch, rows, cols, dtype, ptr(x), ptr(v_y), ptr(v_x), ctx.steps,
+                 ctx.coefficients, ctx.eps, ptr(scratch), scratch.numel(), stream_of(x))
+        return v_x, None, None, None
+
+
+@torch.no_grad()
+def muon(
+    params,  # [M, N] or [B, ..., M, N], or a list of them
+    param_grads,
+    momentum_buffers,
+    valid: Optional[Tensor],  # [B]
+    lr,
+    momentum: float,
+    weight_decay: float = 0.0,
+    nesterov: bool = True,
+    steps: int = 5,
+    coefficients=MUON_COEFFICIENTS,
+    eps: float = 1e-7,
+) -> None:
+    """One Muon step, in place, of one tensor or of a list (``lr`` then one number or a list).
+
+    For every matrix: m += (1 - momentum) (grad - m); u = grad + momentum (m - grad) with
+    ``nesterov``, else m; param = param (1 - lr weight_decay) - lr ``orthogonalize(u)``. Gradients have
+    their parameter's type (float32, bfloat16 or float16), buffers that type or float32. As in :func:`adam`, ``valid``
+    masks the leading dimension, which all params then share (three dimensions or more): masked matrices keep their parameter
+    and momentum. Tensors of one shape and type go through the kernels together. A tensor must not be listed
+    twice or overlap another.
+    """
+    if isinstance(params, Tensor):
+        params, param_grads, momentum_buffers = [params], [param_grads], [momentum_buffers]
+    params, param_grads, momentum_buffers = list(params), list(param_grads), list(momentum_buffers)
+    lrs = [float(v) for v in lr] if isinstance(lr, (list, tuple)) else [float(lr)] * len(params)
+    if not len(params) == len(param_grads) == len(momentum_buffers) == len(lrs):
+        raise ValueError("params, param_grads, momentum_buffers and lr must have the same length")
+    if not 0.0 <= momentum < 1.0:
+        raise ValueError(f"momentum must be in [0, 1), got {momentum}")
+    if not eps > 0:
+        raise ValueError(f"eps must be positive, got {eps}")
+    coefficients = _ortho_coefficients(coefficients, steps)
+    if not params:
+        return
+    device = params[0].device
+    check_cuda("valid", valid)
+    if valid is not None and (valid.dtype != torch.bool or valid.dim() != 1 or valid.device != device):
+        raise ValueError("valid must be a bool tensor [B] on the params' device")
+    groups = {}
+    spans = []
+    for p, g, m, rate in zip(params, param_grads, momentum_buffers, lrs):
+        for name, t in (("param", p), ("param_grad", g), ("momentum_buffer", m)):
+            check_cuda(name, t)
+            if t.device != device:
+                raise ValueError("params, param_grads and momentum_buffers must be on one device")
+            if t.numel():
+                spans.append((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), t is g))
+        if p.dim() < 2 or g.shape != p.shape or m.shape != p.shape:
+            raise ValueError(f"param, param_grad and momentum_buffer must be [..., M, N] alike, got {tuple(p.shape)}, "
+                             f"{tuple(g.shape)}, {tuple(m.shape)}")
+        dtype = _ortho_dtype("param", p)
+        if g.dtype != p.dtype or m.dtype not in (p.dtype, torch.float32):
+            raise TypeError(f"param_grad must have the param's type and momentum_buffer that or float32, got {p.dtype}, "
+                            f"{g.dtype}, {m.dtype}")
+        if valid is not None and (p.dim() < 3 or p.shape[0] != valid.shape[0]):
+            raise ValueError(f"valid [{valid.shape[0]}] does not mask the leading dimension of {tuple(p.shape)}")
+        if p.numel() == 0:
+            continue
+        batch = math.prod(p.shape[:-2])
+        inner = batch // p.shape[0] if p.dim() > 2 else 1
+        groups.setdefault((p.shape[-2], p.shape[-1], dtype, _ORTHO_DTYPES[m.dtype]), []).append(
+            (p, g, m, batch, inner, rate))
+    read_end = write_end = 0
+    for start, end, read_only in sorted(spans):
+        if start < write_end or (not read_only and start < read_end):
+            raise ValueError("muon: tensors overlap")
+        if read_only:
+            read_end = max(read_end, end)
+        else:
+            write_end = max(write_end, end)
+    with device_guard(device):
+        for (rows, cols, dtype, state_dtype), entries in groups.items():
+            arr = (_B.GsbMuonTensor * len(entries))()
+            for i, (p, g, m, batch, inner, rate) in enumerate(entries):
+                arr[i] = _B.GsbMuonTensor(p.data_ptr(), g.data_ptr(), m.data_ptr(), batch, inner, rate,
+                                          1.0 - rate * weight_decay)
+            scratch = _ortho_scratch(sum(e[3] for e in entries), rows, cols, dtype, steps, False, device)
+            call("gsb_muon", len(entries), arr, rows, cols, dtype, state_dtype, ptr(valid), momentum, int(nesterov),
+                 steps, coefficients, eps, ptr(scratch), scratch.numel(), stream_of(params[0]))
+            for p, _, m, _, _, _ in entries:
+                torch.autograd.graph.increment_version((p, m))
 
 
 # ---------------------------------------------------------------------------

@@ -1,3 +1,4 @@
+from .muon import Muon
 from .selective_adam import SelectiveAdam
 
-__all__ = ["SelectiveAdam"]
+__all__ = ["Muon", "SelectiveAdam"]

@@ -1,0 +1,64 @@
+"""Muon: momentum whose matrices are orthogonalised before they are taken from the parameters.
+
+No counterpart in the reference; constructor arguments, state (``momentum_buffer``) and
+learning-rate rules are those of ``torch.optim.Muon``. Parameters may also be batches of matrices
+[B, ..., M, N] (the SH bands of N splats, [N, 15, 3], are N matrices), and ``step`` takes
+the visibility mask of ``SelectiveAdam`` for them. All parameters of one shape and type go through the
+kernels together (``gsb_muon``).
+"""
+
+import math
+
+import torch
+
+from ..cuda._wrapper import MUON_COEFFICIENTS, muon
+
+
+class Muon(torch.optim.Optimizer):
+    """``adjust_lr_fn`` scales the learning rate by the matrix's shape: None or ``"original"``:
+    sqrt(max(1, M / N)); ``"match_rms_adamw"``: 0.2 sqrt(max(M, N)), the root mean square of an Adam step.
+    ``momentum_dtype``: the type of the momentum buffers (None: the parameter's; or torch.float32)."""
+
+    def __init__(self, params, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True,
+                 ns_coefficients=MUON_COEFFICIENTS, eps=1e-7, ns_steps=5, adjust_lr_fn=None, momentum_dtype=None):
+        if lr < 0.0 or weight_decay < 0.0:
+            raise ValueError(f"lr and weight_decay must not be negative, got {lr}, {weight_decay}")
+        if adjust_lr_fn not in (None, "original", "match_rms_adamw"):
+            raise ValueError(f"adjust_lr_fn must be None, 'original' or 'match_rms_adamw', got {adjust_lr_fn!r}")
+        defaults = dict(lr=lr, weight_decay=weight_decay, momentum=momentum, nesterov=nesterov,
+                        ns_coefficients=ns_coefficients, eps=eps, ns_steps=ns_steps, adjust_lr_fn=adjust_lr_fn,
+                        momentum_dtype=momentum_dtype)
+        super().__init__(params, defaults)
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.dim() < 2:
+                    raise ValueError(f"Muon takes matrices [..., M, N], got a parameter {tuple(p.shape)}")
+
+    @torch.no_grad()
+    def step(self, visibility=None):
+        if visibility is not None:
+            visibility = visibility.contiguous()
+        for group in self.param_groups:
+            params, grads, buffers, lrs = [], [], [], []
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                state = self.state[p]
+                if "momentum_buffer" not in state:
+                    state["momentum_buffer"] = torch.zeros_like(p, dtype=group["momentum_dtype"],
+                                                                memory_format=torch.contiguous_format)
+                grad = p.grad
+                if grad.is_sparse:
+                    grad = grad.to_dense()
+                params.append(p)
+                grads.append(grad.contiguous())
+                buffers.append(state["momentum_buffer"])
+                lrs.append(group["lr"] * _shape_factor(group["adjust_lr_fn"], *p.shape[-2:]))
+            muon(params, grads, buffers, visibility, lrs, group["momentum"], group["weight_decay"], group["nesterov"],
+                 group["ns_steps"], group["ns_coefficients"], group["eps"])
+
+
+def _shape_factor(rule, rows: int, cols: int) -> float:
+    if rule == "match_rms_adamw":
+        return 0.2 * math.sqrt(max(rows, cols))
+    return math.sqrt(max(1.0, rows / cols)) if cols else 1.0

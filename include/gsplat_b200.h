@@ -458,6 +458,46 @@ GSB_API int gsb_adam(float *param, const float *grad, float *exp_avg, float *exp
 GSB_API int gsb_adam_multi(int n_groups, const GsbAdamGroup *groups, const bool *valid, float b1,
                    float b2, cudaStream_t stream);
 
+/* --- Orthogonalised matrices and the Muon step ------------------------------
+ * No counterpart in the reference. For matrices U [rows, cols] (dtype 0 float32,
+ * 1 bfloat16, 2 float16; `batch` of them, contiguous):
+ *   X0 = U / max(|U|_F, eps); for each of `steps` (1 to 32) triples (a, b, c) of
+ *   `coefficients` (host, [steps, 3]): A = X X^T, X <- a X + (b A + c A A) X
+ * (X transposed where rows > cols). Coefficients whose polynomials a s + b s^3 + c s^5 take
+ * a singular value in [0, 1] above 16 are refused. Matrices are multiplied with
+ * 22 significand bits; bfloat16 ones with a side above 128 with 11.
+ * gsb_orthogonalize_bwd: v_x = the gradient of x for the gradient v_y of y.
+ * gsb_muon: for the listed tensors, each a batch of matrices of one shape and
+ * type: m <- m + (1 - momentum)(grad - m); u = grad + momentum (m - grad) (nesterov)
+ * or m; param <- decay * param - lr * orthogonalized(u). momentum_buffer has
+ * the type of param or float32 (state_dtype). valid (optional): a row of a tensor's leading
+ * dimension (`inner` matrices) whose entry is false is neither read nor
+ * written. Tensors must not overlap.
+ * Scratch: gsb_orthogonalize_scratch_bytes of the whole batch (gsb_muon: the sum
+ * of the tensors' batches, backward = 0); 0 for thin matrices (one side <= 4, the
+ * other <= 128), which need none. Calls that may run at the same time need scratch of their own. */
+GSB_API size_t gsb_orthogonalize_scratch_bytes(long long batch, int rows, int cols, int dtype,
+                                       int steps, int backward);
+GSB_API int gsb_orthogonalize_fwd(long long batch, int rows, int cols, int dtype, const void *x,
+                          void *y, int steps, const float *coefficients, float eps, void *scratch,
+                          size_t scratch_bytes, cudaStream_t stream);
+GSB_API int gsb_orthogonalize_bwd(long long batch, int rows, int cols, int dtype, const void *x,
+                          const void *v_y, void *v_x, int steps, const float *coefficients,
+                          float eps, void *scratch, size_t scratch_bytes, cudaStream_t stream);
+typedef struct GsbMuonTensor {
+    void *param;
+    const void *grad;
+    void *momentum_buffer;
+    long long batch; /* matrices */
+    int inner;       /* matrices of one row of the leading dimension */
+    float lr;
+    float decay;     /* 1 - lr * weight_decay */
+} GsbMuonTensor;
+GSB_API int gsb_muon(int n_tensors, const GsbMuonTensor *tensors, int rows, int cols, int dtype,
+             int state_dtype, const bool *valid, float momentum, int nesterov, int steps,
+             const float *coefficients, float eps, void *scratch, size_t scratch_bytes,
+             cudaStream_t stream);
+
 /* --- Gaussian-sharded exchange (multi-GPU) ---------------------------------
  * Replace the column concatenation, split and id arithmetic around the
  * all-to-all of the reference's distributed rasterization

@@ -138,6 +138,7 @@ struct OrthoGemm {
     float *diag_out;         // [batch, M]
     void *y;                 // kEpiOut: [batch, rows, cols] of `dtype`
     int dtype, transposed;   // transposed: y / param are [N, M] in memory
+    int *error;              // set when a kernel's wait ran out; the last product then writes NaN
 };
 
 int ortho_gemm(const OrthoGemm &g, const MuonTable *table, cudaStream_t stream);

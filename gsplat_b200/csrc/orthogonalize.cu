@@ -58,7 +58,9 @@ __device__ __forceinline__ double block_sum(double v) {
 
 // Sums of squares of the chunks of each matrix, in 64 bits and a fixed order.
 __global__ void __launch_bounds__(kNormThreads)
-    ortho_norm_kernel(OrthoSource src, const __grid_constant__ MuonTable tab, size_t numel, int chunks, double *partial) {
+    ortho_norm_kernel(OrthoSource src, const __grid_constant__ MuonTable tab, size_t numel, int chunks, double *partial,
+                      int *error) {
+    if (blockIdx.x == 0 && threadIdx.x == 0 && error) *error = 0; // nothing has waited yet
     const long long b = blockIdx.x / chunks;
     const int chunk = (int)(blockIdx.x % chunks);
     const int t = tab.n > 0 ? muon_tensor_of(tab, b) : 0;
@@ -165,7 +167,7 @@ __global__ void __launch_bounds__(kNormThreads)
 __global__ void __launch_bounds__(kNormThreads)
     ortho_grad_out_kernel(OrthoPlanes g, OrthoPlanes x, int rows, int cols, int transposed, const double *partial,
                           int chunks, const float *norms, const float *g_factor, float g_scale, float x_scale, float eps,
-                          void *v_x, int dtype, int tiles_r, int tiles_c) {
+                          void *v_x, int dtype, int tiles_r, int tiles_c, const int *error) {
     __shared__ float tile[kSplitTile][kSplitTile + 1];
     const long long per = (long long)tiles_r * tiles_c;
     const long long b = blockIdx.x / per;
@@ -185,7 +187,7 @@ __global__ void __launch_bounds__(kNormThreads)
             const size_t gi = (size_t)b * g.stride + (size_t)i * g.ld + j, xi = (size_t)b * x.stride + (size_t)i * x.ld + j;
             const float gv = __half2float(g.hi[gi]) + __half2float(g.lo[gi]);
             const float xv = __half2float(x.hi[xi]) + __half2float(x.lo[xi]);
-            const float v = fmaf(-xv, along, gv) / g_scale / f / div;
+            const float v = *error ? NAN : fmaf(-xv, along, gv) / g_scale / f / div;
             if (transposed) tile[cx][r] = v;
             else tile[r][cx] = v;
         }
@@ -320,9 +322,9 @@ struct OrthoBuffers {
 };
 
 static int run_split(const OrthoPlan &p, long long nb, const OrthoSource &src, const MuonTable &tab, float scale,
-                     float eps, float *norm_out, double *partial, const OrthoPlanes &out, cudaStream_t stream) {
+                     float eps, float *norm_out, double *partial, const OrthoPlanes &out, int *error, cudaStream_t stream) {
     ortho_norm_kernel<<<(unsigned)(nb * p.chunks), kNormThreads, 0, stream>>>(src, tab, (size_t)p.rows * p.cols,
-                                                                             p.chunks, partial);
+                                                                             p.chunks, partial, error);
     if (int e = check_launch("ortho_norm_kernel")) return e;
     const int tr = (p.rows + kSplitTile - 1) / kSplitTile, tc = (p.cols + kSplitTile - 1) / kSplitTile;
     ortho_split_kernel<<<(unsigned)(nb * tr * tc), kNormThreads, 0, stream>>>(
@@ -330,8 +332,9 @@ static int run_split(const OrthoPlan &p, long long nb, const OrthoSource &src, c
     return check_launch("ortho_split_kernel");
 }
 
-static OrthoGemm gemm_base(const OrthoPlan &p, long long nb) {
+static OrthoGemm gemm_base(const OrthoPlan &p, long long nb, int *error) {
     OrthoGemm g = {};
+    g.error = error;
     g.batch = nb;
     g.pairs = 1;
     g.split = p.split;
@@ -342,8 +345,8 @@ static OrthoGemm gemm_base(const OrthoPlan &p, long long nb) {
 // A and its polynomial B of step k, from X_k.
 static int run_poly(const OrthoPlan &p, long long nb, const float c[3], double sb, const OrthoPlanes &x,
                     const OrthoPlanes &a, const OrthoPlanes &b, float *da, float *db, const MuonTable *tab,
-                    cudaStream_t stream) {
-    OrthoGemm g = gemm_base(p, nb);
+                    int *error, cudaStream_t stream) {
+    OrthoGemm g = gemm_base(p, nb, error);
     g.M = g.N = p.m;
     g.K = p.n;
     g.q_k_major = g.symmetric = 1;
@@ -370,8 +373,8 @@ static int run_poly(const OrthoPlan &p, long long nb, const float c[3], double s
 }
 
 static OrthoGemm apply_gemm(const OrthoPlan &p, long long nb, float a, double sb, const OrthoPlanes &x,
-                            const OrthoPlanes &b, const float *db) {
-    OrthoGemm g = gemm_base(p, nb);
+                            const OrthoPlanes &b, const float *db, int *error) {
+    OrthoGemm g = gemm_base(p, nb, error);
     g.M = g.K = p.m;
     g.N = p.n;
     g.p[0] = b;
@@ -392,12 +395,13 @@ static int ortho_tiled_fwd(const OrthoPlan &p, const OrthoCoefficients &co, long
     float *da = ws.take<float>((size_t)nb * p.m), *db = ws.take<float>((size_t)nb * p.m);
     double *partial = ws.take<double>((size_t)nb * p.chunks);
     float *norms = ws.take<float>(nb);
+    int *error = ws.take<int>(1);
     const MuonTable *t = tab.n > 0 ? &tab : nullptr;
-    if (int e = run_split(p, nb, src, tab, (float)p.s.x, eps, norms, partial, x[0], stream)) return e;
+    if (int e = run_split(p, nb, src, tab, (float)p.s.x, eps, norms, partial, x[0], error, stream)) return e;
     for (int k = 0; k < co.steps; ++k) {
         const OrthoPlanes &from = x[k & 1];
-        if (int e = run_poly(p, nb, co.c[k], p.s.b, from, a, b, da, db, t, stream)) return e;
-        OrthoGemm g = apply_gemm(p, nb, co.c[k][0], p.s.b, from, b, db);
+        if (int e = run_poly(p, nb, co.c[k], p.s.b, from, a, b, da, db, t, error, stream)) return e;
+        OrthoGemm g = apply_gemm(p, nb, co.c[k][0], p.s.b, from, b, db, error);
         if (k + 1 < co.steps) {
             g.out = x[(k + 1) & 1];
         } else {
@@ -432,27 +436,28 @@ static int ortho_tiled_bwd(const OrthoPlan &p, const OrthoCoefficients &co, long
     const OrthoPlanes s = ws.planes(nb, p.pa, p.lda), t = ws.planes(nb, p.pa, p.lda);
     double *partial = ws.take<double>((size_t)nb * p.chunks);
     float *norms = ws.take<float>(nb), *factor[2] = {ws.take<float>(nb), ws.take<float>(nb)};
+    int *error = ws.take<int>(1);
     const MuonTable none = {};
     const double shrink = std::exp2(std::ceil(std::log2(p.s.slope)));
     // both products of G's step accumulate together: (B's scale)(G's) = (T's)(X's).
     // With |G| scaled to at most kPlaneTop, T's scaled bound is worst_t kPlaneTop sb / sx.
     const double sb = std::fmin(p.s.b, pow2_floor(p.s.x / p.s.worst_t));
-    if (int e = run_split(p, nb, src, none, (float)p.s.x, eps, norms, partial, w.x[0], stream)) return e;
+    if (int e = run_split(p, nb, src, none, (float)p.s.x, eps, norms, partial, w.x[0], error, stream)) return e;
     for (int k = 0; k < K; ++k) {
-        if (int e = run_poly(p, nb, co.c[k], sb, w.x[k], w.a[k], w.b[k], w.da[k], w.db[k], nullptr, stream)) return e;
+        if (int e = run_poly(p, nb, co.c[k], sb, w.x[k], w.a[k], w.b[k], w.da[k], w.db[k], nullptr, error, stream)) return e;
         if (k + 1 == K) break;
-        OrthoGemm g = apply_gemm(p, nb, co.c[k][0], sb, w.x[k], w.b[k], w.db[k]);
+        OrthoGemm g = apply_gemm(p, nb, co.c[k][0], sb, w.x[k], w.b[k], w.db[k], error);
         g.out = w.x[k + 1];
         if (int e = ortho_gemm(g, nullptr, stream)) return e;
     }
-    if (int e = run_split(p, nb, v, none, (float)kPlaneTop, 0.f, factor[0], partial, gr[K & 1], stream)) return e;
+    if (int e = run_split(p, nb, v, none, (float)kPlaneTop, 0.f, factor[0], partial, gr[K & 1], nullptr, stream)) return e;
     double grown = 1.0; // G's scale has fallen by this
     for (int k = K - 1; k >= 0; --k) {
         const OrthoPlanes &from = gr[(k + 1) & 1], &to = gr[k & 1];
         // scaled G is at most kPlaneTop, so S is at most 2 top kPlaneTop sx before its own scale
         const double ss = pow2_floor(1.0 / (2.0 * p.s.top));      // S's scale for G's scaled values
         const double st = sb / p.s.x;                             // T's
-        OrthoGemm g = gemm_base(p, nb);
+        OrthoGemm g = gemm_base(p, nb, error);
         g.pairs = 2;
         g.M = g.N = p.m;
         g.K = p.n;
@@ -473,7 +478,7 @@ static int ortho_tiled_bwd(const OrthoPlan &p, const OrthoCoefficients &co, long
         g.c[2] = (float)(co.c[k][2] * st / (ss * p.s.a));
         g.out = t;
         if (int e = ortho_gemm(g, nullptr, stream)) return e;
-        OrthoGemm h = apply_gemm(p, nb, co.c[k][0], sb, from, w.b[k], w.db[k]);
+        OrthoGemm h = apply_gemm(p, nb, co.c[k][0], sb, from, w.b[k], w.db[k], error);
         h.pairs = 2;
         h.p[1] = t;
         h.q[1] = w.x[k];
@@ -496,7 +501,7 @@ static int ortho_tiled_bwd(const OrthoPlan &p, const OrthoCoefficients &co, long
     const int tr = (p.rows + kSplitTile - 1) / kSplitTile, tc = (p.cols + kSplitTile - 1) / kSplitTile;
     ortho_grad_out_kernel<<<(unsigned)(nb * tr * tc), kNormThreads, 0, stream>>>(
         gr[0], w.x[0], p.rows, p.cols, p.transposed, partial, p.chunks, norms, factor[0], (float)grown, (float)p.s.x, eps,
-        v_x, dtype, tr, tc);
+        v_x, dtype, tr, tc, error);
     return check_launch("ortho_grad_out_kernel");
 }
 

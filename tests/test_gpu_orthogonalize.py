@@ -12,7 +12,8 @@ pytestmark = pytest.mark.gpu
 
 FLOATS = [torch.float32, torch.bfloat16, torch.float16]
 # both sides of every kernel's limits, odd sizes, tall and wide, one row, one column
-SHAPES = [(1, 1, 1), (3, 1, 7), (2, 7, 1), (1, 1, 300), (5, 2, 3), (70, 3, 3), (33, 15, 3), (9, 3, 16), (4, 4, 128),
+MANY = [(8200, 1, 1), (9000, 3, 3), (8193, 15, 3), (8300, 2, 7), (8195, 4, 25), (8200, 32, 2), (8200, 4, 33), (8192, 16, 4)]
+SHAPES = MANY + [(1, 1, 1), (3, 1, 7), (2, 7, 1), (1, 1, 300), (5, 2, 3), (70, 3, 3), (33, 15, 3), (9, 3, 16), (4, 4, 128),
           (2, 129, 4), (3, 5, 5), (2, 5, 131), (2, 64, 64), (1, 64, 35), (2, 100, 128), (1, 128, 128), (2, 128, 129),
           (1, 129, 127), (2, 257, 65), (1, 300, 300), (1, 130, 517), (1, 513, 384)]
 
@@ -208,7 +209,7 @@ def check_step(p, g, m, got_p, got_m, valid, lr, mu, wd, nesterov):
 @pytest.mark.parametrize("dtype,state", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16),
                                          (torch.bfloat16, torch.float32), (torch.float16, torch.float32),
                                          (torch.float16, torch.float16)])
-@pytest.mark.parametrize("shape", [(1, 1), (41, 3), (7, 15, 3), (3, 4, 20), (64, 35), (2, 3, 30, 40), (200, 140), (3, 150, 300)])
+@pytest.mark.parametrize("shape", [(8200, 15, 3), (2, 4100, 4, 9), (9001, 3, 30), (1, 1), (41, 3), (7, 15, 3), (3, 4, 20), (64, 35), (2, 3, 30, 40), (200, 140), (3, 150, 300)])
 @pytest.mark.parametrize("nesterov", [True, False])
 def test_muon(shape, dtype, state, nesterov):
     p, g, m = data(shape, dtype, 20, 0.02), data(shape, dtype, 21, 1e-2), data(shape, state, 22, 1e-2)
@@ -218,7 +219,7 @@ def test_muon(shape, dtype, state, nesterov):
     check_step(p, g, m, tp.cpu(), tm.cpu(), None, 0.03, 0.95, 0.1, nesterov)
 
 
-@pytest.mark.parametrize("shape", [(67, 15, 3), (40, 2, 3, 8), (12, 20, 30), (5, 140, 150)])
+@pytest.mark.parametrize("shape", [(8300, 15, 3), (4200, 2, 3, 8), (67, 15, 3), (40, 2, 3, 8), (12, 20, 30), (5, 140, 150)])
 def test_muon_valid(shape):
     p, g, m = (data(shape, torch.float32, s, 0.02) for s in (23, 24, 25))
     gen = torch.Generator().manual_seed(0)

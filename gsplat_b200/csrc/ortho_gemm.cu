@@ -11,6 +11,7 @@
 #include <cuda.h>
 
 #include "ortho.cuh"
+#include "tcgen05.cuh"
 
 namespace gsb {
 
@@ -21,7 +22,6 @@ constexpr int kChunk = 8;          // stages between two readings of the accumul
 constexpr int kEpilogueWarps = 8;  // four lane quarters x two column halves
 constexpr int kGemmThreads = 32 * (kEpilogueWarps + 2);
 constexpr int kTmemColumns = 2 * kBN;
-constexpr unsigned kWaitLimit = 1u << 22; // polls of about a microsecond at most
 
 struct GemmMaps {
     CUtensorMap p_hi[2], p_lo[2], q_hi[2], q_lo[2];
@@ -34,71 +34,11 @@ struct GemmShared {
     int abort;
 };
 
-__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-__device__ __forceinline__ void mbar_init(unsigned long long *b, int count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(b)), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(unsigned long long *b) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(b)) : "memory");
-}
-__device__ __forceinline__ void mbar_expect(unsigned long long *b, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(b)), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ bool mbar_try(unsigned long long *b, uint32_t phase) {
-    uint32_t done;
-    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}"
-                 : "=r"(done)
-                 : "r"(smem_u32(b)), "r"(phase), "r"(1000u)
-                 : "memory");
-    return done != 0;
-}
-// False when the wait ran out, here or in another role of the block.
-__device__ __forceinline__ bool mbar_wait(unsigned long long *b, uint32_t phase, volatile int *abort) {
-    for (unsigned i = 0; i < kWaitLimit; ++i) {
-        if (mbar_try(b, phase)) return true;
-        if (*abort) return false;
-    }
-    *abort = 1;
-    return false;
-}
-
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, int x, int y, int z,
                                          unsigned long long *bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
                  "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
                  : "memory");
-}
-
-__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
-    asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-                 "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
-                 : "memory");
-}
-__device__ __forceinline__ void mma_commit(unsigned long long *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-
-__device__ __forceinline__ void tmem_load32(uint32_t addr, float v[32]) {
-    uint32_t *r = reinterpret_cast<uint32_t *>(v);
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
-                 "tcgen05.wait::ld.sync.aligned;" // in one statement: nothing that uses v comes between
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-                   "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-                 : "r"(addr)
-                 : "memory");
-}
-
-// Shared-memory descriptor of a 128-byte-swizzled operand. Depth-major (K-major):
-// rows of 128 bytes, groups of 8 rows 1024 bytes apart. Row-major the other way
-// (N-major): 64 columns x 8 depths a 1024-byte group, the next 64 columns 8 KiB on.
-__device__ __forceinline__ uint64_t operand_desc(uint32_t addr, bool k_major) {
-    const uint64_t lbo = k_major ? 1 : 64 * 128 / 16, sbo = 1024 / 16;
-    return (uint64_t)((addr & 0x3ffff) >> 4) | lbo << 16 | sbo << 32 | 1ull << 46 | 2ull << 61;
 }
 
 // Eight values of a row of planes; past the row's 8-column groups, zeros.
@@ -321,7 +261,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     } else if (warp == kEpilogueWarps + 1) {
         // the products
         if (lane == 0) {
-            const uint32_t idesc = 1u << 4 | (g.q_k_major ? 0u : 1u << 16) | (uint32_t)(kBN / 8) << 17 | (uint32_t)(kBM / 16) << 24;
+            const uint32_t idesc = mma_desc(kBN, g.q_k_major);
             const uint32_t q_step = g.q_k_major ? 32 / 16 : 2048 / 16; // 16 deep, in the descriptor's units
             int stage = 0, acc = 0;
             uint32_t phase = 0, acc_phase = 0;
@@ -340,8 +280,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                         if (!ok) break;
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                         const uint32_t src = stage0 + stage * kStageBytes;
-                        const uint64_t p = operand_desc(src, true);
-                        const uint64_t q = operand_desc(src + (SPLIT ? 2 : 1) * kPlaneBytes, g.q_k_major);
+                        const uint64_t p = operand_desc(src, true, 0);
+                        const uint64_t q = operand_desc(src + (SPLIT ? 2 : 1) * kPlaneBytes, g.q_k_major, kPlaneBytes / 2);
                         const uint64_t lo = kPlaneBytes / 16; // from hi to lo
 #pragma unroll
                         for (int k = 0; k < kBK / 16; ++k) {
@@ -376,7 +316,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             if (tab.n > 0 && !muon_visible(tab, tensor, at.b)) continue;
             float v[64];
             for (int s0 = 0; s0 < total; s0 += chunk) {
-                ok = mbar_wait(&sh.acc_full[acc], acc_phase, abort);
+                ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[acc], acc_phase, abort));
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t src = tmem + ((uint32_t)(32 * (warp % 4)) << 16) + acc * kBN + half * 64;

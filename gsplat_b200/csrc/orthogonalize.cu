@@ -549,6 +549,7 @@ using namespace gsb;
 
 extern "C" size_t gsb_orthogonalize_scratch_bytes(long long batch, int rows, int cols, int dtype, int steps, int backward) {
     if (batch <= 0 || rows <= 0 || cols <= 0 || steps < 1 || steps > kOrthoMaxSteps || ortho_is_thin(rows, cols)) return 0;
+    if (!backward && ortho_is_clustered(rows, cols)) return 0;
     OrthoCoefficients co = {};
     co.steps = steps;
     return plan_bytes(ortho_plan(rows, cols, dtype, co, backward != 0), batch);
@@ -566,6 +567,8 @@ extern "C" int gsb_orthogonalize_fwd(long long batch, int rows, int cols, int dt
     if (batch == 0 || rows == 0 || cols == 0) return kOk;
     if (ortho_is_thin(rows, cols)) return ortho_thin_fwd(batch, rows, cols, dtype, x, y, co, eps, stream);
     const OrthoPlan p = make_plan(rows, cols, dtype, co, false);
+    if (ortho_is_clustered(rows, cols))
+        return ortho_cluster_fwd(batch, rows, cols, dtype, x, y, co, (float)p.s.x, (float)p.s.a, (float)p.s.b, eps, stream);
     if (scratch == nullptr || scratch_bytes < plan_bytes(p, batch))
         return set_error(kErrInvalidArgument, "orthogonalize: %zu scratch bytes are needed", plan_bytes(p, batch));
     const long long chunk = ortho_chunk(p, batch);
@@ -639,11 +642,11 @@ extern "C" int gsb_muon(int n_tensors, const GsbMuonTensor *tensors, int rows, i
         total += tensors[i].batch;
     }
     if (total == 0 || rows == 0 || cols == 0) return kOk;
-    const bool thin = ortho_is_thin(rows, cols);
+    const bool thin = ortho_is_thin(rows, cols), clustered = !thin && ortho_is_clustered(rows, cols);
     OrthoPlan p = {};
     if (!thin) {
         p = make_plan(rows, cols, dtype, co, false);
-        if (scratch == nullptr || scratch_bytes < plan_bytes(p, total))
+        if (!clustered && (scratch == nullptr || scratch_bytes < plan_bytes(p, total)))
             return set_error(kErrInvalidArgument, "muon: %zu scratch bytes are needed", plan_bytes(p, total));
     }
     for (int at = 0; at < n_tensors; at += kOrthoMaxTensors) {
@@ -668,6 +671,10 @@ extern "C" int gsb_muon(int n_tensors, const GsbMuonTensor *tensors, int rows, i
         if (t.n == 0) continue;
         if (thin) {
             if (int e = ortho_thin_muon(t, rows, cols, co, eps, stream)) return e;
+            continue;
+        }
+        if (clustered) {
+            if (int e = ortho_cluster_muon(t, rows, cols, co, (float)p.s.x, (float)p.s.a, (float)p.s.b, eps, stream)) return e;
             continue;
         }
         const long long here = t.first[t.n], chunk = ortho_chunk(p, total);

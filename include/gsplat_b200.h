@@ -474,8 +474,7 @@ GSB_API int gsb_adam_multi(int n_groups, const GsbAdamGroup *groups, const bool 
  * dimension (`inner` matrices) whose entry is false is neither read nor
  * written. Tensors must not overlap.
  * Scratch: gsb_orthogonalize_scratch_bytes of the whole batch (gsb_muon: the sum
- * of the tensors' batches, backward = 0); 0 for thin matrices (one side <= 4, the
- * other <= 128), which need none. Calls that may run at the same time need scratch of their own. */
+ * of the tensors' batches, backward = 0); 0 where none is needed. Calls that may run at the same time need scratch of their own. */
 GSB_API size_t gsb_orthogonalize_scratch_bytes(long long batch, int rows, int cols, int dtype,
                                        int steps, int backward);
 GSB_API int gsb_orthogonalize_fwd(long long batch, int rows, int cols, int dtype, const void *x,

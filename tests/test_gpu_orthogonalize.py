@@ -15,7 +15,8 @@ FLOATS = [torch.float32, torch.bfloat16, torch.float16]
 MANY = [(8200, 1, 1), (9000, 3, 3), (8193, 15, 3), (8300, 2, 7), (8195, 4, 25), (8200, 32, 2), (8200, 4, 33), (8192, 16, 4)]
 SHAPES = MANY + [(1, 1, 1), (3, 1, 7), (2, 7, 1), (1, 1, 300), (5, 2, 3), (70, 3, 3), (33, 15, 3), (9, 3, 16), (4, 4, 128),
           (2, 129, 4), (3, 5, 5), (2, 5, 131), (2, 64, 64), (1, 64, 35), (2, 100, 128), (1, 128, 128), (2, 128, 129),
-          (1, 129, 127), (2, 257, 65), (1, 300, 300), (1, 130, 517), (1, 513, 384)]
+          (1, 129, 127), (3, 16, 16), (2, 17, 1000), (2, 1000, 77), (1, 100, 700), (1, 128, 1024),
+          (1, 1100, 128), (1, 5, 2300), (2, 48, 95), (2, 257, 65), (1, 300, 300), (1, 130, 517), (1, 513, 384)]
 
 
 def gs():

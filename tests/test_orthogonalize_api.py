@@ -79,9 +79,9 @@ def test_c_entry_points_refuse_before_any_launch():
     assert fwd(co=triples(*[(2.0, 0.0, 0.0)] * 5)) == -1 and b"32" in L.gsb_last_error()
     # the peak lies inside: 12 s - 12 s^3 is 0 at 1 and 4.6 at 0.58, and grows from there
     assert fwd(co=triples(*[(12.0, -12.0, 0.0)] * 5)) == -1
-    assert fwd() == -1 and b"scratch" in L.gsb_last_error()  # a matrix that is not thin needs some
+    assert fwd(rows=200, cols=200) == -1 and b"scratch" in L.gsb_last_error()
     assert fwd(batch=0) == 0 and fwd(rows=0) == 0 and fwd(cols=0) == 0
-    rc = L.gsb_orthogonalize_bwd(1, 8, 8, 0, None, None, None, 5, c, 1e-7, None, 0, None)
+    rc = L.gsb_orthogonalize_bwd(1, 200, 200, 0, None, None, None, 5, c, 1e-7, None, 0, None)
     assert rc == -1 and b"scratch" in L.gsb_last_error()
     assert L.gsb_muon(1, None, 8, 8, 0, 0, None, 0.9, 1, 5, c, 1e-7, None, 0, None) == -1
     assert b"no tensor list" in L.gsb_last_error()
@@ -94,7 +94,8 @@ def test_scratch_sizes():
     L = lib()
     size = L.gsb_orthogonalize_scratch_bytes
     assert size(1000000, 15, 3, 0, 5, 0) == 0 and size(10, 3, 128, 1, 5, 1) == 0  # thin
-    assert size(10, 3, 129, 0, 5, 0) > 0 and size(0, 64, 64, 0, 5, 0) == 0
+    assert size(10, 64, 64, 0, 5, 0) == 0 and size(10, 64, 64, 0, 5, 1) > 0  # on chip, forward
+    assert size(10, 129, 129, 0, 5, 0) > 0 and size(0, 200, 200, 0, 5, 0) == 0
     assert size(1, 512, 256, 0, 5, 0) == size(1, 256, 512, 0, 5, 0)
     assert size(1, 256, 256, 0, 5, 1) > size(1, 256, 256, 0, 5, 0)
     # a large batch is taken in pieces: the scratch stays near 1 GiB

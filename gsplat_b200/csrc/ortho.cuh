@@ -36,6 +36,37 @@ template <> __device__ __forceinline__ float from_f32<float>(float v) { return v
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
+// Four values of a type at a 4-value boundary.
+template <typename T> struct Quad;
+template <> struct Quad<float> {
+    using type = float4;
+    static __device__ __forceinline__ float4 get(float4 v) { return v; }
+    static __device__ __forceinline__ float4 put(float4 f) { return f; }
+};
+template <> struct Quad<__half> {
+    using type = uint2;
+    static __device__ __forceinline__ float4 get(uint2 v) {
+        const float2 a = __half22float2(*reinterpret_cast<__half2 *>(&v.x)), b = __half22float2(*reinterpret_cast<__half2 *>(&v.y));
+        return make_float4(a.x, a.y, b.x, b.y);
+    }
+    static __device__ __forceinline__ uint2 put(float4 f) {
+        const __half2 a = __floats2half2_rn(f.x, f.y), b = __floats2half2_rn(f.z, f.w);
+        return make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+    }
+};
+template <> struct Quad<__nv_bfloat16> {
+    using type = uint2;
+    static __device__ __forceinline__ float4 get(uint2 v) {
+        const float2 a = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162 *>(&v.x)),
+                     b = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162 *>(&v.y));
+        return make_float4(a.x, a.y, b.x, b.y);
+    }
+    static __device__ __forceinline__ uint2 put(float4 f) {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(f.x, f.y), b = __floats2bfloat162_rn(f.z, f.w);
+        return make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+    }
+};
+
 // One value of a type known at run time (uniform over the launch).
 __device__ __forceinline__ float load_as_f32(const void *p, size_t i, int dtype) {
     if (dtype == kOrthoF32) return static_cast<const float *>(p)[i];

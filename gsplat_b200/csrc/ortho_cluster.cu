@@ -32,8 +32,15 @@ struct ClusterShape {
     int m16, mk, ns, ns64;  // rounded up: m to 16 and 64, a block's columns to 16 and 64
     int blocks, columns;    // of a cluster; of TMEM
     int slack;              // bytes behind the planes that a 128-row operand may touch
-    float x_scale, a_scale, b_scale;
+    int per;                // rows of A that a block of a cluster adds up
+    float x_scale, to_a, to_d, unscale_b, unscale_x;
     size_t smem;
+};
+
+// The constants of a step: X <- a X + B X; B = c0 .. of A as kEpiSquare of OrthoGemm has it.
+struct ClusterSteps {
+    int n;
+    float c[kOrthoMaxSteps][7]; // a, c0, c1, c2, c3, c4, c5
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -49,11 +56,6 @@ __device__ __forceinline__ uint32_t remote(uint32_t addr, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
-__device__ __forceinline__ float4 remote_load4(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-    return v;
-}
 __device__ __forceinline__ double remote_load_f64(uint32_t addr) {
     double v;
     asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(addr) : "memory");
@@ -66,7 +68,7 @@ __device__ __forceinline__ void remote_store_f32(uint32_t addr, float v) {
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 // Shared memory written by threads is read by the tensor cores after this and a barrier.
-__device__ __forceinline__ void async_proxy_fence() { asm volatile("fence.proxy.async;" ::: "memory"); }
+__device__ __forceinline__ void async_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // Byte of (row, column) in a plane of `rows` rows: blocks of 64 columns, rows of 128 bytes
 // whose 16-byte pieces are permuted by the row.
@@ -110,34 +112,35 @@ __device__ __forceinline__ void planes_put16(char *hi, char *lo, int rows, int r
     }
 }
 
-// One thread: D[128, n] = P Q over `depth`, hi and lo planes of both; P and Q depth-major from their
+// One warp: D[128, n] = P Q over `depth`, hi and lo planes of both; P and Q depth-major from their
 // first row (X X^T, A A), or Q column-major (B X). `rows`: of the planes.
 __device__ __forceinline__ void multiply(uint32_t d, uint32_t p, uint32_t p_lo, uint32_t q, uint32_t q_lo, int rows_p,
-                                         int rows_q, bool q_k_major, int n, int depth) {
+                                         int rows_q, bool q_k_major, int n, int depth, uint32_t leader) {
     const uint32_t idesc = mma_desc(n, q_k_major);
     const uint32_t chunk_p = rows_p * 128, chunk_q = rows_q * 128;
-    for (int k = 0; k < depth; k += 16) {
-        const uint32_t po = (k >> 6) * chunk_p + ((k >> 4) & 3) * 32;
-        const uint32_t qo = q_k_major ? (k >> 6) * chunk_q + ((k >> 4) & 3) * 32 : k * 128;
-        const uint64_t ph = operand_desc(p + po, true, 0), pl = operand_desc(p_lo + po, true, 0);
-        const uint64_t qh = operand_desc(q + qo, q_k_major, chunk_q), ql = operand_desc(q_lo + qo, q_k_major, chunk_q);
-        mma_f16(d, ph, qh, idesc, k > 0);
-        mma_f16(d, ph, ql, idesc, true);
-        mma_f16(d, pl, qh, idesc, true);
+    const uint64_t ph = operand_desc(p, true, 0), pl = operand_desc(p_lo, true, 0);
+    const uint64_t qh = operand_desc(q, q_k_major, chunk_q), ql = operand_desc(q_lo, q_k_major, chunk_q);
+    for (int k = 0; k < depth; k += 16) { // 16 bytes a unit of the descriptors' addresses
+        const uint32_t po = ((k >> 6) * chunk_p + ((k >> 4) & 3) * 32) >> 4;
+        const uint32_t qo = (q_k_major ? (k >> 6) * chunk_q + ((k >> 4) & 3) * 32 : k * 128) >> 4;
+        mma_f16(d, ph + po, qh + qo, idesc, k > 0, leader);
+        mma_f16(d, ph + po, ql + qo, idesc, true, leader);
+        mma_f16(d, pl + po, qh + qo, idesc, true, leader);
     }
 }
 
 template <typename T, typename M, bool MUON>
 __global__ void __launch_bounds__(kClusterThreads, 1)
     ortho_cluster_kernel(const __grid_constant__ ClusterShape sh, const T *x_in, T *y, const __grid_constant__ MuonTable tab,
-                         const __grid_constant__ OrthoCoefficients co, float eps) {
+                         const __grid_constant__ ClusterSteps co, float eps) {
     extern __shared__ char raw[];
-    __shared__ float diag_a[kClusterMaxShort], diag_b[kClusterMaxShort];
+    __shared__ alignas(16) float diag_a[kClusterMaxShort];
+    __shared__ float diag_b[kClusterMaxShort];
     __shared__ double warp_sum[kClusterThreads / 32], block_total;
     __shared__ alignas(8) unsigned long long done;
     __shared__ uint32_t tmem_at;
     __shared__ int abort_flag;
-    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+    const int tid = threadIdx.x, warp = uniform_warp(), lane = tid % 32;
     const uint32_t rank = sh.blocks > 1 ? cluster_rank() : 0;
     const long long b = blockIdx.x / sh.blocks;
     const int tensor = MUON ? muon_tensor_of(tab, b) : 0;
@@ -146,7 +149,7 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
     char *base = reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     const int x_plane = sh.m16 * sh.ns64 * 2, a_plane = sh.m16 * sh.mk * 2;
     char *x_hi = base, *x_lo = x_hi + x_plane, *a_hi = x_lo + x_plane, *a_lo = a_hi + a_plane;
-    float *partial = reinterpret_cast<float *>(a_lo + a_plane); // several blocks: [m16, m16 + 4]
+    float *partial = reinterpret_cast<float *>(a_lo + a_plane); // several blocks: [blocks, per, m16 + 4]
     const int pitch = sh.m16 + 4;
     volatile int *abort = &abort_flag;
 
@@ -155,14 +158,59 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
     const size_t mat = (size_t)(MUON ? b - tab.first[tensor] : b) * numel;
     const T *grad = MUON ? static_cast<const T *>(tab.grad[tensor]) + mat : x_in + mat;
     M *mom = MUON ? static_cast<M *>(tab.momentum[tensor]) + mat : nullptr;
-    // value e of the block's slab, in the tensor's order: its place there, its row and column here
+    // The slab is moved four values at a time where they lie together and are aligned. Move e of `moves`: its
+    // place in the tensor, the row and column of its first value here; with a transposed tensor the next values are
+    // further rows, at the last of which the next column begins.
     const int inner = sh.transposed ? sh.m : cols, count = sh.m * cols;
+    const uint32_t magic = inner > 1 ? 0xffffffffu / (uint32_t)inner + 1u : 0u;
+    const bool whole = sh.transposed || cols == sh.n; // the slab lies in one piece
+    bool quads = (whole || (sh.n % 4 == 0 && cols % 4 == 0)) && (whole ? (size_t)j0 * sh.m % 4 == 0 : true);
+    if (MUON) {
+        T *p = static_cast<T *>(tab.param[tensor]) + mat;
+        quads = quads && reinterpret_cast<uintptr_t>(grad) % (4 * sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(p) % (4 * sizeof(T)) == 0 &&
+                reinterpret_cast<uintptr_t>(mom) % (4 * sizeof(M)) == 0;
+    } else {
+        quads = quads && reinterpret_cast<uintptr_t>(grad) % (4 * sizeof(T)) == 0 &&
+                reinterpret_cast<uintptr_t>(y + mat) % (4 * sizeof(T)) == 0;
+    }
+    const int fours = quads ? count / 4 : 0, moves = fours + (count - 4 * fours);
     auto place = [&](int e, int &i, int &j) -> size_t {
-        const int o = e / inner, k = e - o * inner;
+        const int v = e < fours ? 4 * e : e + 3 * fours;
+        const int o = inner > 1 ? (int)__umulhi((uint32_t)v, magic) : v, k = v - o * inner;
         i = sh.transposed ? k : o;
         j = sh.transposed ? o : k;
-        return sh.transposed ? (size_t)(j0 + o) * sh.m + k : (size_t)o * sh.n + j0 + k;
+        return sh.transposed ? (size_t)j0 * sh.m + v : (size_t)o * sh.n + j0 + k;
     };
+    auto next = [&](int &i, int &j) {
+        if (sh.transposed) {
+            if (++i == sh.m) i = 0, ++j;
+        } else if (++j == cols) { // only where the slab is whole rows
+            j = 0, ++i;
+        }
+    };
+    using VT = typename Quad<T>::type;
+    using VM = typename Quad<M>::type;
+    // The matrix to orthogonalise at a move: one value in .x, or four.
+    auto fetch = [&](size_t at, bool four, float4 &m) -> float4 {
+        float4 g = {};
+        m = g;
+        if (four) {
+            g = Quad<T>::get(*reinterpret_cast<const VT *>(grad + at));
+            if (MUON) m = Quad<M>::get(*reinterpret_cast<const VM *>(mom + at));
+        } else {
+            g.x = to_f32(grad[at]);
+            if (MUON) m.x = to_f32(mom[at]);
+        }
+        return g;
+    };
+    auto updated = [&](float4 g, float4 &m) -> float4 {
+        if (!MUON) return g;
+        m.x = muon_momentum(g.x, m.x, tab.one_minus_mu), m.y = muon_momentum(g.y, m.y, tab.one_minus_mu);
+        m.z = muon_momentum(g.z, m.z, tab.one_minus_mu), m.w = muon_momentum(g.w, m.w, tab.one_minus_mu);
+        return make_float4(muon_update(g.x, m.x, tab.mu, tab.nesterov), muon_update(g.y, m.y, tab.mu, tab.nesterov),
+                           muon_update(g.z, m.z, tab.mu, tab.nesterov), muon_update(g.w, m.w, tab.mu, tab.nesterov));
+    };
+    constexpr int U = 4; // moves on their way at once
 
     if (tid == 0) {
         mbar_init(&done, 1);
@@ -180,20 +228,30 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
         reinterpret_cast<uint4 *>(base)[i] = make_uint4(0, 0, 0, 0);
     // the norm: sums in 64 bits, in a fixed order
     double s = 0.0;
-#pragma unroll 4
-    for (int e = tid; e < count; e += kClusterThreads) {
-        int i, j;
-        const size_t at = place(e, i, j);
-        float v = to_f32(grad[at]);
-        if (MUON) v = muon_update(v, muon_momentum(v, to_f32(mom[at]), tab.one_minus_mu), tab.mu, tab.nesterov);
-        s = fma((double)v, (double)v, s);
+    for (int e0 = tid; e0 < moves; e0 += U * kClusterThreads) {
+        float4 g[U], m[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int e = e0 + u * kClusterThreads;
+            int i, j;
+            g[u] = m[u] = make_float4(0, 0, 0, 0);
+            if (e < moves) g[u] = fetch(place(e, i, j), e < fours, m[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float4 w = updated(g[u], m[u]);
+            s = fma((double)w.x, (double)w.x, s);
+            s = fma((double)w.y, (double)w.y, s);
+            s = fma((double)w.z, (double)w.z, s);
+            s = fma((double)w.w, (double)w.w, s);
+        }
     }
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if (lane == 0) warp_sum[warp] = s;
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem = tmem_at;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_at, 0);
     s = 0.0;
     for (int w = 0; w < kClusterThreads / 32; ++w) s += warp_sum[w];
     if (sh.blocks > 1) {
@@ -203,21 +261,43 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
         for (int r = 0; r < sh.blocks; ++r) s += remote_load_f64(remote(smem_u32(&block_total), r));
     }
     const float norm = (float)sqrt(s), div = norm < eps ? eps : norm;
-#pragma unroll 4
-    for (int e = tid; e < count; e += kClusterThreads) {
-        int i, j;
-        const size_t at = place(e, i, j);
-        float v = to_f32(grad[at]);
-        if (MUON) {
-            const float m = muon_momentum(v, to_f32(mom[at]), tab.one_minus_mu);
-            mom[at] = from_f32<M>(m);
-            v = muon_update(v, m, tab.mu, tab.nesterov);
-        }
+    auto put = [&](int i, int j, float v) {
         v = v / div * sh.x_scale;
         const __half h = __float2half_rn(v);
         const uint32_t p = plane_byte(sh.m16, i, j);
         *reinterpret_cast<__half *>(x_hi + p) = h;
         *reinterpret_cast<__half *>(x_lo + p) = __float2half_rn(v - __half2float(h));
+    };
+    for (int e0 = tid; e0 < moves; e0 += U * kClusterThreads) {
+        float4 g[U], m[U];
+        size_t at[U];
+        int i[U], j[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int e = e0 + u * kClusterThreads;
+            if (e < moves) {
+                at[u] = place(e, i[u], j[u]);
+                g[u] = fetch(at[u], e < fours, m[u]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int e = e0 + u * kClusterThreads;
+            if (e >= moves) continue;
+            const float4 w = updated(g[u], m[u]);
+            put(i[u], j[u], w.x);
+            if (e < fours) {
+                if (MUON) *reinterpret_cast<VM *>(mom + at[u]) = Quad<M>::put(m[u]);
+                next(i[u], j[u]);
+                put(i[u], j[u], w.y);
+                next(i[u], j[u]);
+                put(i[u], j[u], w.z);
+                next(i[u], j[u]);
+                put(i[u], j[u], w.w);
+            } else if (MUON) {
+                mom[at[u]] = from_f32<M>(m[u].x);
+            }
+        }
     }
 
     const int row = 32 * (warp % 4) + lane, turn = warp / 4; // columns 16 (turn + 4 k) ..
@@ -226,6 +306,7 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
     const bool mine = row < sh.m16;
     const uint32_t xh = smem_u32(x_hi), xl = smem_u32(x_lo), ah = smem_u32(a_hi), al = smem_u32(a_lo);
     const int ns16 = (sh.ns + 15) / 16 * 16;
+    const uint32_t leader = elect_leader();
     uint32_t phase = 0;
     // what was written to shared memory is multiplied, and every thread waits for the product
     auto begin = [&] {
@@ -240,16 +321,17 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
         __syncwarp();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     };
-    for (int step = 0; step < co.steps; ++step) {
-        const float ca = co.c[step][0], cb = co.c[step][1], cc = co.c[step][2];
+    for (int step = 0; step < co.n; ++step) {
+        const float *cf = co.c[step];
         // A
         begin();
-        if (tid == 0) {
-            multiply(tmem, xh, xl, xh, xl, sh.m16, sh.m16, true, sh.m16, ns16);
-            mma_commit(&done);
+        if (warp == 0) {
+            multiply(tmem, xh, xl, xh, xl, sh.m16, sh.m16, true, sh.m16, ns16, leader);
+            mma_commit(&done, leader);
         }
+        const uint32_t owner = mine ? row / sh.per : 0; // of this row of A
+        const uint32_t to = sh.blocks > 1 ? remote(smem_u32(partial + ((int)rank * sh.per + row - (int)owner * sh.per) * pitch), owner) : 0u;
         finish();
-        const float to_a = sh.a_scale / (sh.x_scale * sh.x_scale), to_d = 1.f / (sh.x_scale * sh.x_scale);
         if (rows_here)
             for (int c = 16 * turn; c < sh.m16; c += 64) {
                 float v[16];
@@ -257,107 +339,122 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
                 tmem_load16(acc + c, v);
                 if (!mine) continue;
                 if (sh.blocks > 1) {
-                    float4 *p = reinterpret_cast<float4 *>(partial + row * pitch + c);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) p[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+                    for (int k = 0; k < 4; ++k)
+                        remote_store4(to + (c + 4 * k) * 4, make_uint4(__float_as_uint(v[4 * k]), __float_as_uint(v[4 * k + 1]),
+                                                                       __float_as_uint(v[4 * k + 2]), __float_as_uint(v[4 * k + 3])));
                 } else {
+                    float on = 0.f;
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
-                        if (c + k == row) diag_a[row] = v[k] * to_d;
-                        v[k] = c + k == row ? 0.f : v[k] * to_a;
+                        on = c + k == row ? v[k] : on;
+                        v[k] = c + k == row ? 0.f : v[k] * sh.to_a;
                     }
+                    if ((row & ~15) == c) diag_a[row] = on * sh.to_d;
                     planes_put16(a_hi, a_lo, sh.m16, row, c, v);
                 }
             }
         if (sh.blocks > 1) {
             cluster_sync();
-            const int per = (sh.m16 + sh.blocks - 1) / sh.blocks, r0 = (int)rank * per, r1 = min(sh.m16, r0 + per);
-            const int eights = sh.m16 / 8;
-            for (int t = tid; t < (r1 - r0) * eights; t += kClusterThreads) {
-                const int i = r0 + t / eights, c = (t % eights) * 8;
+            // add up this block's rows, in the order of the blocks, and give them to all
+            const int r0 = (int)rank * sh.per, rows = max(0, min(sh.m16, r0 + sh.per) - r0), eights = sh.m16 / 8;
+            for (int t = tid; t < rows * eights; t += kClusterThreads) {
+                const int i = t / eights, c = (t - i * eights) * 8;
                 float v[8] = {};
+#pragma unroll 4
                 for (int r = 0; r < sh.blocks; ++r) {
-                    const uint32_t p = remote(smem_u32(partial + i * pitch + c), r);
-                    const float4 f = remote_load4(p), g = remote_load4(p + 16);
+                    const float4 *p = reinterpret_cast<const float4 *>(partial + (r * sh.per + i) * pitch + c);
+                    const float4 f = p[0], g = p[1];
                     v[0] += f.x, v[1] += f.y, v[2] += f.z, v[3] += f.w;
                     v[4] += g.x, v[5] += g.y, v[6] += g.z, v[7] += g.w;
                 }
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    if (c + k == i)
-                        for (int r = 0; r < sh.blocks; ++r) remote_store_f32(remote(smem_u32(&diag_a[i]), r), v[k] * to_d);
-                    v[k] = c + k == i ? 0.f : v[k] * to_a;
+                    if (c + k == r0 + i)
+                        for (int r = 0; r < sh.blocks; ++r) remote_store_f32(remote(smem_u32(&diag_a[r0 + i]), r), v[k] * sh.to_d);
+                    v[k] = c + k == r0 + i ? 0.f : v[k] * sh.to_a;
                 }
                 uint4 hi, lo;
                 split8(v, hi, lo);
-                const uint32_t at = plane_byte(sh.m16, i, c);
+                const uint32_t at = plane_byte(sh.m16, r0 + i, c);
                 for (int r = 0; r < sh.blocks; ++r) {
                     remote_store4(remote(ah + at, r), hi);
                     remote_store4(remote(al + at, r), lo);
                 }
             }
-            async_proxy_fence();
+            asm volatile("fence.proxy.async.shared::cluster;" ::: "memory");
             cluster_sync();
         }
         // B
         begin();
-        if (tid == 0) {
-            multiply(tmem, ah, al, ah, al, sh.m16, sh.m16, true, sh.m16, sh.m16);
-            mma_commit(&done);
+        if (warp == 0) {
+            multiply(tmem, ah, al, ah, al, sh.m16, sh.m16, true, sh.m16, sh.m16, leader);
+            mma_commit(&done, leader);
+        }
+        float o[16];
+        float di = 0.f;
+        if (mine) {
+            di = diag_a[row];
+            if (16 * turn < sh.m16) planes_get16(a_hi, a_lo, sh.m16, row, 16 * turn, o);
         }
         finish();
-        if (rows_here) {
-            const float di = mine ? diag_a[row] : 0.f;
-            const float c0 = cb * (sh.b_scale / sh.a_scale), c1 = cc * (sh.b_scale / sh.a_scale),
-                        c2 = cc * (sh.b_scale / (sh.a_scale * sh.a_scale)), c5 = cc / (sh.a_scale * sh.a_scale);
+        if (rows_here)
             for (int c = 16 * turn; c < sh.m16; c += 64) {
-                float v[16], o[16];
+                float v[16];
                 __syncwarp();
                 tmem_load16(acc + c, v);
                 if (!mine) continue;
-                planes_get16(a_hi, a_lo, sh.m16, row, c, o);
+                const float base = fmaf(cf[2], di, cf[1]);
+                float on = 0.f; // the diagonal's sum
 #pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    if (c + k == row) {
-                        diag_b[row] = fmaf(cb, di, fmaf(cc * di, di, c5 * v[k]));
-                        v[k] = 0.f;
-                    } else {
-                        v[k] = fmaf(fmaf(c1, di + diag_a[c + k], c0), o[k], c2 * v[k]);
+                for (int k4 = 0; k4 < 16; k4 += 4) {
+                    const float4 dj = *reinterpret_cast<const float4 *>(diag_a + c + k4);
+                    const float d4[4] = {dj.x, dj.y, dj.z, dj.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int k = k4 + i;
+                        const float w = fmaf(fmaf(cf[2], d4[i], base), o[k], cf[3] * v[k]);
+                        on = c + k == row ? v[k] : on;
+                        v[k] = c + k == row ? 0.f : w;
                     }
                 }
+                if ((row & ~15) == c) diag_b[row] = fmaf(cf[4], di, fmaf(cf[5] * di, di, cf[6] * on));
                 planes_put16(a_hi, a_lo, sh.m16, row, c, v);
+                if (c + 64 < sh.m16) planes_get16(a_hi, a_lo, sh.m16, row, c + 64, o);
             }
-        }
         // X
         begin();
-        if (tid == 0) {
+        if (warp == 0) {
             for (int c = 0; c < ns16; c += 256)
                 multiply(tmem + c, ah, al, xh + (c >> 6) * sh.m16 * 128, xl + (c >> 6) * sh.m16 * 128, sh.m16, sh.m16, false,
-                         min(256, ns16 - c), sh.m16);
-            mma_commit(&done);
+                         min(256, ns16 - c), sh.m16, leader);
+            mma_commit(&done, leader);
+        }
+        float f = 0.f;
+        if (mine) {
+            f = cf[0] + diag_b[row];
+            if (16 * turn < ns16) planes_get16(x_hi, x_lo, sh.m16, row, 16 * turn, o);
         }
         finish();
         if (rows_here) {
-            const bool last = step + 1 == co.steps;
-            const float f = ca + (mine ? diag_b[row] : 0.f), unscale = 1.f / sh.b_scale, out = 1.f / sh.x_scale;
+            const bool last = step + 1 == co.n;
             for (int c = 16 * turn; c < ns16; c += 64) {
-                float v[16], o[16];
+                float v[16];
                 __syncwarp();
                 tmem_load16(acc + c, v);
                 if (!mine) continue;
-                planes_get16(x_hi, x_lo, sh.m16, row, c, o);
 #pragma unroll
-                for (int k = 0; k < 16; ++k) v[k] = fmaf(f, o[k], unscale * v[k]);
+                for (int k = 0; k < 16; ++k) v[k] = fmaf(f, o[k], sh.unscale_b * v[k]);
+                if (c + 64 < ns16) planes_get16(x_hi, x_lo, sh.m16, row, c + 64, o);
                 if (!last) {
                     planes_put16(x_hi, x_lo, sh.m16, row, c, v);
                 } else { // the result itself, 32-bit, in the place of the two planes: hi 0..3, 4..7, lo 8..11, 12..15
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const uint32_t at = plane_byte(sh.m16, row, c + 8 * h);
-                        *reinterpret_cast<float4 *>(x_hi + at) =
-                            make_float4(v[4 * h] * out, v[4 * h + 1] * out, v[4 * h + 2] * out, v[4 * h + 3] * out);
-                        *reinterpret_cast<float4 *>(x_lo + at) =
-                            make_float4(v[8 + 4 * h] * out, v[9 + 4 * h] * out, v[10 + 4 * h] * out, v[11 + 4 * h] * out);
+                        const float u = sh.unscale_x;
+                        *reinterpret_cast<float4 *>(x_hi + at) = make_float4(v[4 * h] * u, v[4 * h + 1] * u, v[4 * h + 2] * u, v[4 * h + 3] * u);
+                        *reinterpret_cast<float4 *>(x_lo + at) = make_float4(v[8 + 4 * h] * u, v[9 + 4 * h] * u, v[10 + 4 * h] * u, v[11 + 4 * h] * u);
                     }
                 }
             }
@@ -369,19 +466,49 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
     if (warp == 0)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(sh.columns) : "memory");
     const bool poisoned = *abort != 0; // a wait ran out
-#pragma unroll 4
-    for (int e = tid; e < count; e += kClusterThreads) {
-        int i, j;
-        const size_t at = place(e, i, j);
+    auto get = [&](int i, int j) -> float {
         const int w = j & 15;
-        const char *plane = w < 8 ? x_hi : x_lo;
-        float v = *reinterpret_cast<const float *>(plane + plane_byte(sh.m16, i, (j & ~15) + ((w >> 2) & 1) * 8) + (w & 3) * 4);
-        if (poisoned) v = NAN;
-        if (MUON) {
-            T *p = static_cast<T *>(tab.param[tensor]) + mat + at;
-            *p = from_f32<T>(muon_param(to_f32(*p), v, tab.lr[tensor], tab.decay[tensor]));
-        } else {
-            y[mat + at] = from_f32<T>(v);
+        const float v = *reinterpret_cast<const float *>((w < 8 ? x_hi : x_lo) + plane_byte(sh.m16, i, (j & ~15) + ((w >> 2) & 1) * 8) + (w & 3) * 4);
+        return poisoned ? NAN : v;
+    };
+    for (int e0 = tid; e0 < moves; e0 += U * kClusterThreads) {
+        float4 p[U];
+        size_t at[U];
+        int i[U], j[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int e = e0 + u * kClusterThreads;
+            if (e < moves) {
+                at[u] = place(e, i[u], j[u]);
+                if (MUON) {
+                    const T *q = static_cast<const T *>(tab.param[tensor]) + mat + at[u];
+                    if (e < fours) p[u] = Quad<T>::get(*reinterpret_cast<const VT *>(q));
+                    else p[u].x = to_f32(*q);
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int e = e0 + u * kClusterThreads;
+            if (e >= moves) continue;
+            float4 v = {};
+            v.x = get(i[u], j[u]);
+            if (e < fours) {
+                next(i[u], j[u]);
+                v.y = get(i[u], j[u]);
+                next(i[u], j[u]);
+                v.z = get(i[u], j[u]);
+                next(i[u], j[u]);
+                v.w = get(i[u], j[u]);
+            }
+            T *out = (MUON ? static_cast<T *>(tab.param[tensor]) : y) + mat + at[u];
+            if (MUON) {
+                const float lr = tab.lr[tensor], decay = tab.decay[tensor];
+                v = make_float4(muon_param(p[u].x, v.x, lr, decay), muon_param(p[u].y, v.y, lr, decay),
+                                muon_param(p[u].z, v.z, lr, decay), muon_param(p[u].w, v.w, lr, decay));
+            }
+            if (e < fours) *reinterpret_cast<VT *>(out) = Quad<T>::put(v);
+            else *out = from_f32<T>(v.x);
         }
     }
 }
@@ -396,11 +523,12 @@ static ClusterShape cluster_shape(int rows, int cols, int blocks) {
     s.blocks = blocks;
     s.ns = ((s.n + blocks - 1) / blocks + 15) / 16 * 16;
     s.ns64 = (s.ns + 63) / 64 * 64;
+    s.per = (s.m16 + blocks - 1) / blocks;
     s.columns = 32;
     while (s.columns < std::max(s.m16, s.ns)) s.columns *= 2;
     const size_t planes = 4 * (size_t)s.m16 * (s.ns64 + s.mk);
     // a 128-row operand reads past a plane of fewer rows: into what follows, whose rows of the product are not read
-    size_t smem = 1024 + planes + std::max<size_t>(blocks > 1 ? 4 * (size_t)s.m16 * (s.m16 + 4) : 0, (size_t)(128 - s.m16) * 128);
+    size_t smem = 1024 + planes + std::max<size_t>(blocks > 1 ? 4 * (size_t)s.per * blocks * (s.m16 + 4) : 0, (size_t)(128 - s.m16) * 128);
     // blocks that share an SM must find their TMEM columns free: as large a part of its shared memory as of its TMEM
     smem = std::max(smem, kClusterSmem * s.columns / 512 - kClusterStatic);
     s.smem = smem;
@@ -421,7 +549,7 @@ bool ortho_is_clustered(int rows, int cols) { return cluster_blocks(rows, cols) 
 
 template <typename T, typename M, bool MUON>
 static int cluster_launch(long long batch, const ClusterShape &sh, const void *x, void *y, const MuonTable &tab,
-                          const OrthoCoefficients &co, float eps, cudaStream_t stream) {
+                          const ClusterSteps &steps, float eps, cudaStream_t stream) {
     auto *kernel = ortho_cluster_kernel<T, M, MUON>;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sh.smem) != cudaSuccess)
         return check_launch("ortho_cluster_kernel attributes");
@@ -436,16 +564,26 @@ static int cluster_launch(long long batch, const ClusterShape &sh, const void *x
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, sh, static_cast<const T *>(x), static_cast<T *>(y), tab, co, eps);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, sh, static_cast<const T *>(x), static_cast<T *>(y), tab, steps, eps);
     if (e != cudaSuccess) return set_error(kErrLaunch, "ortho_cluster_kernel: %s", cudaGetErrorString(e));
     return check_launch("ortho_cluster_kernel");
 }
 
-static int cluster_shape_for(const char *what, long long batch, int rows, int cols, float x_scale, float a_scale, float b_scale, ClusterShape *sh) {
+static int cluster_plan(const char *what, long long batch, int rows, int cols, const OrthoCoefficients &co, float x_scale,
+                        float a_scale, float b_scale, ClusterShape *sh, ClusterSteps *steps) {
     *sh = cluster_shape(rows, cols, cluster_blocks(rows, cols));
     sh->x_scale = x_scale;
-    sh->a_scale = a_scale;
-    sh->b_scale = b_scale;
+    sh->to_a = a_scale / (x_scale * x_scale);
+    sh->to_d = 1.f / (x_scale * x_scale);
+    sh->unscale_b = 1.f / b_scale;
+    sh->unscale_x = 1.f / x_scale;
+    steps->n = co.steps;
+    for (int k = 0; k < co.steps; ++k) {
+        const float a = co.c[k][0], b = co.c[k][1], c = co.c[k][2];
+        const float v[7] = {a, b * (b_scale / a_scale), c * (b_scale / a_scale), c * (b_scale / (a_scale * a_scale)), b, c,
+                            c / (a_scale * a_scale)};
+        std::copy(v, v + 7, steps->c[k]);
+    }
     if (batch * sh->blocks > 0x7fffffffll) return set_error(kErrInvalidArgument, "%s: too many matrices", what);
     return kOk;
 }
@@ -453,25 +591,27 @@ static int cluster_shape_for(const char *what, long long batch, int rows, int co
 int ortho_cluster_fwd(long long batch, int rows, int cols, int dtype, const void *x, void *y, const OrthoCoefficients &co,
                       float x_scale, float a_scale, float b_scale, float eps, cudaStream_t stream) {
     ClusterShape sh;
-    if (int e = cluster_shape_for("orthogonalize", batch, rows, cols, x_scale, a_scale, b_scale, &sh)) return e;
+    ClusterSteps st = {};
+    if (int e = cluster_plan("orthogonalize", batch, rows, cols, co, x_scale, a_scale, b_scale, &sh, &st)) return e;
     static const MuonTable none = {};
-    if (dtype == kOrthoF32) return cluster_launch<float, float, false>(batch, sh, x, y, none, co, eps, stream);
-    if (dtype == kOrthoBF16) return cluster_launch<__nv_bfloat16, float, false>(batch, sh, x, y, none, co, eps, stream);
-    return cluster_launch<__half, float, false>(batch, sh, x, y, none, co, eps, stream);
+    if (dtype == kOrthoF32) return cluster_launch<float, float, false>(batch, sh, x, y, none, st, eps, stream);
+    if (dtype == kOrthoBF16) return cluster_launch<__nv_bfloat16, float, false>(batch, sh, x, y, none, st, eps, stream);
+    return cluster_launch<__half, float, false>(batch, sh, x, y, none, st, eps, stream);
 }
 
 int ortho_cluster_muon(const MuonTable &t, int rows, int cols, const OrthoCoefficients &co, float x_scale, float a_scale,
                        float b_scale, float eps, cudaStream_t stream) {
     ClusterShape sh;
+    ClusterSteps st = {};
     const long long batch = t.first[t.n];
-    if (int e = cluster_shape_for("muon", batch, rows, cols, x_scale, a_scale, b_scale, &sh)) return e;
+    if (int e = cluster_plan("muon", batch, rows, cols, co, x_scale, a_scale, b_scale, &sh, &st)) return e;
     const bool same = t.dtype == t.state_dtype;
-    if (t.dtype == kOrthoF32) return cluster_launch<float, float, true>(batch, sh, nullptr, nullptr, t, co, eps, stream);
+    if (t.dtype == kOrthoF32) return cluster_launch<float, float, true>(batch, sh, nullptr, nullptr, t, st, eps, stream);
     if (t.dtype == kOrthoBF16)
-        return same ? cluster_launch<__nv_bfloat16, __nv_bfloat16, true>(batch, sh, nullptr, nullptr, t, co, eps, stream)
-                    : cluster_launch<__nv_bfloat16, float, true>(batch, sh, nullptr, nullptr, t, co, eps, stream);
-    return same ? cluster_launch<__half, __half, true>(batch, sh, nullptr, nullptr, t, co, eps, stream)
-                : cluster_launch<__half, float, true>(batch, sh, nullptr, nullptr, t, co, eps, stream);
+        return same ? cluster_launch<__nv_bfloat16, __nv_bfloat16, true>(batch, sh, nullptr, nullptr, t, st, eps, stream)
+                    : cluster_launch<__nv_bfloat16, float, true>(batch, sh, nullptr, nullptr, t, st, eps, stream);
+    return same ? cluster_launch<__half, __half, true>(batch, sh, nullptr, nullptr, t, st, eps, stream)
+                : cluster_launch<__half, float, true>(batch, sh, nullptr, nullptr, t, st, eps, stream);
 }
 
 } // namespace gsb

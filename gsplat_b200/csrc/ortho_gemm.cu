@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     extern __shared__ char raw[];
     __shared__ GemmShared sh;
     const uint32_t stage0 = (smem_u32(raw) + 1023u) & ~1023u;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = uniform_warp(), lane = threadIdx.x % 32;
     volatile int *abort = &sh.abort;
 
     if (warp == kEpilogueWarps && lane == 0) {
@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem = sh.tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
 
     const int kblocks = (g.K + kBK - 1) / kBK;
     const int total = kblocks * g.pairs;               // stages of a tile
@@ -260,7 +260,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         }
     } else if (warp == kEpilogueWarps + 1) {
         // the products
-        if (lane == 0) {
+        const uint32_t leader = elect_leader();
+        {
             const uint32_t idesc = mma_desc(kBN, g.q_k_major);
             const uint32_t q_step = g.q_k_major ? 32 / 16 : 2048 / 16; // 16 deep, in the descriptor's units
             int stage = 0, acc = 0;
@@ -270,13 +271,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                 const TileAt at = tile_at(t, per, tiles_n, g.symmetric);
                 if (tab.n > 0 && !muon_visible(tab, muon_tensor_of(tab, at.b), at.b)) continue;
                 for (int s0 = 0; ok && s0 < total; s0 += chunk) {
-                    ok = mbar_wait(&sh.acc_empty[acc], acc_phase ^ 1u, abort);
+                    ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_empty[acc], acc_phase ^ 1u, abort));
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint32_t d = tmem + acc * kBN;
                     const int s1 = min(total, s0 + chunk);
                     for (int s = s0; s < s1; ++s) {
-                        ok = mbar_wait(&sh.full[stage], phase, abort);
+                        ok = __all_sync(0xffffffffu, mbar_wait(&sh.full[stage], phase, abort));
                         if (!ok) break;
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                         const uint32_t src = stage0 + stage * kStageBytes;
@@ -285,19 +286,19 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                         const uint64_t lo = kPlaneBytes / 16; // from hi to lo
 #pragma unroll
                         for (int k = 0; k < kBK / 16; ++k) {
-                            mma_f16(d, p + k * 2, q + k * q_step, idesc, s > s0 || k > 0);
+                            mma_f16(d, p + k * 2, q + k * q_step, idesc, s > s0 || k > 0, leader);
                             if (SPLIT) {
-                                mma_f16(d, p + k * 2, q + lo + k * q_step, idesc, true);
-                                mma_f16(d, p + lo + k * 2, q + k * q_step, idesc, true);
+                                mma_f16(d, p + k * 2, q + lo + k * q_step, idesc, true, leader);
+                                mma_f16(d, p + lo + k * 2, q + k * q_step, idesc, true, leader);
                             }
                         }
-                        mma_commit(&sh.empty[stage]);
+                        mma_commit(&sh.empty[stage], leader);
                         if (++stage == kStages) {
                             stage = 0;
                             phase ^= 1u;
                         }
                     }
-                    mma_commit(&sh.acc_full[acc]); // also after a wait that ran out: what was issued is waited for
+                    mma_commit(&sh.acc_full[acc], leader); // also after a wait that ran out: what was issued is waited for
                     acc ^= 1;
                     if (acc == 0) acc_phase ^= 1u;
                 }

@@ -37,13 +37,25 @@ __device__ __forceinline__ bool mbar_wait(unsigned long long *b, uint32_t phase,
     return false;
 }
 
-__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
-    asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-                 "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+// Products are issued by a whole warp under the predicate `leader`, true in one lane: the
+// descriptors are then computed in uniform registers, where the instruction wants them. Issued from a
+// branch of one thread, each took 85 cycles, more than most products last.
+__device__ __forceinline__ int uniform_warp() { return __shfl_sync(0xffffffffu, (int)threadIdx.x / 32, 0); }
+__device__ __forceinline__ uint32_t elect_leader() {
+    uint32_t e;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(e));
+    return e;
+}
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate, uint32_t leader) {
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %4, 0;\n setp.ne.u32 q, %5, 0;\n"
+                 " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+                 "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(leader)
                  : "memory");
 }
-__device__ __forceinline__ void mma_commit(unsigned long long *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+__device__ __forceinline__ void mma_commit(unsigned long long *bar, uint32_t leader) {
+    asm volatile("{\n .reg .pred q;\n setp.ne.u32 q, %1, 0;\n"
+                 " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(smem_u32(bar)), "r"(leader)
+                 : "memory");
 }
 
 __device__ __forceinline__ void tmem_load32(uint32_t addr, float v[32]) {

@@ -116,6 +116,26 @@ __device__ __forceinline__ bool muon_visible(const MuonTable &t, int i, long lon
     return t.valid == nullptr || t.valid[(b - t.first[i] + t.skipped[i]) / t.inner[i]];
 }
 
+// A launch whose blocks may set up while the launch before it in the stream ends; the kernel
+// waits for that one (griddepcontrol.wait) before it touches memory.
+template <typename... P, typename... A>
+inline int launch_after(void (*kernel)(P...), unsigned blocks, int threads, size_t smem, cudaStream_t stream, const char *what,
+                        const A &...args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+    if (e != cudaSuccess) return set_error(kErrLaunch, "%s: %s", what, cudaGetErrorString(e));
+    return check_launch(what);
+}
+
 // --- thin matrices (ortho_thin.cu) -----------------------------------------
 // short side <= 4 and long side <= 128: a few lanes hold one matrix.
 bool ortho_is_thin(int rows, int cols);

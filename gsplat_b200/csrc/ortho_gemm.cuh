@@ -1,0 +1,433 @@
+// Batched products of the Newton-Schulz iteration with their element-wise ends, on
+// the fifth-generation tensor cores: one persistent block an SM, TMA into 128-byte-swizzled
+// stages, tcgen05.mma into double-buffered TMEM accumulators, and eight warps that
+// finish a tile while the next one is multiplied.
+//
+// A tile is 128 x BN of the result, 64 deep a stage. With SPLIT, a stage holds
+// the hi and lo planes of both operands and feeds three products (hi hi, hi lo, lo hi);
+// the sum is taken out of the tensor cores every kChunk stages and continued in
+// registers, since their 32-bit adder truncates and the bias of a long sum of
+// squares would be seen in the diagonal of A.
+// A launch follows the one before it without a gap: its blocks set up while that one ends (griddepcontrol).
+#pragma once
+
+#include <cuda.h>
+
+#include "ortho.cuh"
+#include "tcgen05.cuh"
+
+namespace gsb {
+
+constexpr int kBM = 128, kBK = 64;
+constexpr int kChunk = 8;          // stages between two readings of the accumulator, split
+constexpr int kEpilogueWarps = 8;  // four lane quarters x two column halves
+constexpr int kGemmThreads = 32 * (kEpilogueWarps + 2);
+constexpr int kStagePitch = 33;    // floats a row of a warp's 32 x 32 values on their way out
+constexpr int kOutStage = kEpilogueWarps * 32 * kStagePitch * 4;
+constexpr int kMaxStages = 8;
+
+// Bytes of a stage, and how many fit beside the epilogue's.
+template <bool SPLIT, int BN> struct Stages {
+    static constexpr int p = kBM * kBK * 2, q = BN * kBK * 2, bytes = (SPLIT ? 2 : 1) * (p + q);
+    static constexpr int fit = (227 * 1024 - 1024 - 512 - kOutStage) / bytes;
+    static constexpr int n = fit < kMaxStages ? fit : kMaxStages;
+    static constexpr int smem = n * bytes + kOutStage + 1024;
+};
+
+struct GemmMaps {
+    CUtensorMap p_hi[2], p_lo[2], q_hi[2], q_lo[2];
+};
+
+struct GemmShared {
+    alignas(8) unsigned long long full[kMaxStages], empty[kMaxStages];
+    unsigned long long acc_full[2], acc_empty[2];
+    uint32_t tmem;
+    int abort;
+};
+
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, int x, int y, int z,
+                                         unsigned long long *bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+                 "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+                 : "memory");
+}
+
+// Eight values of a row of planes, as they are stored.
+struct Eight {
+    uint4 hi, lo;
+};
+template <bool LO> __device__ __forceinline__ Eight load8(const OrthoPlanes &p, size_t at) {
+    Eight r;
+    r.hi = *reinterpret_cast<const uint4 *>(p.hi + at);
+    if (LO) r.lo = *reinterpret_cast<const uint4 *>(p.lo + at);
+    return r;
+}
+template <bool LO> __device__ __forceinline__ void unpack8(const Eight &r, float v[8]) {
+    const __half2 *h = reinterpret_cast<const __half2 *>(&r.hi), *l = reinterpret_cast<const __half2 *>(&r.lo);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 a = __half22float2(h[i]);
+        v[2 * i] = a.x;
+        v[2 * i + 1] = a.y;
+        if (LO) {
+            const float2 b = __half22float2(l[i]);
+            v[2 * i] += b.x;
+            v[2 * i + 1] += b.y;
+        }
+    }
+}
+template <bool LO> __device__ __forceinline__ void store8(const OrthoPlanes &p, size_t at, const float v[8]) {
+    uint4 h, l;
+    __half2 *hh = reinterpret_cast<__half2 *>(&h), *ll = reinterpret_cast<__half2 *>(&l);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        hh[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+        const float2 f = __half22float2(hh[i]);
+        ll[i] = __floats2half2_rn(v[2 * i] - f.x, v[2 * i + 1] - f.y);
+    }
+    *reinterpret_cast<uint4 *>(p.hi + at) = h;
+    if (LO) *reinterpret_cast<uint4 *>(p.lo + at) = l;
+}
+
+struct TileAt {
+    long long b;
+    int i, j; // in tiles
+};
+// Tile t of the launch. Symmetric results list, by rows, the tiles with a column on or below the
+// diagonal: of row block i the column tiles 0 .. i * kBM / BN (BN <= kBM: all of the diagonal block's).
+template <int BN> __device__ __forceinline__ TileAt tile_at(long long t, int per, int tiles_n, int symmetric) {
+    constexpr int w = kBM / BN; // column tiles of a row block
+    TileAt r;
+    r.b = t / per;
+    const int k = (int)(t - r.b * per);
+    if (symmetric) { // rows 0 .. i - 1 hold w i (i + 1) / 2 tiles
+        int i = (int)((sqrtf(8.f * (float)(k / w) + 1.f) - 1.f) * 0.5f);
+        while (w * i * (i + 1) / 2 > k) --i;
+        while (w * (i + 1) * (i + 2) / 2 <= k) ++i;
+        r.i = i;
+        r.j = k - w * i * (i + 1) / 2;
+    } else {
+        r.i = k / tiles_n;
+        r.j = k - r.i * tiles_n;
+    }
+    return r;
+}
+
+template <bool SPLIT, int BN, int EPI>
+__global__ void __launch_bounds__(kGemmThreads, 1)
+    ortho_gemm_kernel(const __grid_constant__ OrthoGemm g, const __grid_constant__ GemmMaps maps,
+                      const __grid_constant__ MuonTable tab, int per, int tiles_n, long long tiles) {
+    using Stage = Stages<SPLIT, BN>;
+    constexpr int kStages = Stage::n;
+    constexpr bool kSymmetric = EPI == kEpiGram || EPI == kEpiSquare || EPI == kEpiSym || EPI == kEpiAnti;
+    constexpr bool kQDepthMajor = kSymmetric;
+    constexpr bool kElement = EPI != kEpiGram && EPI != kEpiSym;             // reads e
+    constexpr bool kElementLo = SPLIT || EPI == kEpiApply || EPI == kEpiOut || EPI == kEpiMuon;
+    constexpr bool kToPlanes = EPI != kEpiOut && EPI != kEpiMuon;
+    constexpr bool kOutLo = SPLIT || EPI == kEpiApply;
+    constexpr int W = BN / 2; // columns of a warp
+    extern __shared__ char raw[];
+    __shared__ GemmShared sh;
+    const uint32_t stage0 = (smem_u32(raw) + 1023u) & ~1023u;
+    const int warp = uniform_warp(), lane = threadIdx.x % 32;
+    volatile int *abort = &sh.abort;
+
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); // the next product's blocks may set up; they wait below
+    if (warp == kEpilogueWarps && lane == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(&sh.full[s], 1);
+            mbar_init(&sh.empty[s], 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(&sh.acc_full[a], 1);
+            mbar_init(&sh.acc_empty[a], kEpilogueWarps);
+        }
+        sh.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kEpilogueWarps + 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
+                     "r"(2 * BN)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
+    asm volatile("griddepcontrol.wait;" ::: "memory"); // for what the launches before this one wrote
+
+    const int kblocks = (g.K + kBK - 1) / kBK;
+    const int total = kblocks * g.pairs;      // stages of a tile
+    const int chunk = SPLIT ? kChunk : total; // stages of an accumulation
+    if (warp == kEpilogueWarps) {
+        // the copies
+        if (lane == 0) {
+            int stage = 0;
+            uint32_t phase = 0;
+            long long loads = 0;
+            bool ok = true;
+            for (long long t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+                const TileAt at = tile_at<BN>(t, per, tiles_n, kSymmetric);
+                if (tab.n > 0 && !muon_visible(tab, muon_tensor_of(tab, at.b), at.b)) continue;
+                const int b = (int)at.b, i0 = at.i * kBM, j0 = at.j * BN;
+                for (int s = 0; s < total; ++s) {
+                    const int pair = s >= kblocks, k0 = (s - pair * kblocks) * kBK;
+                    ok = mbar_wait(&sh.empty[stage], phase ^ 1u, abort);
+                    if (!ok) break;
+                    uint32_t dst = stage0 + stage * Stage::bytes;
+                    unsigned long long *bar = &sh.full[stage];
+                    mbar_expect(bar, Stage::bytes);
+                    tma_load(dst, &maps.p_hi[pair], k0, i0, b, bar);
+                    if (SPLIT) tma_load(dst + Stage::p, &maps.p_lo[pair], k0, i0, b, bar);
+                    dst += (SPLIT ? 2 : 1) * Stage::p;
+#pragma unroll
+                    for (int lo = 0; lo < (SPLIT ? 2 : 1); ++lo) {
+                        const CUtensorMap *m = lo ? &maps.q_lo[pair] : &maps.q_hi[pair];
+                        if (kQDepthMajor) {
+                            tma_load(dst + lo * Stage::q, m, k0, j0, b, bar);
+                        } else {
+#pragma unroll
+                            for (int c = 0; c < BN / 64; ++c) tma_load(dst + lo * Stage::q + c * kBK * 128, m, j0 + 64 * c, k0, b, bar);
+                        }
+                    }
+                    ++loads;
+                    if (++stage == kStages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+            if (!ok) { // wait, with a limit, for the copies in flight
+                const long long first = loads > kStages ? loads - kStages : 0;
+                for (long long l = first; l < loads; ++l)
+                    for (unsigned i = 0; i < kWaitLimit && !mbar_try(&sh.full[l % kStages], (uint32_t)(l / kStages) & 1u); ++i) {}
+            }
+        }
+    } else if (warp == kEpilogueWarps + 1) {
+        // the products
+        const uint32_t leader = elect_leader();
+        constexpr uint32_t q_step = kQDepthMajor ? 32 / 16 : 2048 / 16; // 16 deep, in the descriptor's units
+        const uint32_t idesc = mma_desc(BN, kQDepthMajor);
+        int stage = 0, acc = 0;
+        uint32_t phase = 0, acc_phase = 0;
+        bool ok = true;
+        for (long long t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+            const TileAt at = tile_at<BN>(t, per, tiles_n, kSymmetric);
+            if (tab.n > 0 && !muon_visible(tab, muon_tensor_of(tab, at.b), at.b)) continue;
+            for (int s0 = 0; ok && s0 < total; s0 += chunk) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_empty[acc], acc_phase ^ 1u, abort));
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t d = tmem + acc * BN;
+                const int s1 = min(total, s0 + chunk);
+                for (int s = s0; s < s1; ++s) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&sh.full[stage], phase, abort));
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t src = stage0 + stage * Stage::bytes;
+                    const uint64_t p = operand_desc(src, true, 0);
+                    const uint64_t q = operand_desc(src + (SPLIT ? 2 : 1) * Stage::p, kQDepthMajor, kBK * 128);
+                    constexpr uint64_t p_lo = Stage::p / 16, q_lo = Stage::q / 16; // from hi to lo
+#pragma unroll
+                    for (int k = 0; k < kBK / 16; ++k) {
+                        mma_f16(d, p + k * 2, q + k * q_step, idesc, s > s0 || k > 0, leader);
+                        if (SPLIT) {
+                            mma_f16(d, p + k * 2, q + q_lo + k * q_step, idesc, true, leader);
+                            mma_f16(d, p + p_lo + k * 2, q + k * q_step, idesc, true, leader);
+                        }
+                    }
+                    mma_commit(&sh.empty[stage], leader);
+                    if (++stage == kStages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                mma_commit(&sh.acc_full[acc], leader); // also after a wait that ran out: what was issued is waited for
+                acc ^= 1;
+                if (acc == 0) acc_phase ^= 1u;
+            }
+        }
+    } else {
+        // the epilogue: warp w has rows 32 (w % 4) .., columns W (w / 4) ..
+        const int row = 32 * (warp % 4) + lane, half = warp / 4;
+        float *out_stage = reinterpret_cast<float *>(raw + (stage0 - smem_u32(raw)) + kStages * Stage::bytes) + warp * 32 * kStagePitch;
+        const bool poisoned = !kToPlanes && *(volatile const int *)g.error != 0;
+        int acc = 0;
+        uint32_t acc_phase = 0;
+        bool ok = true;
+        for (long long t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+            const TileAt at = tile_at<BN>(t, per, tiles_n, kSymmetric);
+            const int tensor = tab.n > 0 ? muon_tensor_of(tab, at.b) : 0;
+            if (tab.n > 0 && !muon_visible(tab, tensor, at.b)) continue;
+            const int i = at.i * kBM + row, j = at.j * BN + half * W;
+            const bool in_rows = i < g.M;
+            // what the epilogue needs is read while the products run
+            Eight e[W / 8];
+            float di = 0.f, dj[W / 32];
+            if (EPI != kEpiGram && EPI != kEpiSym && in_rows) di = g.diag_in[(size_t)at.b * g.M + i];
+            if (EPI == kEpiSquare || EPI == kEpiAnti) {
+#pragma unroll
+                for (int c = 0; c < W / 32; ++c)
+                    dj[c] = j + 32 * c + lane < g.N ? g.diag_in[(size_t)at.b * g.M + j + 32 * c + lane] : 0.f;
+            }
+            if (kElement && in_rows) {
+                const size_t at_e = (size_t)at.b * g.e.stride + (size_t)i * g.e.ld + j;
+#pragma unroll
+                for (int c = 0; c < W / 8; ++c)
+                    if (j + 8 * c < g.N) e[c] = load8<kElementLo>(g.e, at_e + 8 * c);
+            }
+            float v[W];
+            for (int s0 = 0; s0 < total; s0 += chunk) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[acc], acc_phase, abort));
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t src = tmem + ((uint32_t)(32 * (warp % 4)) << 16) + acc * BN + half * W;
+#pragma unroll
+                for (int c = 0; c < W; c += 32) {
+                    float u[32];
+                    tmem_load32(src + c, u);
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) v[c + k] = s0 == 0 ? u[k] : v[c + k] + u[k];
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.acc_empty[acc]);
+                acc ^= 1;
+                if (acc == 0) acc_phase ^= 1u;
+            }
+            if (!ok) break;
+            const bool mirror = kSymmetric && (at.j * BN) / kBM != at.i; // off the diagonal block
+            const size_t out_row = (size_t)at.b * g.out.stride + (size_t)i * g.out.ld + j;
+#pragma unroll
+            for (int c = 0; c < W; c += 8) {
+                float *w = v + c, x[8];
+                if (kElement) unpack8<kElementLo>(e[c / 8], x);
+                float on = 0.f;
+                bool diagonal = false;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    if (EPI == kEpiGram || EPI == kEpiSquare) {
+                        const bool here = i == j + c + k;
+                        on = here ? w[k] : on;
+                        diagonal |= here;
+                    }
+                    if (EPI == kEpiGram || EPI == kEpiSym) {
+                        w[k] *= g.c[0];
+                    } else if (EPI == kEpiSquare || EPI == kEpiAnti) {
+                        const float d = __shfl_sync(0xffffffffu, dj[c / 32], (c + k) & 31);
+                        w[k] = fmaf(fmaf(g.c[1], di + d, g.c[0]), x[k], g.c[2] * w[k]);
+                    } else {
+                        w[k] = fmaf(g.c[0] + di, x[k], g.c[1] * w[k]) * g.c[2];
+                    }
+                    if (EPI == kEpiGram || EPI == kEpiSquare) w[k] = i == j + c + k ? 0.f : w[k];
+                }
+                if ((EPI == kEpiGram || EPI == kEpiSquare) && diagonal && in_rows)
+                    g.diag_out[(size_t)at.b * g.M + i] =
+                        EPI == kEpiGram ? g.c[1] * on : fmaf(g.c[3], di, fmaf(g.c[4] * di, di, g.c[5] * on));
+                if (kToPlanes && in_rows && j + c < g.N) {
+                    store8<kOutLo>(g.out, out_row + c, w);
+                    if (mirror) { // tiles off the diagonal have all their columns
+                        __half *mh = g.out.hi + (size_t)at.b * g.out.stride + (size_t)(j + c) * g.out.ld + i;
+                        __half *ml = g.out.lo + (mh - g.out.hi);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const __half h = __float2half_rn(w[k]);
+                            mh[(size_t)k * g.out.ld] = h;
+                            if (kOutLo) ml[(size_t)k * g.out.ld] = __float2half_rn(w[k] - __half2float(h));
+                        }
+                    }
+                }
+            }
+            if (!kToPlanes) {
+                const size_t base = (size_t)(at.b - (EPI == kEpiMuon ? tab.first[tensor] : 0)) * g.M * g.N;
+                const int rows_left = g.M - (at.i * kBM + 32 * (warp % 4));
+                void *to = EPI == kEpiMuon ? tab.param[tensor] : g.y;
+                const int dtype = EPI == kEpiMuon ? tab.dtype : g.dtype;
+                const float lr = EPI == kEpiMuon ? tab.lr[tensor] : 0.f, decay = EPI == kEpiMuon ? tab.decay[tensor] : 0.f;
+                // 32 x 32 values at a time, neighbouring lanes at neighbouring places of the tensor: with a
+                // transposed tensor the lanes' rows are; else the values are turned through shared memory
+#pragma unroll
+                for (int c = 0; c < W; c += 32) {
+                    const int cols_left = g.N - (j + c);
+                    if (!g.transposed) {
+                        __syncwarp();
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) out_stage[lane * kStagePitch + k] = v[c + k];
+                        __syncwarp();
+                    }
+                    const int n = g.transposed ? cols_left : rows_left;            // turns: columns, or rows
+                    const bool lane_in = g.transposed ? in_rows : lane < cols_left; // the lane's row, or column
+                    const size_t at0 = base + (g.transposed ? (size_t)(j + c) * g.M + i
+                                                            : (size_t)(i - lane) * g.N + j + c + lane);
+                    const size_t step = g.transposed ? g.M : g.N;
+                    if (!lane_in) continue;
+#pragma unroll
+                    for (int k0 = 0; k0 < 32; k0 += 8) {
+                        float p[8];
+                        if (EPI == kEpiMuon) {
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) p[k] = k0 + k < n ? load_as_f32(to, at0 + (k0 + k) * step, dtype) : 0.f;
+                        }
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            if (k0 + k >= n) continue;
+                            float r = g.transposed ? v[c + k0 + k] : out_stage[(k0 + k) * kStagePitch + lane];
+                            if (poisoned) r = NAN;
+                            store_from_f32(to, at0 + (k0 + k) * step, dtype, EPI == kEpiMuon ? muon_param(p[k], r, lr, decay) : r);
+                        }
+                    }
+                }
+            }
+        }
+    }
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (warp == kEpilogueWarps + 1)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BN) : "memory");
+    if (threadIdx.x == 0 && sh.abort) atomicExch(g.error, 1);
+}
+
+template <bool SPLIT, int BN, int EPI>
+static int launch_one(const OrthoGemm &g, const GemmMaps &maps, const MuonTable &tab, int per, int tn, long long tiles,
+                      int sms, cudaStream_t stream) {
+    auto *kernel = ortho_gemm_kernel<SPLIT, BN, EPI>;
+    constexpr int smem = Stages<SPLIT, BN>::smem;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+        return check_launch("ortho_gemm_kernel attributes");
+    return launch_after(kernel, (unsigned)(tiles < sms ? tiles : sms), kGemmThreads, smem, stream, "ortho_gemm_kernel", g, maps, tab,
+                        per, tn, tiles);
+}
+
+template <bool SPLIT, int BN>
+int ortho_gemm_launch(const OrthoGemm &g, const GemmMaps &maps, const MuonTable &tab, int sms, cudaStream_t stream) {
+    const int tm = (g.M + kBM - 1) / kBM, tn = (g.N + BN - 1) / BN;
+    int per = tm * tn;
+    if (g.symmetric) { // less the last row block's tiles past the last column
+        constexpr int w = kBM / BN;
+        per = w * tm * (tm + 1) / 2 - (w * tm - tn);
+    }
+    const long long tiles = g.batch * per;
+    switch (g.epilogue) {
+    case kEpiGram: return launch_one<SPLIT, BN, kEpiGram>(g, maps, tab, per, tn, tiles, sms, stream);
+    case kEpiSquare: return launch_one<SPLIT, BN, kEpiSquare>(g, maps, tab, per, tn, tiles, sms, stream);
+    case kEpiApply: return launch_one<SPLIT, BN, kEpiApply>(g, maps, tab, per, tn, tiles, sms, stream);
+    case kEpiOut: return launch_one<SPLIT, BN, kEpiOut>(g, maps, tab, per, tn, tiles, sms, stream);
+    case kEpiMuon: return launch_one<SPLIT, BN, kEpiMuon>(g, maps, tab, per, tn, tiles, sms, stream);
+    default: break;
+    }
+    if constexpr (SPLIT) {
+        if (g.epilogue == kEpiSym) return launch_one<SPLIT, BN, kEpiSym>(g, maps, tab, per, tn, tiles, sms, stream);
+        return launch_one<SPLIT, BN, kEpiAnti>(g, maps, tab, per, tn, tiles, sms, stream);
+    }
+    return set_error(kErrUnsupported, "orthogonalize: a backward product of hi planes alone");
+}
+
+extern template int ortho_gemm_launch<true, 128>(const OrthoGemm &, const GemmMaps &, const MuonTable &, int, cudaStream_t);
+extern template int ortho_gemm_launch<false, 128>(const OrthoGemm &, const GemmMaps &, const MuonTable &, int, cudaStream_t);
+extern template int ortho_gemm_launch<true, 64>(const OrthoGemm &, const GemmMaps &, const MuonTable &, int, cudaStream_t);
+extern template int ortho_gemm_launch<false, 64>(const OrthoGemm &, const GemmMaps &, const MuonTable &, int, cudaStream_t);
+
+} // namespace gsb

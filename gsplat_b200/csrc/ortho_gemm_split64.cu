@@ -1,0 +1,5 @@
+#include "ortho_gemm.cuh"
+
+namespace gsb {
+template int ortho_gemm_launch<true, 64>(const OrthoGemm &, const GemmMaps &, const MuonTable &, int, cudaStream_t);
+} // namespace gsb

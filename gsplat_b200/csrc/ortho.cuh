@@ -103,6 +103,7 @@ struct MuonTable {
     void *momentum[kOrthoMaxTensors];
     float lr[kOrthoMaxTensors], decay[kOrthoMaxTensors]; // decay = 1 - lr * weight_decay
     int inner[kOrthoMaxTensors];         // matrices per leading row
+    bool transposed[kOrthoMaxTensors];   // the tensor's matrices are [long, short] (tiled path)
     long long skipped[kOrthoMaxTensors]; // the tensor's matrices before its first one here
     long long first[kOrthoMaxTensors + 1];
 };
@@ -196,7 +197,7 @@ struct OrthoGemm {
     const float *diag_in;    // [batch, M]
     float *diag_out;         // [batch, M]
     void *y;                 // kEpiOut: [batch, rows, cols] of `dtype`
-    int dtype, transposed;   // transposed: y / param are [N, M] in memory
+    int dtype, transposed;   // transposed: y is [N, M] in memory (kEpiMuon: the table says it)
     int *error;              // set when a kernel's wait ran out; the last product then writes NaN
 };
 

@@ -145,6 +145,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         sh.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (warp == kEpilogueWarps && lane < 8) { // the tensor maps: fetched while the launch before this one ends
+        const CUtensorMap *m = &maps.p_hi[0] + lane;
+        asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
+    }
     if (warp == kEpilogueWarps + 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
                      "r"(2 * BN)
@@ -341,6 +345,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             }
             if (!kToPlanes) {
                 const size_t base = (size_t)(at.b - (EPI == kEpiMuon ? tab.first[tensor] : 0)) * g.M * g.N;
+                const bool turned = EPI == kEpiMuon ? tab.transposed[tensor] : (bool)g.transposed;
                 const int rows_left = g.M - (at.i * kBM + 32 * (warp % 4));
                 void *to = EPI == kEpiMuon ? tab.param[tensor] : g.y;
                 const int dtype = EPI == kEpiMuon ? tab.dtype : g.dtype;
@@ -350,17 +355,17 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 #pragma unroll
                 for (int c = 0; c < W; c += 32) {
                     const int cols_left = g.N - (j + c);
-                    if (!g.transposed) {
+                    if (!turned) {
                         __syncwarp();
 #pragma unroll
                         for (int k = 0; k < 32; ++k) out_stage[lane * kStagePitch + k] = v[c + k];
                         __syncwarp();
                     }
-                    const int n = g.transposed ? cols_left : rows_left;            // turns: columns, or rows
-                    const bool lane_in = g.transposed ? in_rows : lane < cols_left; // the lane's row, or column
-                    const size_t at0 = base + (g.transposed ? (size_t)(j + c) * g.M + i
+                    const int n = turned ? cols_left : rows_left;            // turns: columns, or rows
+                    const bool lane_in = turned ? in_rows : lane < cols_left; // the lane's row, or column
+                    const size_t at0 = base + (turned ? (size_t)(j + c) * g.M + i
                                                             : (size_t)(i - lane) * g.N + j + c + lane);
-                    const size_t step = g.transposed ? g.M : g.N;
+                    const size_t step = turned ? g.M : g.N;
                     if (!lane_in) continue;
 #pragma unroll
                     for (int k0 = 0; k0 < 32; k0 += 8) {
@@ -372,7 +377,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 #pragma unroll
                         for (int k = 0; k < 8; ++k) {
                             if (k0 + k >= n) continue;
-                            float r = g.transposed ? v[c + k0 + k] : out_stage[(k0 + k) * kStagePitch + lane];
+                            float r = turned ? v[c + k0 + k] : out_stage[(k0 + k) * kStagePitch + lane];
                             if (poisoned) r = NAN;
                             store_from_f32(to, at0 + (k0 + k) * step, dtype, EPI == kEpiMuon ? muon_param(p[k], r, lr, decay) : r);
                         }

@@ -26,24 +26,53 @@
 namespace gsb {
 
 // --- norms and the split into planes ----------------------------------------
+// These passes are bound by memory: four values to an access where the matrix allows it, and
+// several accesses a thread on their way at once.
 constexpr int kNormThreads = 256;
-constexpr long long kNormChunk = 16384; // elements a block
 constexpr int kSplitTile = 64;
 
-struct OrthoSource { // what is read: x, or the Muon update of its matrix
-    const void *x;
-    int dtype;
-};
+// What is read: x, or the Muon update of its matrix.
+template <typename T, typename M, bool MUON> struct OrthoSource {
+    const T *x; // or the gradient
+    M *mom;
+    float mu, one_minus_mu;
+    int nesterov;
+    using VT = typename Quad<T>::type;
+    using VM = typename Quad<M>::type;
 
-__device__ __forceinline__ float source_at(const OrthoSource &s, const MuonTable &tab, int t, long long b, size_t numel,
-                                           size_t e, bool write_momentum) {
-    if (tab.n == 0) return load_as_f32(s.x, (size_t)b * numel + e, s.dtype);
-    const size_t at = (size_t)(b - tab.first[t]) * numel + e;
-    const float g = load_as_f32(tab.grad[t], at, tab.dtype);
-    const float m = muon_momentum(g, load_as_f32(tab.momentum[t], at, tab.state_dtype), tab.one_minus_mu);
-    if (write_momentum) store_from_f32(tab.momentum[t], at, tab.state_dtype, m);
-    return muon_update(g, m, tab.mu, tab.nesterov);
-}
+    __device__ __forceinline__ OrthoSource(const void *xs, const MuonTable &tab, int t, long long b, size_t numel) {
+        if (MUON) {
+            const size_t at = (size_t)(b - tab.first[t]) * numel;
+            x = static_cast<const T *>(tab.grad[t]) + at;
+            mom = static_cast<M *>(tab.momentum[t]) + at;
+            mu = tab.mu;
+            one_minus_mu = tab.one_minus_mu;
+            nesterov = tab.nesterov;
+        } else {
+            x = static_cast<const T *>(xs) + (size_t)b * numel;
+        }
+    }
+    __device__ __forceinline__ bool aligned() const {
+        return reinterpret_cast<uintptr_t>(x) % (4 * sizeof(T)) == 0 &&
+               (!MUON || reinterpret_cast<uintptr_t>(mom) % (4 * sizeof(M)) == 0);
+    }
+    __device__ __forceinline__ float4 get4(size_t e, float4 &m) const {
+        if (MUON) m = Quad<M>::get(*reinterpret_cast<const VM *>(mom + e));
+        return Quad<T>::get(*reinterpret_cast<const VT *>(x + e));
+    }
+    __device__ __forceinline__ float get1(size_t e, float &m) const {
+        if (MUON) m = to_f32(mom[e]);
+        return to_f32(x[e]);
+    }
+    __device__ __forceinline__ float update(float g, float &m) const {
+        if (!MUON) return g;
+        m = muon_momentum(g, m, one_minus_mu);
+        return muon_update(g, m, mu, nesterov);
+    }
+    __device__ __forceinline__ float4 update(float4 g, float4 &m) const {
+        return make_float4(update(g.x, m.x), update(g.y, m.y), update(g.z, m.z), update(g.w, m.w));
+    }
+};
 
 __device__ __forceinline__ double block_sum(double v) {
     __shared__ double part[kNormThreads / 32];
@@ -56,19 +85,44 @@ __device__ __forceinline__ double block_sum(double v) {
     return v;
 }
 
-// Sums of squares of the chunks of each matrix, in 64 bits and a fixed order.
+// Sums of squares of the chunks (a multiple of 4 values) of each matrix, in 64 bits and a fixed order.
+template <typename T, typename M, bool MUON>
 __global__ void __launch_bounds__(kNormThreads)
-    ortho_norm_kernel(OrthoSource src, const __grid_constant__ MuonTable tab, size_t numel, int chunks, double *partial,
-                      int *error) {
+    ortho_norm_kernel(const void *x, const __grid_constant__ MuonTable tab, size_t numel, size_t chunk_size, int chunks,
+                      double *partial, int *error) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (blockIdx.x == 0 && threadIdx.x == 0 && error) *error = 0; // nothing has waited yet
     const long long b = blockIdx.x / chunks;
     const int chunk = (int)(blockIdx.x % chunks);
-    const int t = tab.n > 0 ? muon_tensor_of(tab, b) : 0;
-    if (tab.n > 0 && !muon_visible(tab, t, b)) return;
-    const size_t first = (size_t)chunk * kNormChunk, last = min(numel, first + (size_t)kNormChunk);
+    const int t = MUON ? muon_tensor_of(tab, b) : 0;
+    if (MUON && !muon_visible(tab, t, b)) return;
+    const OrthoSource<T, M, MUON> src(x, tab, t, b, numel);
+    const size_t first = (size_t)chunk * chunk_size, last = min(numel, first + chunk_size);
+    const int quads = src.aligned() ? (int)((last - first) / 4) : 0;
+    constexpr int U = 4;
     double s = 0.0;
-    for (size_t e = first + threadIdx.x; e < last; e += kNormThreads) {
-        const double v = source_at(src, tab, t, b, numel, e, false);
+    for (int i0 = threadIdx.x; i0 < quads; i0 += U * kNormThreads) {
+        float4 g[U], m[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            g[u] = m[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (i0 + u * kNormThreads < quads) g[u] = src.get4(first + 4 * (size_t)(i0 + u * kNormThreads), m[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float4 w = src.update(g[u], m[u]);
+            s = fma((double)w.x, (double)w.x, s);
+            s = fma((double)w.y, (double)w.y, s);
+            s = fma((double)w.z, (double)w.z, s);
+            s = fma((double)w.w, (double)w.w, s);
+        }
+    }
+#pragma unroll 4
+    for (size_t e = first + 4 * (size_t)quads + threadIdx.x; e < last; e += kNormThreads) {
+        float m = 0.f;
+        const float g = src.get1(e, m);
+        const double v = src.update(g, m);
         s = fma(v, v, s);
     }
     s = block_sum(s);
@@ -81,21 +135,66 @@ __device__ __forceinline__ double sum_partials(const double *partial, long long 
     return block_sum(s);
 }
 
+__device__ __forceinline__ uint2 pack4(float4 f) {
+    return Quad<__half>::put(f);
+}
+// Four values to both planes; a row has room for whole fours (its length is rounded up to 8).
+__device__ __forceinline__ void planes_put4(const OrthoPlanes &p, size_t at, float4 v) {
+    const uint2 h = pack4(v);
+    const float4 f = Quad<__half>::get(h);
+    *reinterpret_cast<uint2 *>(p.hi + at) = h;
+    *reinterpret_cast<uint2 *>(p.lo + at) = pack4(make_float4(v.x - f.x, v.y - f.y, v.z - f.z, v.w - f.w));
+}
+__device__ __forceinline__ float4 planes_get4(const OrthoPlanes &p, size_t at) {
+    const float4 h = Quad<__half>::get(*reinterpret_cast<const uint2 *>(p.hi + at));
+    const float4 l = Quad<__half>::get(*reinterpret_cast<const uint2 *>(p.lo + at));
+    return make_float4(h.x + l.x, h.y + l.y, h.z + l.z, h.w + l.w);
+}
+
 // planes <- factor * source, in the orientation whose rows are the shorter side.
 // eps > 0: factor = scale / max(norm, eps), and norm_out gets the norm, negated
 // below eps. eps = 0: factor = the power of two that brings the norm to (scale / 2, scale], and
-// norm_out gets the factor.
+// norm_out gets the factor. A block takes 64 x 64 values, a thread four rows of four.
+template <typename T, typename M, bool MUON>
 __global__ void __launch_bounds__(kNormThreads)
-    ortho_split_kernel(OrthoSource src, const __grid_constant__ MuonTable tab, int rows, int cols, int transposed,
+    ortho_split_kernel(const void *x, const __grid_constant__ MuonTable tab, int rows, int cols, int transposed,
                        const double *partial, int chunks, float scale, float eps, float *norm_out, OrthoPlanes out,
                        int tiles_r, int tiles_c) {
     __shared__ float tile[kSplitTile][kSplitTile + 1];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const long long per = (long long)tiles_r * tiles_c;
     const long long b = blockIdx.x / per;
     const int ti = (int)(blockIdx.x % per);
     const int r0 = (ti / tiles_c) * kSplitTile, c0 = (ti % tiles_c) * kSplitTile;
-    const int t = tab.n > 0 ? muon_tensor_of(tab, b) : 0;
-    if (tab.n > 0 && !muon_visible(tab, t, b)) return;
+    const int t = MUON ? muon_tensor_of(tab, b) : 0;
+    if (MUON && !muon_visible(tab, t, b)) return;
+    const bool turned = MUON ? tab.transposed[t] : transposed;
+    if (MUON && turned != (bool)transposed) { // the tensor of the other orientation: its own rows and columns
+        const int k = rows;
+        rows = cols;
+        cols = k;
+    }
+    const int tr0 = MUON && turned != (bool)transposed ? c0 : r0, tc0 = MUON && turned != (bool)transposed ? r0 : c0;
+    const OrthoSource<T, M, MUON> src(x, tab, t, b, (size_t)rows * cols);
+    const bool quads = src.aligned() && cols % 4 == 0;
+    const int q = threadIdx.x % 16 * 4, r = threadIdx.x / 16; // columns q .. q + 3 of rows r, r + 16, ..
+    float4 g[4], m[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const int row = tr0 + r + 16 * u, col = tc0 + q;
+        const size_t e = (size_t)row * cols + col;
+        g[u] = m[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (row >= rows) continue;
+        if (quads) {
+            if (col < cols) g[u] = src.get4(e, m[u]);
+        } else {
+            if (col < cols) g[u].x = src.get1(e, m[u].x);
+            if (col + 1 < cols) g[u].y = src.get1(e + 1, m[u].y);
+            if (col + 2 < cols) g[u].z = src.get1(e + 2, m[u].z);
+            if (col + 3 < cols) g[u].w = src.get1(e + 3, m[u].w);
+        }
+    }
     const float norm = (float)sqrt(sum_partials(partial, b, chunks));
     float div, mul;
     if (eps > 0.f) {
@@ -108,36 +207,60 @@ __global__ void __launch_bounds__(kNormThreads)
         mul = scale * exp2f((float)-e);
         if (ti == 0 && threadIdx.x == 0) norm_out[b] = mul;
     }
-    const size_t numel = (size_t)rows * cols;
-    const int cx = threadIdx.x % kSplitTile, ry = threadIdx.x / kSplitTile;
-    for (int r = ry; r < kSplitTile; r += kNormThreads / kSplitTile)
-        if (r0 + r < rows && c0 + cx < cols)
-            tile[r][cx] = source_at(src, tab, t, b, numel, (size_t)(r0 + r) * cols + c0 + cx, true) / div * mul;
-    __syncthreads();
-    for (int r = ry; r < kSplitTile; r += kNormThreads / kSplitTile) {
-        const int i = transposed ? c0 + r : r0 + r, j = transposed ? r0 + cx : c0 + cx;
-        if (i < (transposed ? cols : rows) && j < (transposed ? rows : cols)) {
-            const float v = transposed ? tile[cx][r] : tile[r][cx];
-            const __half h = __float2half_rn(v);
-            const size_t at = (size_t)b * out.stride + (size_t)i * out.ld + j;
-            out.hi[at] = h;
-            out.lo[at] = __float2half_rn(v - __half2float(h));
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const int row = tr0 + r + 16 * u, col = tc0 + q;
+        if (row >= rows || col >= cols) continue;
+        float4 w = src.update(g[u], m[u]);
+        if (MUON) {
+            M *to = src.mom + (size_t)row * cols + col;
+            if (quads) {
+                *reinterpret_cast<typename Quad<M>::type *>(to) = Quad<M>::put(m[u]);
+            } else {
+                to[0] = from_f32<M>(m[u].x);
+                if (col + 1 < cols) to[1] = from_f32<M>(m[u].y);
+                if (col + 2 < cols) to[2] = from_f32<M>(m[u].z);
+                if (col + 3 < cols) to[3] = from_f32<M>(m[u].w);
+            }
         }
+        w = make_float4(w.x / div * mul, w.y / div * mul, w.z / div * mul, w.w / div * mul);
+        if (!turned) {
+            planes_put4(out, (size_t)b * out.stride + (size_t)row * out.ld + col, w);
+        } else {
+            float *to = &tile[r + 16 * u][q];
+            to[0] = w.x, to[1] = w.y, to[2] = w.z, to[3] = w.w;
+        }
+    }
+    if (!turned) return;
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < 4; ++u) { // the planes' rows are the tensor's columns
+        const int k = r + 16 * u, row = tc0 + k, col = tr0 + q;
+        if (row < cols && col < rows)
+            planes_put4(out, (size_t)b * out.stride + (size_t)row * out.ld + col,
+                        make_float4(tile[q][k], tile[q + 1][k], tile[q + 2][k], tile[q + 3][k]));
     }
 }
 
-// Partial sums of <G, X> over the rows of each matrix (32-bit products of planes).
+// Partial sums of <G, X> over the rows of each matrix, eight values at a time in 64 bits.
 __global__ void __launch_bounds__(kNormThreads)
     ortho_dot_kernel(OrthoPlanes g, OrthoPlanes x, int m, int n, int chunks, double *partial) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const long long b = blockIdx.x / chunks;
     const int chunk = (int)(blockIdx.x % chunks);
+    const int fours = (n + 3) / 4, rows = (m - chunk + chunks - 1) / chunks; // rows chunk, chunk + chunks, ..
     double s = 0.0;
-    for (int i = chunk; i < m; i += chunks)
-        for (int j = threadIdx.x; j < n; j += kNormThreads) {
-            const size_t gi = (size_t)b * g.stride + (size_t)i * g.ld + j, xi = (size_t)b * x.stride + (size_t)i * x.ld + j;
-            s += (double)(__half2float(g.hi[gi]) + __half2float(g.lo[gi])) *
-                 (double)(__half2float(x.hi[xi]) + __half2float(x.lo[xi]));
-        }
+#pragma unroll 4
+    for (long long e = threadIdx.x; e < (long long)rows * fours; e += kNormThreads) {
+        const int i = (int)(e / fours), j = 4 * (int)(e - (long long)i * fours);
+        const size_t row = (size_t)(chunk + i * chunks);
+        const float4 u = planes_get4(g, (size_t)b * g.stride + row * g.ld + j), v = planes_get4(x, (size_t)b * x.stride + row * x.ld + j);
+        s = fma((double)u.x, (double)v.x, s);
+        if (j + 1 < n) s = fma((double)u.y, (double)v.y, s);
+        if (j + 2 < n) s = fma((double)u.z, (double)v.z, s);
+        if (j + 3 < n) s = fma((double)u.w, (double)v.w, s);
+    }
     s = block_sum(s);
     if (threadIdx.x == 0) partial[blockIdx.x] = s;
 }
@@ -164,38 +287,69 @@ __global__ void __launch_bounds__(kNormThreads)
 }
 
 // v_x = (G - X0 <G, X0>) / norm, or G / eps for a matrix whose norm is below eps.
+template <typename T>
 __global__ void __launch_bounds__(kNormThreads)
     ortho_grad_out_kernel(OrthoPlanes g, OrthoPlanes x, int rows, int cols, int transposed, const double *partial,
                           int chunks, const float *norms, const float *g_factor, float g_scale, float x_scale, float eps,
-                          void *v_x, int dtype, int tiles_r, int tiles_c, const int *error) {
+                          T *v_x, int tiles_r, int tiles_c, const int *error) {
     __shared__ float tile[kSplitTile][kSplitTile + 1];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const long long per = (long long)tiles_r * tiles_c;
     const long long b = blockIdx.x / per;
     const int ti = (int)(blockIdx.x % per);
-    const int r0 = (ti / tiles_c) * kSplitTile, c0 = (ti % tiles_c) * kSplitTile; // of v_x
+    const int i0 = (ti / tiles_c) * kSplitTile, j0 = (ti % tiles_c) * kSplitTile; // of the planes
+    const int m = transposed ? cols : rows, n = transposed ? rows : cols;
+    const int q = threadIdx.x % 16 * 4, r = threadIdx.x / 16;
+    float4 gv[4], xv[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const int i = i0 + r + 16 * u, j = j0 + q;
+        if (i < m && j < n) {
+            gv[u] = planes_get4(g, (size_t)b * g.stride + (size_t)i * g.ld + j);
+            xv[u] = planes_get4(x, (size_t)b * x.stride + (size_t)i * x.ld + j);
+        }
+    }
     const double dot = sum_partials(partial, b, chunks);
     const float norm = norms[b];
     const bool small = norm < 0.f;
     const float along = small ? 0.f : (float)(dot / ((double)x_scale * x_scale));
     const float div = small ? eps : norm;
-    // g_factor and g_scale are powers of two; one after the other keeps both in range
-    const float f = g_factor[b];
-    const int cx = threadIdx.x % kSplitTile, ry = threadIdx.x / kSplitTile;
-    for (int r = ry; r < kSplitTile; r += kNormThreads / kSplitTile) {
-        const int i = transposed ? c0 + r : r0 + r, j = transposed ? r0 + cx : c0 + cx;
-        if (i < (transposed ? cols : rows) && j < (transposed ? rows : cols)) {
-            const size_t gi = (size_t)b * g.stride + (size_t)i * g.ld + j, xi = (size_t)b * x.stride + (size_t)i * x.ld + j;
-            const float gv = __half2float(g.hi[gi]) + __half2float(g.lo[gi]);
-            const float xv = __half2float(x.hi[xi]) + __half2float(x.lo[xi]);
-            const float v = *error ? NAN : fmaf(-xv, along, gv) / g_scale / f / div;
-            if (transposed) tile[cx][r] = v;
-            else tile[r][cx] = v;
+    const float f = g_factor[b]; // f and g_scale are powers of two; one after the other keeps both in range
+    const bool poisoned = *error != 0;
+    auto value = [&](float gw, float xw) { return poisoned ? NAN : fmaf(-xw, along, gw) / g_scale / f / div; };
+    T *out = v_x + (size_t)b * rows * cols;
+    const bool quads = cols % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (4 * sizeof(T)) == 0;
+    auto put = [&](int row, int col, float4 v) {
+        T *to = out + (size_t)row * cols + col;
+        if (quads) {
+            *reinterpret_cast<typename Quad<T>::type *>(to) = Quad<T>::put(v);
+        } else {
+            to[0] = from_f32<T>(v.x);
+            if (col + 1 < cols) to[1] = from_f32<T>(v.y);
+            if (col + 2 < cols) to[2] = from_f32<T>(v.z);
+            if (col + 3 < cols) to[3] = from_f32<T>(v.w);
+        }
+    };
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const int i = i0 + r + 16 * u, j = j0 + q;
+        if (i >= m || j >= n) continue;
+        const float4 v = make_float4(value(gv[u].x, xv[u].x), value(gv[u].y, xv[u].y), value(gv[u].z, xv[u].z),
+                                     value(gv[u].w, xv[u].w));
+        if (!transposed) {
+            put(i, j, v);
+        } else {
+            float *to = &tile[r + 16 * u][q];
+            to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
         }
     }
+    if (!transposed) return;
     __syncthreads();
-    for (int r = ry; r < kSplitTile; r += kNormThreads / kSplitTile)
-        if (r0 + r < rows && c0 + cx < cols)
-            store_from_f32(v_x, (size_t)b * rows * cols + (size_t)(r0 + r) * cols + c0 + cx, dtype, tile[r][cx]);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const int k = r + 16 * u, row = j0 + k, col = i0 + q; // of v_x
+        if (row < rows && col < cols) put(row, col, make_float4(tile[q][k], tile[q + 1][k], tile[q + 2][k], tile[q + 3][k]));
+    }
 }
 
 // --- the plan of one call -----------------------------------------------------
@@ -249,7 +403,8 @@ constexpr double kOrthoMaxTop = 16.0; // larger singular values would leave the 
 struct OrthoPlan {
     int rows, cols, m, n, transposed, steps;
     bool split, backward;
-    int chunks;
+    int chunks;        // of the norm's sum
+    size_t chunk_size; // values
     OrthoScales s;
     int ldx, lda;
     long long px, pa; // elements of one matrix's plane
@@ -269,7 +424,9 @@ static OrthoPlan ortho_plan(int rows, int cols, int dtype, const OrthoCoefficien
     p.steps = co.steps;
     p.backward = backward;
     p.split = dtype != kOrthoBF16 || backward || p.n <= 128;
-    p.chunks = (int)(((long long)rows * cols + kNormChunk - 1) / kNormChunk);
+    const size_t numel = (size_t)rows * cols;
+    p.chunk_size = std::max<size_t>(8192, (numel / 512 + 3) / 4 * 4); // about 512 blocks for a large matrix
+    p.chunks = (int)((numel + p.chunk_size - 1) / p.chunk_size);
     p.s = ortho_scales(co);
     p.ldx = (p.n + 7) / 8 * 8;
     p.lda = (p.m + 7) / 8 * 8;
@@ -321,15 +478,39 @@ struct OrthoBuffers {
     float *da[kOrthoMaxSteps], *db[kOrthoMaxSteps];
 };
 
-static int run_split(const OrthoPlan &p, long long nb, const OrthoSource &src, const MuonTable &tab, float scale,
-                     float eps, float *norm_out, double *partial, const OrthoPlanes &out, int *error, cudaStream_t stream) {
-    ortho_norm_kernel<<<(unsigned)(nb * p.chunks), kNormThreads, 0, stream>>>(src, tab, (size_t)p.rows * p.cols,
-                                                                             p.chunks, partial, error);
-    if (int e = check_launch("ortho_norm_kernel")) return e;
-    const int tr = (p.rows + kSplitTile - 1) / kSplitTile, tc = (p.cols + kSplitTile - 1) / kSplitTile;
-    ortho_split_kernel<<<(unsigned)(nb * tr * tc), kNormThreads, 0, stream>>>(
-        src, tab, p.rows, p.cols, p.transposed, partial, p.chunks, scale, eps, norm_out, out, tr, tc);
-    return check_launch("ortho_split_kernel");
+// f(T, M, is it a Muon step)
+template <typename F> static int with_source(int dtype, const MuonTable &tab, F f) {
+    using std::false_type;
+    using std::true_type;
+    if (tab.n == 0) {
+        if (dtype == kOrthoF32) return f(float(), float(), false_type());
+        if (dtype == kOrthoBF16) return f(__nv_bfloat16(), float(), false_type());
+        return f(__half(), float(), false_type());
+    }
+    if (tab.dtype == kOrthoF32) return f(float(), float(), true_type());
+    if (tab.dtype == kOrthoBF16)
+        return tab.state_dtype == kOrthoF32 ? f(__nv_bfloat16(), float(), true_type()) : f(__nv_bfloat16(), __nv_bfloat16(), true_type());
+    return tab.state_dtype == kOrthoF32 ? f(__half(), float(), true_type()) : f(__half(), __half(), true_type());
+}
+
+static int run_split(const OrthoPlan &p, long long nb, const void *x, int dtype, const MuonTable &tab, float scale, float eps,
+                     float *norm_out, double *partial, const OrthoPlanes &out, int *error, cudaStream_t stream) {
+    return with_source(dtype, tab, [&](auto tv, auto mv, auto muon) {
+        using T = decltype(tv);
+        using M = decltype(mv);
+        constexpr bool kMuon = decltype(muon)::value;
+        if (int e = launch_after(ortho_norm_kernel<T, M, kMuon>, (unsigned)(nb * p.chunks), kNormThreads, 0, stream, "ortho_norm_kernel",
+                                 x, tab, (size_t)p.rows * p.cols, p.chunk_size, p.chunks, partial, error))
+            return e;
+        const int tr = (p.rows + kSplitTile - 1) / kSplitTile, tc = (p.cols + kSplitTile - 1) / kSplitTile;
+        return launch_after(ortho_split_kernel<T, M, kMuon>, (unsigned)(nb * tr * tc), kNormThreads, 0, stream, "ortho_split_kernel",
+                            x, tab, p.rows, p.cols, p.transposed, (const double *)partial, p.chunks, scale, eps, norm_out, out, tr, tc);
+    });
+}
+
+static int run_dot(const OrthoPlan &p, long long nb, const OrthoPlanes &g, const OrthoPlanes &x, double *partial, cudaStream_t stream) {
+    return launch_after(ortho_dot_kernel, (unsigned)(nb * p.chunks), kNormThreads, 0, stream, "ortho_dot_kernel", g, x, p.m, p.n, p.chunks,
+                        partial);
 }
 
 static OrthoGemm gemm_base(const OrthoPlan &p, long long nb, int *error) {
@@ -387,7 +568,7 @@ static OrthoGemm apply_gemm(const OrthoPlan &p, long long nb, float a, double sb
     return g;
 }
 
-static int ortho_tiled_fwd(const OrthoPlan &p, const OrthoCoefficients &co, long long nb, const OrthoSource &src,
+static int ortho_tiled_fwd(const OrthoPlan &p, const OrthoCoefficients &co, long long nb, const void *src,
                            void *y, int dtype, const MuonTable &tab, float eps, char *scratch, cudaStream_t stream) {
     Carver ws{scratch};
     OrthoPlanes x[2] = {ws.planes(nb, p.px, p.ldx), ws.planes(nb, p.px, p.ldx)};
@@ -397,7 +578,7 @@ static int ortho_tiled_fwd(const OrthoPlan &p, const OrthoCoefficients &co, long
     float *norms = ws.take<float>(nb);
     int *error = ws.take<int>(1);
     const MuonTable *t = tab.n > 0 ? &tab : nullptr;
-    if (int e = run_split(p, nb, src, tab, (float)p.s.x, eps, norms, partial, x[0], error, stream)) return e;
+    if (int e = run_split(p, nb, src, dtype, tab, (float)p.s.x, eps, norms, partial, x[0], error, stream)) return e;
     for (int k = 0; k < co.steps; ++k) {
         const OrthoPlanes &from = x[k & 1];
         if (int e = run_poly(p, nb, co.c[k], p.s.b, from, a, b, da, db, t, error, stream)) return e;
@@ -420,8 +601,8 @@ static int ortho_tiled_fwd(const OrthoPlan &p, const OrthoCoefficients &co, long
 // G's scale falls by the power of two above the largest slope |p'| at each
 // step, which bounds how far its norm can grow; it is measured anew before
 // that has cost it its low bits.
-static int ortho_tiled_bwd(const OrthoPlan &p, const OrthoCoefficients &co, long long nb, const OrthoSource &src,
-                           const OrthoSource &v, void *v_x, int dtype, float eps, char *scratch, cudaStream_t stream) {
+static int ortho_tiled_bwd(const OrthoPlan &p, const OrthoCoefficients &co, long long nb, const void *src,
+                           const void *v, void *v_x, int dtype, float eps, char *scratch, cudaStream_t stream) {
     const int K = co.steps;
     Carver ws{scratch};
     OrthoBuffers w;
@@ -442,7 +623,7 @@ static int ortho_tiled_bwd(const OrthoPlan &p, const OrthoCoefficients &co, long
     // both products of G's step accumulate together: (B's scale)(G's) = (T's)(X's).
     // With |G| scaled to at most kPlaneTop, T's scaled bound is worst_t kPlaneTop sb / sx.
     const double sb = std::fmin(p.s.b, pow2_floor(p.s.x / p.s.worst_t));
-    if (int e = run_split(p, nb, src, none, (float)p.s.x, eps, norms, partial, w.x[0], error, stream)) return e;
+    if (int e = run_split(p, nb, src, dtype, none, (float)p.s.x, eps, norms, partial, w.x[0], error, stream)) return e;
     for (int k = 0; k < K; ++k) {
         if (int e = run_poly(p, nb, co.c[k], sb, w.x[k], w.a[k], w.b[k], w.da[k], w.db[k], nullptr, error, stream)) return e;
         if (k + 1 == K) break;
@@ -450,7 +631,7 @@ static int ortho_tiled_bwd(const OrthoPlan &p, const OrthoCoefficients &co, long
         g.out = w.x[k + 1];
         if (int e = ortho_gemm(g, nullptr, stream)) return e;
     }
-    if (int e = run_split(p, nb, v, none, (float)kPlaneTop, 0.f, factor[0], partial, gr[K & 1], nullptr, stream)) return e;
+    if (int e = run_split(p, nb, v, dtype, none, (float)kPlaneTop, 0.f, factor[0], partial, gr[K & 1], nullptr, stream)) return e;
     double grown = 1.0; // G's scale has fallen by this
     for (int k = K - 1; k >= 0; --k) {
         const OrthoPlanes &from = gr[(k + 1) & 1], &to = gr[k & 1];
@@ -487,8 +668,7 @@ static int ortho_tiled_bwd(const OrthoPlan &p, const OrthoCoefficients &co, long
         if (int e = ortho_gemm(h, nullptr, stream)) return e;
         grown /= shrink;
         if (grown < 1.0 / 256 && k > 0) { // the bound is far off by now: measure the norm
-            ortho_dot_kernel<<<(unsigned)(nb * p.chunks), kNormThreads, 0, stream>>>(to, to, p.m, p.n, p.chunks, partial);
-            if (int e = check_launch("ortho_dot_kernel")) return e;
+            if (int e = run_dot(p, nb, to, to, partial, stream)) return e;
             ortho_rescale_kernel<<<(unsigned)(nb * p.chunks), kNormThreads, 0, stream>>>(
                 to, p.m, p.n, p.chunks, partial, (float)kPlaneTop, factor[0], (float)grown, factor[1]);
             if (int e = check_launch("ortho_rescale_kernel")) return e;
@@ -496,13 +676,14 @@ static int ortho_tiled_bwd(const OrthoPlan &p, const OrthoCoefficients &co, long
             grown = 1.0;
         }
     }
-    ortho_dot_kernel<<<(unsigned)(nb * p.chunks), kNormThreads, 0, stream>>>(gr[0], w.x[0], p.m, p.n, p.chunks, partial);
-    if (int e = check_launch("ortho_dot_kernel")) return e;
-    const int tr = (p.rows + kSplitTile - 1) / kSplitTile, tc = (p.cols + kSplitTile - 1) / kSplitTile;
-    ortho_grad_out_kernel<<<(unsigned)(nb * tr * tc), kNormThreads, 0, stream>>>(
-        gr[0], w.x[0], p.rows, p.cols, p.transposed, partial, p.chunks, norms, factor[0], (float)grown, (float)p.s.x, eps,
-        v_x, dtype, tr, tc, error);
-    return check_launch("ortho_grad_out_kernel");
+    if (int e = run_dot(p, nb, gr[0], w.x[0], partial, stream)) return e;
+    const int tr = (p.m + kSplitTile - 1) / kSplitTile, tc = (p.n + kSplitTile - 1) / kSplitTile;
+    return with_source(dtype, none, [&](auto tv, auto, auto) {
+        using T = decltype(tv);
+        return launch_after(ortho_grad_out_kernel<T>, (unsigned)(nb * tr * tc), kNormThreads, 0, stream, "ortho_grad_out_kernel", gr[0],
+                            w.x[0], p.rows, p.cols, p.transposed, (const double *)partial, p.chunks, (const float *)norms,
+                            (const float *)factor[0], (float)grown, (float)p.s.x, eps, static_cast<T *>(v_x), tr, tc, (const int *)error);
+    });
 }
 
 static int check_common(const char *what, long long batch, int rows, int cols, int dtype, int steps,
@@ -574,8 +755,7 @@ extern "C" int gsb_orthogonalize_fwd(long long batch, int rows, int cols, int dt
     const long long chunk = ortho_chunk(p, batch);
     const MuonTable none = {};
     for (long long b = 0; b < batch; b += chunk) {
-        const OrthoSource src = {at_matrix(x, b, rows, cols, dtype), dtype};
-        if (int e = ortho_tiled_fwd(p, co, std::min(chunk, batch - b), src,
+        if (int e = ortho_tiled_fwd(p, co, std::min(chunk, batch - b), at_matrix(x, b, rows, cols, dtype),
                                     const_cast<char *>(at_matrix(y, b, rows, cols, dtype)), dtype, none, eps,
                                     static_cast<char *>(scratch), stream))
             return e;
@@ -595,8 +775,8 @@ extern "C" int gsb_orthogonalize_bwd(long long batch, int rows, int cols, int dt
         return set_error(kErrInvalidArgument, "orthogonalize: %zu scratch bytes are needed", plan_bytes(p, batch));
     const long long chunk = ortho_chunk(p, batch);
     for (long long b = 0; b < batch; b += chunk) {
-        const OrthoSource src = {at_matrix(x, b, rows, cols, dtype), dtype}, v = {at_matrix(v_y, b, rows, cols, dtype), dtype};
-        if (int e = ortho_tiled_bwd(p, co, std::min(chunk, batch - b), src, v,
+        if (int e = ortho_tiled_bwd(p, co, std::min(chunk, batch - b), at_matrix(x, b, rows, cols, dtype),
+                                    at_matrix(v_y, b, rows, cols, dtype),
                                     const_cast<char *>(at_matrix(v_x, b, rows, cols, dtype)), dtype, eps,
                                     static_cast<char *>(scratch), stream))
             return e;
@@ -618,6 +798,7 @@ static MuonTable table_part(const MuonTable &all, long long from, long long n, i
         t.lr[t.n] = all.lr[i];
         t.decay[t.n] = all.decay[i];
         t.inner[t.n] = all.inner[i];
+        t.transposed[t.n] = all.transposed[i];
         t.skipped[t.n] = all.skipped[i] + skip;
         t.first[t.n] = lo - from;
         ++t.n;
@@ -649,41 +830,49 @@ extern "C" int gsb_muon(int n_tensors, const GsbMuonTensor *tensors, int rows, i
         if (!clustered && (scratch == nullptr || scratch_bytes < plan_bytes(p, total)))
             return set_error(kErrInvalidArgument, "muon: %zu scratch bytes are needed", plan_bytes(p, total));
     }
-    for (int at = 0; at < n_tensors; at += kOrthoMaxTensors) {
-        MuonTable t = {};
-        t.dtype = dtype;
-        t.state_dtype = state_dtype;
-        t.nesterov = nesterov;
-        t.mu = momentum;
-        t.one_minus_mu = (float)(1.0 - (double)momentum);
-        t.valid = valid;
-        for (int i = at; i < n_tensors && i < at + kOrthoMaxTensors; ++i) {
-            if (tensors[i].batch == 0) continue;
+    MuonTable t = {};
+    t.dtype = dtype;
+    t.state_dtype = state_dtype;
+    t.nesterov = nesterov;
+    t.mu = momentum;
+    t.one_minus_mu = (float)(1.0 - (double)momentum);
+    t.valid = valid;
+    auto run = [&](bool turned) -> int { // the tensors gathered in t
+        if (t.n == 0) return kOk;
+        int e = kOk;
+        const int r = turned ? cols : rows, c = turned ? rows : cols;
+        if (thin) {
+            e = ortho_thin_muon(t, r, c, co, eps, stream);
+        } else if (clustered) {
+            e = ortho_cluster_muon(t, r, c, co, (float)p.s.x, (float)p.s.a, (float)p.s.b, eps, stream);
+        } else {
+            const long long here = t.first[t.n], chunk = ortho_chunk(p, total);
+            for (long long b = 0; b < here && e == kOk; b += chunk) {
+                const long long n = std::min(chunk, here - b);
+                e = ortho_tiled_fwd(p, co, n, nullptr, nullptr, dtype, table_part(t, b, n, rows, cols), eps,
+                                    static_cast<char *>(scratch), stream);
+            }
+        }
+        t.n = 0;
+        return e;
+    };
+    // the tiled path takes both orientations together, the others one after the other
+    for (int pass = 0; pass < (thin || clustered ? 2 : 1); ++pass) {
+        for (int i = 0; i < n_tensors; ++i) {
+            const bool turned = tensors[i].turned != 0;
+            if (tensors[i].batch == 0 || ((thin || clustered) && turned != (pass == 1))) continue;
             t.param[t.n] = tensors[i].param;
             t.grad[t.n] = tensors[i].grad;
             t.momentum[t.n] = tensors[i].momentum_buffer;
             t.lr[t.n] = tensors[i].lr;
             t.decay[t.n] = tensors[i].decay;
             t.inner[t.n] = tensors[i].inner;
+            t.transposed[t.n] = turned != (rows > cols);
             t.first[t.n + 1] = t.first[t.n] + tensors[i].batch;
-            ++t.n;
+            if (++t.n == kOrthoMaxTensors)
+                if (int e = run(pass == 1)) return e;
         }
-        if (t.n == 0) continue;
-        if (thin) {
-            if (int e = ortho_thin_muon(t, rows, cols, co, eps, stream)) return e;
-            continue;
-        }
-        if (clustered) {
-            if (int e = ortho_cluster_muon(t, rows, cols, co, (float)p.s.x, (float)p.s.a, (float)p.s.b, eps, stream)) return e;
-            continue;
-        }
-        const long long here = t.first[t.n], chunk = ortho_chunk(p, total);
-        for (long long b = 0; b < here; b += chunk) {
-            const long long n = std::min(chunk, here - b);
-            if (int e = ortho_tiled_fwd(p, co, n, OrthoSource{nullptr, dtype}, nullptr, dtype,
-                                        table_part(t, b, n, rows, cols), eps, static_cast<char *>(scratch), stream))
-                return e;
-        }
+        if (int e = run(pass == 1)) return e;
     }
     return kOk;
 }

@@ -64,6 +64,7 @@ class GsbMuonTensor(ctypes.Structure):
         ("momentum_buffer", P),
         ("batch", I64),
         ("inner", I32),
+        ("turned", I32),
         ("lr", F32),
         ("decay", F32),
     ]

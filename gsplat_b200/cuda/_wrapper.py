@@ -215,7 +215,7 @@ def muon(
     ``nesterov``, else m; param = param (1 - lr weight_decay) - lr ``orthogonalize(u)``. Gradients have
     their parameter's type (float32, bfloat16 or float16), buffers that type or float32. As in :func:`adam`, ``valid``
     masks the leading dimension, which all params then share (three dimensions or more): masked matrices keep their parameter
-    and momentum. Tensors of one shape and type go through the kernels together. A tensor must not be listed
+    and momentum. Tensors of one type and one shape (or its transpose) go through the kernels together. A tensor must not be listed
     twice or overlap another.
     """
     if isinstance(params, Tensor):
@@ -257,8 +257,9 @@ def muon(
             continue
         batch = math.prod(p.shape[:-2])
         inner = batch // p.shape[0] if p.dim() > 2 else 1
-        groups.setdefault((p.shape[-2], p.shape[-1], dtype, _ORTHO_DTYPES[m.dtype]), []).append(
-            (p, g, m, batch, inner, rate))
+        rows, cols = p.shape[-2:]
+        groups.setdefault((min(rows, cols), max(rows, cols), dtype, _ORTHO_DTYPES[m.dtype]), []).append(
+            (p, g, m, batch, inner, int(rows > cols), rate))
     read_end = write_end = 0
     for start, end, read_only in sorted(spans):
         if start < write_end or (not read_only and start < read_end):
@@ -270,14 +271,13 @@ def muon(
     with device_guard(device):
         for (rows, cols, dtype, state_dtype), entries in groups.items():
             arr = (_B.GsbMuonTensor * len(entries))()
-            for i, (p, g, m, batch, inner, rate) in enumerate(entries):
-                arr[i] = _B.GsbMuonTensor(p.data_ptr(), g.data_ptr(), m.data_ptr(), batch, inner, rate,
+            for i, (p, g, m, batch, inner, turned, rate) in enumerate(entries):
+                arr[i] = _B.GsbMuonTensor(p.data_ptr(), g.data_ptr(), m.data_ptr(), batch, inner, turned, rate,
                                           1.0 - rate * weight_decay)
             scratch = _ortho_scratch(sum(e[3] for e in entries), rows, cols, dtype, steps, False, device)
             call("gsb_muon", len(entries), arr, rows, cols, dtype, state_dtype, ptr(valid), momentum, int(nesterov),
                  steps, coefficients, eps, ptr(scratch), scratch.numel(), stream_of(params[0]))
-            for p, _, m, _, _, _ in entries:
-                torch.autograd.graph.increment_version((p, m))
+            torch.autograd.graph.increment_version([t for e in entries for t in (e[0], e[2])])
 
 
 # ---------------------------------------------------------------------------

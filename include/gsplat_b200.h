@@ -467,8 +467,8 @@ GSB_API int gsb_adam_multi(int n_groups, const GsbAdamGroup *groups, const bool 
  * a singular value in [0, 1] above 16 are refused. Matrices are multiplied with
  * 22 significand bits; bfloat16 ones with a side above 128 with 11.
  * gsb_orthogonalize_bwd: v_x = the gradient of x for the gradient v_y of y.
- * gsb_muon: for the listed tensors, each a batch of matrices of one shape and
- * type: m <- m + (1 - momentum)(grad - m); u = grad + momentum (m - grad) (nesterov)
+ * gsb_muon: for the listed tensors, each a batch of matrices of one shape (or its
+ * transpose) and type: m <- m + (1 - momentum)(grad - m); u = grad + momentum (m - grad) (nesterov)
  * or m; param <- decay * param - lr * orthogonalized(u). momentum_buffer has
  * the type of param or float32 (state_dtype). valid (optional): a row of a tensor's leading
  * dimension (`inner` matrices) whose entry is false is neither read nor
@@ -489,6 +489,7 @@ typedef struct GsbMuonTensor {
     void *momentum_buffer;
     long long batch; /* matrices */
     int inner;       /* matrices of one row of the leading dimension */
+    int turned;      /* the tensor's matrices are [cols, rows] */
     float lr;
     float decay;     /* 1 - lr * weight_decay */
 } GsbMuonTensor;

@@ -236,7 +236,8 @@ def test_muon_valid(shape):
 
 
 def test_muon_list_of_shapes_matches_one_by_one():
-    shapes = [(64, 35), (64, 64), (64, 64), (3, 64), (200, 130), (9, 15, 3), (200, 130), (0, 4), (2, 200, 130)]
+    shapes = [(64, 35), (64, 64), (64, 64), (3, 64), (200, 130), (9, 15, 3), (200, 130), (0, 4), (2, 200, 130), (130, 200), (64, 3), (35, 64),
+              (2, 3, 130, 200), (3, 15, 9)]
     ps, grads, ms = ([data(s, torch.float32, 30 + 3 * i + j).cuda() for i, s in enumerate(shapes)] for j in range(3))
     alone = [(p.clone(), m.clone()) for p, m in zip(ps, ms)]
     lrs = [0.01 * (i + 1) for i in range(len(shapes))]

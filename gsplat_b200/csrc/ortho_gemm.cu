@@ -1,5 +1,6 @@
 // Tensor maps and the choice of a tile for the products of ortho_gemm.cuh.
 #include "ortho_gemm.cuh"
+#include "ortho_gemm_pair.cuh"
 
 namespace gsb {
 
@@ -39,9 +40,16 @@ static int sm_count() {
 int ortho_gemm(const OrthoGemm &g, const MuonTable *table, cudaStream_t stream) {
     if (encode_fn() == nullptr) return set_error(kErrUnsupported, "orthogonalize: the driver offers no tensor maps");
     GemmMaps maps;
-    // narrow tiles where the wide ones would leave half of the SMs idle
+    // The tile with the least time for its rounds over the SMs. A round of 256 x 256 tiles takes a pair of SMs 130 cycles
+    // for 16 deep, one of 128 x 128 tiles an SM 107 (split) or 126, bound by shared memory. Narrow
+    // tiles where the wide ones would leave half of the SMs idle.
     const int sms = sm_count(), tm = (g.M + kBM - 1) / kBM, tn = (g.N + 127) / 128;
-    const int bn = g.batch * (g.symmetric ? tm * (tm + 1) / 2 : tm * tn) <= sms / 2 ? 64 : 128;
+    const int pm = (g.M + kPair - 1) / kPair, pn = (g.N + kPair - 1) / kPair;
+    const long long n128 = g.batch * (g.symmetric ? tm * (tm + 1) / 2 : tm * tn);
+    const long long n256 = g.batch * (g.symmetric ? pm * (pm + 1) / 2 : pm * pn);
+    const long long t128 = (n128 + sms - 1) / sms * (g.split ? 107 : 126), t256 = (n256 + sms / 2 - 1) / (sms / 2) * 130;
+    const bool pair = t256 < t128;
+    const int bn = !pair && n128 <= sms / 2 ? 64 : 128;
     for (int i = 0; i < g.pairs; ++i) {
         const int qr = g.q_k_major ? g.N : g.K, qc = g.q_k_major ? g.K : g.N, qb = g.q_k_major ? bn : 64;
         if (!encode(&maps.p_hi[i], g.p[i].hi, g.p[i], g.M, g.K, g.batch, kBM) ||
@@ -58,6 +66,7 @@ int ortho_gemm(const OrthoGemm &g, const MuonTable *table, cudaStream_t stream) 
     }
     static const MuonTable none = {};
     const MuonTable &tab = table ? *table : none;
+    if (pair) return g.split ? ortho_pair_launch<true>(g, maps, tab, sms, stream) : ortho_pair_launch<false>(g, maps, tab, sms, stream);
     if (bn == 64)
         return g.split ? ortho_gemm_launch<true, 64>(g, maps, tab, sms, stream) : ortho_gemm_launch<false, 64>(g, maps, tab, sms, stream);
     return g.split ? ortho_gemm_launch<true, 128>(g, maps, tab, sms, stream) : ortho_gemm_launch<false, 128>(g, maps, tab, sms, stream);

@@ -113,18 +113,117 @@ template <int BN> __device__ __forceinline__ TileAt tile_at(long long t, int per
     return r;
 }
 
+// What an epilogue reads and writes.
+template <bool SPLIT, int EPI> struct Epilogue {
+    static constexpr bool symmetric = EPI == kEpiGram || EPI == kEpiSquare || EPI == kEpiSym || EPI == kEpiAnti;
+    static constexpr bool element = EPI != kEpiGram && EPI != kEpiSym; // reads e
+    static constexpr bool row_diag = element;                         // and the diagonal at its row
+    static constexpr bool col_diag = EPI == kEpiSquare || EPI == kEpiAnti;
+    static constexpr bool element_lo = SPLIT || !symmetric;
+    static constexpr bool to_planes = EPI != kEpiOut && EPI != kEpiMuon;
+    static constexpr bool out_lo = SPLIT || EPI == kEpiApply;
+};
+
+// The epilogue of 32 columns from j of a lane's row i, the accumulator's values in v. e: the element-wise
+// operand; di, dj: the diagonal at the row, and at the lane's one of the columns. stage: the warp's shared memory.
+template <bool SPLIT, int EPI>
+__device__ __forceinline__ void finish32(const OrthoGemm &g, const MuonTable &tab, int tensor, long long b, int i, int j, int lane,
+                                         float v[32], const Eight e[4], float di, float dj, bool mirror, bool poisoned, float *stage) {
+    using E = Epilogue<SPLIT, EPI>;
+    const bool in_rows = i < g.M;
+    const size_t out_row = (size_t)b * g.out.stride + (size_t)i * g.out.ld + j;
+#pragma unroll
+    for (int c = 0; c < 32; c += 8) {
+        float *w = v + c, x[8];
+        if (E::element) unpack8<E::element_lo>(e[c / 8], x);
+        float on = 0.f;
+        bool diagonal = false;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const bool here = (EPI == kEpiGram || EPI == kEpiSquare) && i == j + c + k;
+            on = here ? w[k] : on;
+            diagonal |= here;
+            if (EPI == kEpiGram || EPI == kEpiSym) {
+                w[k] *= g.c[0];
+            } else if (E::col_diag) {
+                const float d = __shfl_sync(0xffffffffu, dj, c + k);
+                w[k] = fmaf(fmaf(g.c[1], di + d, g.c[0]), x[k], g.c[2] * w[k]);
+            } else {
+                w[k] = fmaf(g.c[0] + di, x[k], g.c[1] * w[k]) * g.c[2];
+            }
+            if (here) w[k] = 0.f;
+        }
+        if (diagonal && in_rows)
+            g.diag_out[(size_t)b * g.M + i] = EPI == kEpiGram ? g.c[1] * on : fmaf(g.c[3], di, fmaf(g.c[4] * di, di, g.c[5] * on));
+        if (E::to_planes && in_rows && j + c < g.N) {
+            store8<E::out_lo>(g.out, out_row + c, w);
+            if (E::symmetric && mirror) { // blocks off the diagonal have all their columns
+                __half *mh = g.out.hi + (size_t)b * g.out.stride + (size_t)(j + c) * g.out.ld + i;
+                __half *ml = g.out.lo + (mh - g.out.hi);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const __half h = __float2half_rn(w[k]);
+                    mh[(size_t)k * g.out.ld] = h;
+                    if (E::out_lo) ml[(size_t)k * g.out.ld] = __float2half_rn(w[k] - __half2float(h));
+                }
+            }
+        }
+    }
+    if (E::to_planes) return;
+    const bool turned = EPI == kEpiMuon ? tab.transposed[tensor] : (bool)g.transposed;
+    const size_t base = (size_t)(b - (EPI == kEpiMuon ? tab.first[tensor] : 0)) * g.M * g.N;
+    void *to = EPI == kEpiMuon ? tab.param[tensor] : g.y;
+    const int dtype = EPI == kEpiMuon ? tab.dtype : g.dtype;
+    const float lr = EPI == kEpiMuon ? tab.lr[tensor] : 0.f, decay = EPI == kEpiMuon ? tab.decay[tensor] : 0.f;
+    // neighbouring lanes at neighbouring places of the tensor: with a transposed tensor the lanes' rows are;
+    // else the values are turned through shared memory
+    if (!turned) {
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 32; ++k) stage[lane * kStagePitch + k] = v[k];
+        __syncwarp();
+    }
+    const int n = turned ? g.N - j : g.M - (i - lane);       // turns: columns, or rows
+    const bool lane_in = turned ? in_rows : lane < g.N - j; // the lane's row, or column
+    const size_t at0 = base + (turned ? (size_t)j * g.M + i : (size_t)(i - lane) * g.N + j + lane);
+    const size_t step = turned ? g.M : g.N;
+    if (!lane_in) return;
+#pragma unroll
+    for (int k0 = 0; k0 < 32; k0 += 8) {
+        float p[8];
+        if (EPI == kEpiMuon) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) p[k] = k0 + k < n ? load_as_f32(to, at0 + (k0 + k) * step, dtype) : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (k0 + k >= n) continue;
+            float r = turned ? v[k0 + k] : stage[(k0 + k) * kStagePitch + lane];
+            if (poisoned) r = NAN;
+            store_from_f32(to, at0 + (k0 + k) * step, dtype, EPI == kEpiMuon ? muon_param(p[k], r, lr, decay) : r);
+        }
+    }
+}
+
+// The operand e of 32 columns, or nothing past the matrix.
+template <bool SPLIT, int EPI>
+__device__ __forceinline__ void fetch32(const OrthoGemm &g, long long b, int i, int j, Eight e[4]) {
+    using E = Epilogue<SPLIT, EPI>;
+    if (!E::element || i >= g.M) return;
+    const size_t at = (size_t)b * g.e.stride + (size_t)i * g.e.ld + j;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+        if (j + 8 * c < g.N) e[c] = load8<E::element_lo>(g.e, at + 8 * c);
+}
+
 template <bool SPLIT, int BN, int EPI>
 __global__ void __launch_bounds__(kGemmThreads, 1)
     ortho_gemm_kernel(const __grid_constant__ OrthoGemm g, const __grid_constant__ GemmMaps maps,
                       const __grid_constant__ MuonTable tab, int per, int tiles_n, long long tiles) {
     using Stage = Stages<SPLIT, BN>;
     constexpr int kStages = Stage::n;
-    constexpr bool kSymmetric = EPI == kEpiGram || EPI == kEpiSquare || EPI == kEpiSym || EPI == kEpiAnti;
-    constexpr bool kQDepthMajor = kSymmetric;
-    constexpr bool kElement = EPI != kEpiGram && EPI != kEpiSym;             // reads e
-    constexpr bool kElementLo = SPLIT || EPI == kEpiApply || EPI == kEpiOut || EPI == kEpiMuon;
-    constexpr bool kToPlanes = EPI != kEpiOut && EPI != kEpiMuon;
-    constexpr bool kOutLo = SPLIT || EPI == kEpiApply;
+    using E = Epilogue<SPLIT, EPI>;
+    constexpr bool kSymmetric = E::symmetric, kQDepthMajor = kSymmetric;
     constexpr int W = BN / 2; // columns of a warp
     extern __shared__ char raw[];
     __shared__ GemmShared sh;
@@ -256,7 +355,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         // the epilogue: warp w has rows 32 (w % 4) .., columns W (w / 4) ..
         const int row = 32 * (warp % 4) + lane, half = warp / 4;
         float *out_stage = reinterpret_cast<float *>(raw + (stage0 - smem_u32(raw)) + kStages * Stage::bytes) + warp * 32 * kStagePitch;
-        const bool poisoned = !kToPlanes && *(volatile const int *)g.error != 0;
+        const bool poisoned = !E::to_planes && *(volatile const int *)g.error != 0;
         int acc = 0;
         uint32_t acc_phase = 0;
         bool ok = true;
@@ -265,21 +364,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             const int tensor = tab.n > 0 ? muon_tensor_of(tab, at.b) : 0;
             if (tab.n > 0 && !muon_visible(tab, tensor, at.b)) continue;
             const int i = at.i * kBM + row, j = at.j * BN + half * W;
-            const bool in_rows = i < g.M;
             // what the epilogue needs is read while the products run
             Eight e[W / 8];
-            float di = 0.f, dj[W / 32];
-            if (EPI != kEpiGram && EPI != kEpiSym && in_rows) di = g.diag_in[(size_t)at.b * g.M + i];
-            if (EPI == kEpiSquare || EPI == kEpiAnti) {
+            float di = 0.f, dj[W / 32] = {};
+            if (E::row_diag && i < g.M) di = g.diag_in[(size_t)at.b * g.M + i];
 #pragma unroll
-                for (int c = 0; c < W / 32; ++c)
-                    dj[c] = j + 32 * c + lane < g.N ? g.diag_in[(size_t)at.b * g.M + j + 32 * c + lane] : 0.f;
-            }
-            if (kElement && in_rows) {
-                const size_t at_e = (size_t)at.b * g.e.stride + (size_t)i * g.e.ld + j;
-#pragma unroll
-                for (int c = 0; c < W / 8; ++c)
-                    if (j + 8 * c < g.N) e[c] = load8<kElementLo>(g.e, at_e + 8 * c);
+            for (int c = 0; c < W / 32; ++c) {
+                if (E::col_diag && j + 32 * c + lane < g.N) dj[c] = g.diag_in[(size_t)at.b * g.M + j + 32 * c + lane];
+                fetch32<SPLIT, EPI>(g, at.b, i, j + 32 * c, e + 4 * c);
             }
             float v[W];
             for (int s0 = 0; s0 < total; s0 += chunk) {
@@ -301,88 +393,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                 if (acc == 0) acc_phase ^= 1u;
             }
             if (!ok) break;
-            const bool mirror = kSymmetric && (at.j * BN) / kBM != at.i; // off the diagonal block
-            const size_t out_row = (size_t)at.b * g.out.stride + (size_t)i * g.out.ld + j;
+            const bool mirror = (at.j * BN) / kBM != at.i; // off the diagonal block
 #pragma unroll
-            for (int c = 0; c < W; c += 8) {
-                float *w = v + c, x[8];
-                if (kElement) unpack8<kElementLo>(e[c / 8], x);
-                float on = 0.f;
-                bool diagonal = false;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    if (EPI == kEpiGram || EPI == kEpiSquare) {
-                        const bool here = i == j + c + k;
-                        on = here ? w[k] : on;
-                        diagonal |= here;
-                    }
-                    if (EPI == kEpiGram || EPI == kEpiSym) {
-                        w[k] *= g.c[0];
-                    } else if (EPI == kEpiSquare || EPI == kEpiAnti) {
-                        const float d = __shfl_sync(0xffffffffu, dj[c / 32], (c + k) & 31);
-                        w[k] = fmaf(fmaf(g.c[1], di + d, g.c[0]), x[k], g.c[2] * w[k]);
-                    } else {
-                        w[k] = fmaf(g.c[0] + di, x[k], g.c[1] * w[k]) * g.c[2];
-                    }
-                    if (EPI == kEpiGram || EPI == kEpiSquare) w[k] = i == j + c + k ? 0.f : w[k];
-                }
-                if ((EPI == kEpiGram || EPI == kEpiSquare) && diagonal && in_rows)
-                    g.diag_out[(size_t)at.b * g.M + i] =
-                        EPI == kEpiGram ? g.c[1] * on : fmaf(g.c[3], di, fmaf(g.c[4] * di, di, g.c[5] * on));
-                if (kToPlanes && in_rows && j + c < g.N) {
-                    store8<kOutLo>(g.out, out_row + c, w);
-                    if (mirror) { // tiles off the diagonal have all their columns
-                        __half *mh = g.out.hi + (size_t)at.b * g.out.stride + (size_t)(j + c) * g.out.ld + i;
-                        __half *ml = g.out.lo + (mh - g.out.hi);
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            const __half h = __float2half_rn(w[k]);
-                            mh[(size_t)k * g.out.ld] = h;
-                            if (kOutLo) ml[(size_t)k * g.out.ld] = __float2half_rn(w[k] - __half2float(h));
-                        }
-                    }
-                }
-            }
-            if (!kToPlanes) {
-                const size_t base = (size_t)(at.b - (EPI == kEpiMuon ? tab.first[tensor] : 0)) * g.M * g.N;
-                const bool turned = EPI == kEpiMuon ? tab.transposed[tensor] : (bool)g.transposed;
-                const int rows_left = g.M - (at.i * kBM + 32 * (warp % 4));
-                void *to = EPI == kEpiMuon ? tab.param[tensor] : g.y;
-                const int dtype = EPI == kEpiMuon ? tab.dtype : g.dtype;
-                const float lr = EPI == kEpiMuon ? tab.lr[tensor] : 0.f, decay = EPI == kEpiMuon ? tab.decay[tensor] : 0.f;
-                // 32 x 32 values at a time, neighbouring lanes at neighbouring places of the tensor: with a
-                // transposed tensor the lanes' rows are; else the values are turned through shared memory
-#pragma unroll
-                for (int c = 0; c < W; c += 32) {
-                    const int cols_left = g.N - (j + c);
-                    if (!turned) {
-                        __syncwarp();
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) out_stage[lane * kStagePitch + k] = v[c + k];
-                        __syncwarp();
-                    }
-                    const int n = turned ? cols_left : rows_left;            // turns: columns, or rows
-                    const bool lane_in = turned ? in_rows : lane < cols_left; // the lane's row, or column
-                    const size_t at0 = base + (turned ? (size_t)(j + c) * g.M + i
-                                                            : (size_t)(i - lane) * g.N + j + c + lane);
-                    const size_t step = turned ? g.M : g.N;
-                    if (!lane_in) continue;
-#pragma unroll
-                    for (int k0 = 0; k0 < 32; k0 += 8) {
-                        float p[8];
-                        if (EPI == kEpiMuon) {
-#pragma unroll
-                            for (int k = 0; k < 8; ++k) p[k] = k0 + k < n ? load_as_f32(to, at0 + (k0 + k) * step, dtype) : 0.f;
-                        }
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            if (k0 + k >= n) continue;
-                            float r = turned ? v[c + k0 + k] : out_stage[(k0 + k) * kStagePitch + lane];
-                            if (poisoned) r = NAN;
-                            store_from_f32(to, at0 + (k0 + k) * step, dtype, EPI == kEpiMuon ? muon_param(p[k], r, lr, decay) : r);
-                        }
-                    }
-                }
+            for (int c = 0; c < W / 32; ++c) {
+                __syncwarp();
+                finish32<SPLIT, EPI>(g, tab, tensor, at.b, i, j + 32 * c, lane, v + 32 * c, e + 4 * c, di, dj[c], mirror, poisoned, out_stage);
             }
         }
     }

@@ -1,0 +1,5 @@
+#include "ortho_gemm_pair.cuh"
+
+namespace gsb {
+template int ortho_pair_launch<true>(const OrthoGemm &, const GemmMaps &, const MuonTable &, int, cudaStream_t);
+} // namespace gsb

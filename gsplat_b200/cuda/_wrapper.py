@@ -13,6 +13,7 @@ hand-written sm_100a kernels of ``gsplat_b200/csrc``; there is no CPU path.
 """
 
 import ctypes
+import functools
 import math
 import warnings
 from typing import Optional, Tuple
@@ -125,18 +126,28 @@ def _ortho_coefficients(coefficients, steps: int):
     """``coefficients`` (one (a, b, c) for every step, or a list of them) as a C array of steps triples."""
     if not 1 <= steps <= 32:
         raise ValueError(f"steps must be 1 to 32, got {steps}")
-    triples = list(coefficients)
-    if len(triples) == 3 and not any(isinstance(v, (list, tuple)) for v in triples):
+    triples = tuple(tuple(v) if isinstance(v, (list, tuple)) else v for v in coefficients)
+    return _ortho_coefficient_array(triples, steps)
+
+
+@functools.lru_cache(maxsize=64)
+def _ortho_coefficient_array(triples, steps: int):
+    if len(triples) == 3 and not any(isinstance(v, tuple) for v in triples):
         triples = [triples] * steps
-    if len(triples) != steps or any(len(t) != 3 for t in triples):
+    if len(triples) != steps or any(not isinstance(t, tuple) or len(t) != 3 for t in triples):
         raise ValueError(f"coefficients must be (a, b, c) or a list of steps = {steps} such triples")
     flat = [float(v) for t in triples for v in t]
     return (ctypes.c_float * len(flat))(*flat)
 
 
-def _ortho_scratch(batch: int, rows: int, cols: int, dtype: int, steps: int, backward: bool, device) -> Tensor:
-    size = lib().gsb_orthogonalize_scratch_bytes(batch, rows, cols, dtype, steps, int(backward))
-    return torch.empty(size, dtype=torch.uint8, device=device)
+@functools.lru_cache(maxsize=256)
+def _ortho_scratch_bytes(batch: int, rows: int, cols: int, dtype: int, steps: int, backward: bool) -> int:
+    return lib().gsb_orthogonalize_scratch_bytes(batch, rows, cols, dtype, steps, int(backward))
+
+
+def _ortho_scratch(batch: int, rows: int, cols: int, dtype: int, steps: int, backward: bool, device) -> Optional[Tensor]:
+    size = _ortho_scratch_bytes(batch, rows, cols, dtype, steps, backward)
+    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
 
 
 def orthogonalize(
@@ -159,27 +170,35 @@ def orthogonalize(
     _ortho_dtype("x", x)
     if not eps > 0:
         raise ValueError(f"eps must be positive, got {eps}")
-    return _Orthogonalize.apply(x.contiguous(), steps, _ortho_coefficients(coefficients, steps), eps)
+    x = x.contiguous()
+    coefficients = _ortho_coefficients(coefficients, steps)
+    if x.requires_grad and torch.is_grad_enabled():
+        return _Orthogonalize.apply(x, steps, coefficients, eps)
+    return _orthogonalize_fwd(x, steps, coefficients, eps)
+
+
+def _orthogonalize_fwd(x: Tensor, steps: int, coefficients, eps: float) -> Tensor:
+    check_cuda("x", x)
+    rows, cols = x.shape[-2:]
+    batch = math.prod(x.shape[:-2])
+    dtype = _ORTHO_DTYPES[x.dtype]
+    y = torch.empty_like(x)
+    with device_guard(x.device):
+        scratch = _ortho_scratch(batch, rows, cols, dtype, steps, False, x.device)
+        call("gsb_orthogonalize_fwd", batch, rows, cols, dtype, ptr(x), ptr(y), steps, coefficients, eps,
+             ptr(scratch), 0 if scratch is None else scratch.numel(), stream_of(x))
+    return y
 
 
 class _Orthogonalize(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x: Tensor, steps: int, coefficients, eps: float) -> Tensor:
-        check_cuda("x", x)
-        rows, cols = x.shape[-2:]
-        batch = math.prod(x.shape[:-2])
-        dtype = _ORTHO_DTYPES[x.dtype]
-        y = torch.empty_like(x)
-        with device_guard(x.device):
-            scratch = _ortho_scratch(batch, rows, cols, dtype, steps, False, x.device)
-            call("gsb_orthogonalize_fwd", batch, rows, cols, dtype, ptr(x), ptr(y), steps, coefficients, eps,
-                 ptr(scratch), scratch.numel(), stream_of(x))
+        y = _orthogonalize_fwd(x, steps, coefficients, eps)
         ctx.save_for_backward(x)
         ctx.steps, ctx.coefficients, ctx.eps = steps, coefficients, eps
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, v_y: Tensor):
         (x,) = ctx.saved_tensors
         v_y = v_y.contiguous()
@@ -191,11 +210,24 @@ class _Orthogonalize(torch.autograd.Function):
         with device_guard(x.device):
             scratch = _ortho_scratch(batch, rows, cols, dtype, ctx.steps, True, x.device)
             call("gsb_orthogonalize_bwd", batch, rows, cols, dtype, ptr(x), ptr(v_y), ptr(v_x), ctx.steps,
-                 ctx.coefficients, ctx.eps, ptr(scratch), scratch.numel(), stream_of(x))
+                 ctx.coefficients, ctx.eps, ptr(scratch), 0 if scratch is None else scratch.numel(), stream_of(x))
+        if torch.is_grad_enabled():  # create_graph=True
+            v_x = _DifferentiableOnce.apply(v_x, x, v_y)
         return v_x, None, None, None
 
 
-@torch.no_grad()
+class _DifferentiableOnce(torch.autograd.Function):
+    """The gradient of orthogonalize() as a function of its inputs, which refuses to be differentiated."""
+
+    @staticmethod
+    def forward(ctx, v_x: Tensor, x: Tensor, v_y: Tensor) -> Tensor:
+        return v_x.view_as(v_x)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("orthogonalize is differentiable once")
+
+
 def muon(
     params,  # [M, N] or [B, ..., M, N], or a list of them
     param_grads,
@@ -237,29 +269,35 @@ def muon(
         raise ValueError("valid must be a bool tensor [B] on the params' device")
     groups = {}
     spans = []
+    index = params[0].get_device()
     for p, g, m, rate in zip(params, param_grads, momentum_buffers, lrs):
         for name, t in (("param", p), ("param_grad", g), ("momentum_buffer", m)):
-            check_cuda(name, t)
-            if t.device != device:
+            if not (t.is_cuda and t.is_contiguous()):
+                check_cuda(name, t)
+            if t.get_device() != index:
                 raise ValueError("params, param_grads and momentum_buffers must be on one device")
-            if t.numel():
-                spans.append((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), t is g))
-        if p.dim() < 2 or g.shape != p.shape or m.shape != p.shape:
-            raise ValueError(f"param, param_grad and momentum_buffer must be [..., M, N] alike, got {tuple(p.shape)}, "
+        shape = p.shape
+        if len(shape) < 2 or g.shape != shape or m.shape != shape:
+            raise ValueError(f"param, param_grad and momentum_buffer must be [..., M, N] alike, got {tuple(shape)}, "
                              f"{tuple(g.shape)}, {tuple(m.shape)}")
         dtype = _ortho_dtype("param", p)
         if g.dtype != p.dtype or m.dtype not in (p.dtype, torch.float32):
             raise TypeError(f"param_grad must have the param's type and momentum_buffer that or float32, got {p.dtype}, "
                             f"{g.dtype}, {m.dtype}")
-        if valid is not None and (p.dim() < 3 or p.shape[0] != valid.shape[0]):
-            raise ValueError(f"valid [{valid.shape[0]}] does not mask the leading dimension of {tuple(p.shape)}")
-        if p.numel() == 0:
+        if valid is not None and (len(shape) < 3 or shape[0] != valid.shape[0]):
+            raise ValueError(f"valid [{valid.shape[0]}] does not mask the leading dimension of {tuple(shape)}")
+        numel = p.numel()
+        if numel == 0:
             continue
-        batch = math.prod(p.shape[:-2])
-        inner = batch // p.shape[0] if p.dim() > 2 else 1
-        rows, cols = p.shape[-2:]
-        groups.setdefault((min(rows, cols), max(rows, cols), dtype, _ORTHO_DTYPES[m.dtype]), []).append(
-            (p, g, m, batch, inner, int(rows > cols), rate))
+        at_p, at_g, at_m = p.data_ptr(), g.data_ptr(), m.data_ptr()
+        size, state_dtype = numel * (2 if dtype else 4), _ORTHO_DTYPES[m.dtype]
+        spans += ((at_p, at_p + size, False), (at_g, at_g + size, True),
+                  (at_m, at_m + numel * (2 if state_dtype else 4), False))
+        rows, cols = shape[-2:]
+        batch = numel // (rows * cols)
+        inner = batch // shape[0] if len(shape) > 2 else 1
+        key = (cols, rows, dtype, state_dtype) if rows > cols else (rows, cols, dtype, state_dtype)
+        groups.setdefault(key, []).append((at_p, at_g, at_m, batch, inner, rows > cols, rate, 1.0 - rate * weight_decay))
     read_end = write_end = 0
     for start, end, read_only in sorted(spans):
         if start < write_end or (not read_only and start < read_end):
@@ -269,15 +307,13 @@ def muon(
         else:
             write_end = max(write_end, end)
     with device_guard(device):
+        stream = stream_of(params[0])
         for (rows, cols, dtype, state_dtype), entries in groups.items():
-            arr = (_B.GsbMuonTensor * len(entries))()
-            for i, (p, g, m, batch, inner, turned, rate) in enumerate(entries):
-                arr[i] = _B.GsbMuonTensor(p.data_ptr(), g.data_ptr(), m.data_ptr(), batch, inner, turned, rate,
-                                          1.0 - rate * weight_decay)
+            arr = (_B.GsbMuonTensor * len(entries))(*entries)
             scratch = _ortho_scratch(sum(e[3] for e in entries), rows, cols, dtype, steps, False, device)
             call("gsb_muon", len(entries), arr, rows, cols, dtype, state_dtype, ptr(valid), momentum, int(nesterov),
-                 steps, coefficients, eps, ptr(scratch), scratch.numel(), stream_of(params[0]))
-            torch.autograd.graph.increment_version([t for e in entries for t in (e[0], e[2])])
+                 steps, coefficients, eps, ptr(scratch), 0 if scratch is None else scratch.numel(), stream)
+    torch.autograd.graph.increment_version(params + momentum_buffers)
 
 
 # ---------------------------------------------------------------------------

@@ -56,12 +56,6 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, i
 struct Eight {
     uint4 hi, lo;
 };
-template <bool LO> __device__ __forceinline__ Eight load8(const OrthoPlanes &p, size_t at) {
-    Eight r;
-    r.hi = *reinterpret_cast<const uint4 *>(p.hi + at);
-    if (LO) r.lo = *reinterpret_cast<const uint4 *>(p.lo + at);
-    return r;
-}
 template <bool LO> __device__ __forceinline__ void unpack8(const Eight &r, float v[8]) {
     const __half2 *h = reinterpret_cast<const __half2 *>(&r.hi), *l = reinterpret_cast<const __half2 *>(&r.lo);
 #pragma unroll
@@ -76,17 +70,23 @@ template <bool LO> __device__ __forceinline__ void unpack8(const Eight &r, float
         }
     }
 }
-template <bool LO> __device__ __forceinline__ void store8(const OrthoPlanes &p, size_t at, const float v[8]) {
-    uint4 h, l;
-    __half2 *hh = reinterpret_cast<__half2 *>(&h), *ll = reinterpret_cast<__half2 *>(&l);
+__device__ __forceinline__ Eight pack8(const float v[8]) {
+    Eight r;
+    __half2 *h = reinterpret_cast<__half2 *>(&r.hi), *l = reinterpret_cast<__half2 *>(&r.lo);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        hh[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-        const float2 f = __half22float2(hh[i]);
-        ll[i] = __floats2half2_rn(v[2 * i] - f.x, v[2 * i + 1] - f.y);
+        h[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+        const float2 f = __half22float2(h[i]);
+        l[i] = __floats2half2_rn(v[2 * i] - f.x, v[2 * i + 1] - f.y);
     }
-    *reinterpret_cast<uint4 *>(p.hi + at) = h;
-    if (LO) *reinterpret_cast<uint4 *>(p.lo + at) = l;
+    return r;
+}
+
+// A warp's 32 x 32 values of planes, between a lane to a row (as the accumulator lies) and four
+// lanes to a row's 64 bytes (as memory wants it: lane l has piece l % 4 of rows l / 4 + 8 k), through
+// the warp's shared memory: hi, then lo, 2 KiB each, the pieces of a row permuted so that no banks meet.
+__device__ __forceinline__ uint4 *stage_piece(float *stage, int plane, int row, int piece) {
+    return reinterpret_cast<uint4 *>(stage) + plane * 128 + row * 4 + (piece ^ ((row >> 1) & 3));
 }
 
 struct TileAt {
@@ -124,18 +124,22 @@ template <bool SPLIT, int EPI> struct Epilogue {
     static constexpr bool out_lo = SPLIT || EPI == kEpiApply;
 };
 
-// The epilogue of 32 columns from j of a lane's row i, the accumulator's values in v. e: the element-wise
-// operand; di, dj: the diagonal at the row, and at the lane's one of the columns. stage: the warp's shared memory.
+// The epilogue of 32 columns from j of a lane's row i, the accumulator's values in v. di, dj: the diagonal
+// at the row, and at the lane's one of the columns. stage: the warp's shared memory, with the element-wise operand.
 template <bool SPLIT, int EPI>
 __device__ __forceinline__ void finish32(const OrthoGemm &g, const MuonTable &tab, int tensor, long long b, int i, int j, int lane,
-                                         float v[32], const Eight e[4], float di, float dj, bool mirror, bool poisoned, float *stage) {
+                                         float v[32], float di, float dj, bool mirror, bool poisoned, float *stage) {
     using E = Epilogue<SPLIT, EPI>;
     const bool in_rows = i < g.M;
-    const size_t out_row = (size_t)b * g.out.stride + (size_t)i * g.out.ld + j;
 #pragma unroll
     for (int c = 0; c < 32; c += 8) {
         float *w = v + c, x[8];
-        if (E::element) unpack8<E::element_lo>(e[c / 8], x);
+        if (E::element) {
+            Eight r;
+            r.hi = *stage_piece(stage, 0, lane, c / 8);
+            if (E::element_lo) r.lo = *stage_piece(stage, 1, lane, c / 8);
+            unpack8<E::element_lo>(r, x);
+        }
         float on = 0.f;
         bool diagonal = false;
 #pragma unroll
@@ -155,19 +159,35 @@ __device__ __forceinline__ void finish32(const OrthoGemm &g, const MuonTable &ta
         }
         if (diagonal && in_rows)
             g.diag_out[(size_t)b * g.M + i] = EPI == kEpiGram ? g.c[1] * on : fmaf(g.c[3], di, fmaf(g.c[4] * di, di, g.c[5] * on));
-        if (E::to_planes && in_rows && j + c < g.N) {
-            store8<E::out_lo>(g.out, out_row + c, w);
-            if (E::symmetric && mirror) { // blocks off the diagonal have all their columns
+        if (E::to_planes) { // in the place of the lane's own piece of e
+            const Eight r = pack8(w);
+            *stage_piece(stage, 0, lane, c / 8) = r.hi;
+            if (E::out_lo) *stage_piece(stage, 1, lane, c / 8) = r.lo;
+            if (E::symmetric && mirror && in_rows && j + c < g.N) { // blocks off the diagonal have all their columns
                 __half *mh = g.out.hi + (size_t)b * g.out.stride + (size_t)(j + c) * g.out.ld + i;
                 __half *ml = g.out.lo + (mh - g.out.hi);
+                const __half *h = reinterpret_cast<const __half *>(&r.hi), *l = reinterpret_cast<const __half *>(&r.lo);
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    const __half h = __float2half_rn(w[k]);
-                    mh[(size_t)k * g.out.ld] = h;
-                    if (E::out_lo) ml[(size_t)k * g.out.ld] = __float2half_rn(w[k] - __half2float(h));
+                    mh[(size_t)k * g.out.ld] = h[k];
+                    if (E::out_lo) ml[(size_t)k * g.out.ld] = l[k];
                 }
             }
         }
+    }
+    if (E::to_planes) {
+        __syncwarp();
+        const int first = i - lane + lane / 4, col = j + 8 * (lane % 4);
+        const size_t at = (size_t)b * g.out.stride + (size_t)first * g.out.ld + col;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (first + 8 * k < g.M && col < g.N) {
+                *reinterpret_cast<uint4 *>(g.out.hi + at + (size_t)(8 * k) * g.out.ld) = *stage_piece(stage, 0, lane / 4 + 8 * k, lane % 4);
+                if (E::out_lo)
+                    *reinterpret_cast<uint4 *>(g.out.lo + at + (size_t)(8 * k) * g.out.ld) = *stage_piece(stage, 1, lane / 4 + 8 * k, lane % 4);
+            }
+        }
+        __syncwarp();
     }
     if (E::to_planes) return;
     const bool turned = EPI == kEpiMuon ? tab.transposed[tensor] : (bool)g.transposed;
@@ -205,15 +225,33 @@ __device__ __forceinline__ void finish32(const OrthoGemm &g, const MuonTable &ta
     }
 }
 
-// The operand e of 32 columns, or nothing past the matrix.
+// The operand e of the warp's 32 rows and 32 columns from j, four lanes to a row; nothing past the matrix.
 template <bool SPLIT, int EPI>
-__device__ __forceinline__ void fetch32(const OrthoGemm &g, long long b, int i, int j, Eight e[4]) {
+__device__ __forceinline__ void fetch32(const OrthoGemm &g, long long b, int row0, int j, int lane, Eight e[4]) {
     using E = Epilogue<SPLIT, EPI>;
-    if (!E::element || i >= g.M) return;
-    const size_t at = (size_t)b * g.e.stride + (size_t)i * g.e.ld + j;
+    if (!E::element) return;
+    const int first = row0 + lane / 4, col = j + 8 * (lane % 4);
+    const size_t at = (size_t)b * g.e.stride + (size_t)first * g.e.ld + col;
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-        if (j + 8 * c < g.N) e[c] = load8<E::element_lo>(g.e, at + 8 * c);
+    for (int k = 0; k < 4; ++k) {
+        if (first + 8 * k < g.M && col < g.N) {
+            e[k].hi = *reinterpret_cast<const uint4 *>(g.e.hi + at + (size_t)(8 * k) * g.e.ld);
+            if (E::element_lo) e[k].lo = *reinterpret_cast<const uint4 *>(g.e.lo + at + (size_t)(8 * k) * g.e.ld);
+        }
+    }
+}
+
+// And from the registers to the warp's shared memory, for finish32.
+template <bool SPLIT, int EPI> __device__ __forceinline__ void stage32(float *stage, int lane, const Eight e[4]) {
+    using E = Epilogue<SPLIT, EPI>;
+    __syncwarp();
+    if (!E::element) return;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        *stage_piece(stage, 0, lane / 4 + 8 * k, lane % 4) = e[k].hi;
+        if (E::element_lo) *stage_piece(stage, 1, lane / 4 + 8 * k, lane % 4) = e[k].lo;
+    }
+    __syncwarp();
 }
 
 template <bool SPLIT, int BN, int EPI>
@@ -365,14 +403,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             if (tab.n > 0 && !muon_visible(tab, tensor, at.b)) continue;
             const int i = at.i * kBM + row, j = at.j * BN + half * W;
             // what the epilogue needs is read while the products run
-            Eight e[W / 8];
+            Eight e[4];
             float di = 0.f, dj[W / 32] = {};
             if (E::row_diag && i < g.M) di = g.diag_in[(size_t)at.b * g.M + i];
 #pragma unroll
             for (int c = 0; c < W / 32; ++c) {
                 if (E::col_diag && j + 32 * c + lane < g.N) dj[c] = g.diag_in[(size_t)at.b * g.M + j + 32 * c + lane];
-                fetch32<SPLIT, EPI>(g, at.b, i, j + 32 * c, e + 4 * c);
             }
+            fetch32<SPLIT, EPI>(g, at.b, i - lane, j, lane, e);
             float v[W];
             for (int s0 = 0; s0 < total; s0 += chunk) {
                 ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[acc], acc_phase, abort));
@@ -396,8 +434,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             const bool mirror = (at.j * BN) / kBM != at.i; // off the diagonal block
 #pragma unroll
             for (int c = 0; c < W / 32; ++c) {
-                __syncwarp();
-                finish32<SPLIT, EPI>(g, tab, tensor, at.b, i, j + 32 * c, lane, v + 32 * c, e + 4 * c, di, dj[c], mirror, poisoned, out_stage);
+                stage32<SPLIT, EPI>(out_stage, lane, e);
+                if (c + 1 < W / 32) fetch32<SPLIT, EPI>(g, at.b, i - lane, j + 32 * (c + 1), lane, e);
+                finish32<SPLIT, EPI>(g, tab, tensor, at.b, i, j + 32 * c, lane, v + 32 * c, di, dj[c], mirror, poisoned, out_stage);
             }
         }
     }

@@ -214,7 +214,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             Eight e[4];
             float di = 0.f;
             if (E::row_diag && i < g.M) di = g.diag_in[(size_t)at.b * g.M + i];
-            if (!SPLIT) fetch32<SPLIT, EPI>(g, at.b, i, j, e);
+            fetch32<SPLIT, EPI>(g, at.b, i - lane, j, lane, e);
             auto release = [&] {
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
@@ -224,12 +224,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             };
             auto finish = [&](int c, float *v) {
                 const float dj = E::col_diag && j + c + lane < g.N ? g.diag_in[(size_t)at.b * g.M + j + c + lane] : 0.f;
-                if (SPLIT) fetch32<SPLIT, EPI>(g, at.b, i, j + c, e); // the sums leave no registers to read ahead
-                const Eight now[4] = {e[0], e[1], e[2], e[3]};
-                if (!SPLIT && c + 32 < W) fetch32<SPLIT, EPI>(g, at.b, i, j + c + 32, e);
-                __syncwarp();
-                finish32<SPLIT, EPI>(g, tab, tensor, at.b, i, j + c, lane, v, now, di, dj, mirror, poisoned, out_stage);
-                __syncwarp();
+                stage32<SPLIT, EPI>(out_stage, lane, e);
+                if (c + 32 < W) fetch32<SPLIT, EPI>(g, at.b, i - lane, j + c + 32, lane, e);
+                finish32<SPLIT, EPI>(g, tab, tensor, at.b, i, j + c, lane, v, di, dj, mirror, poisoned, out_stage);
             };
             if (SPLIT) { // the sum goes on in registers
                 float v[W];

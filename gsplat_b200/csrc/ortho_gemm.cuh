@@ -124,11 +124,42 @@ template <bool SPLIT, int EPI> struct Epilogue {
     static constexpr bool out_lo = SPLIT || EPI == kEpiApply;
 };
 
+// Where the last step's 32 x 32 values go: a lane's n values, `step` apart. Neighbouring lanes are at
+// neighbouring places of the tensor: with a transposed tensor the lanes' rows are, and a lane has its row's values;
+// else a lane has a column, and the values are turned through shared memory.
+struct OutAt {
+    void *p;
+    size_t at, step;
+    int n, dtype;
+    bool turned;
+};
+template <int EPI>
+__device__ __forceinline__ OutAt out_at(const OrthoGemm &g, const MuonTable &tab, int tensor, long long b, int i, int j, int lane) {
+    OutAt r;
+    r.turned = EPI == kEpiMuon ? tab.transposed[tensor] : (bool)g.transposed;
+    r.p = EPI == kEpiMuon ? tab.param[tensor] : g.y;
+    r.dtype = EPI == kEpiMuon ? tab.dtype : g.dtype;
+    r.at = (size_t)(b - (EPI == kEpiMuon ? tab.first[tensor] : 0)) * g.M * g.N +
+           (r.turned ? (size_t)j * g.M + i : (size_t)(i - lane) * g.N + j + lane);
+    r.step = r.turned ? g.M : g.N;
+    r.n = r.turned ? (i < g.M ? g.N - j : 0) : (lane < g.N - j ? g.M - (i - lane) : 0);
+    return r;
+}
+// The parameters there, read together before they are needed.
+template <int EPI>
+__device__ __forceinline__ void fetch_params(const OrthoGemm &g, const MuonTable &tab, int tensor, long long b, int i, int j, int lane,
+                                             float p[32]) {
+    if (EPI != kEpiMuon) return;
+    const OutAt from = out_at<EPI>(g, tab, tensor, b, i, j, lane);
+#pragma unroll
+    for (int k = 0; k < 32; ++k) p[k] = k < from.n ? load_as_f32(from.p, from.at + k * from.step, from.dtype) : 0.f;
+}
+
 // The epilogue of 32 columns from j of a lane's row i, the accumulator's values in v. di, dj: the diagonal
 // at the row, and at the lane's one of the columns. stage: the warp's shared memory, with the element-wise operand.
 template <bool SPLIT, int EPI>
 __device__ __forceinline__ void finish32(const OrthoGemm &g, const MuonTable &tab, int tensor, long long b, int i, int j, int lane,
-                                         float v[32], float di, float dj, bool mirror, bool poisoned, float *stage) {
+                                         float v[32], const float p[32], float di, float dj, bool mirror, bool poisoned, float *stage) {
     using E = Epilogue<SPLIT, EPI>;
     const bool in_rows = i < g.M;
 #pragma unroll
@@ -190,38 +221,20 @@ __device__ __forceinline__ void finish32(const OrthoGemm &g, const MuonTable &ta
         __syncwarp();
     }
     if (E::to_planes) return;
-    const bool turned = EPI == kEpiMuon ? tab.transposed[tensor] : (bool)g.transposed;
-    const size_t base = (size_t)(b - (EPI == kEpiMuon ? tab.first[tensor] : 0)) * g.M * g.N;
-    void *to = EPI == kEpiMuon ? tab.param[tensor] : g.y;
-    const int dtype = EPI == kEpiMuon ? tab.dtype : g.dtype;
+    const OutAt to = out_at<EPI>(g, tab, tensor, b, i, j, lane);
     const float lr = EPI == kEpiMuon ? tab.lr[tensor] : 0.f, decay = EPI == kEpiMuon ? tab.decay[tensor] : 0.f;
-    // neighbouring lanes at neighbouring places of the tensor: with a transposed tensor the lanes' rows are;
-    // else the values are turned through shared memory
-    if (!turned) {
+    if (!to.turned) {
         __syncwarp();
 #pragma unroll
         for (int k = 0; k < 32; ++k) stage[lane * kStagePitch + k] = v[k];
         __syncwarp();
     }
-    const int n = turned ? g.N - j : g.M - (i - lane);       // turns: columns, or rows
-    const bool lane_in = turned ? in_rows : lane < g.N - j; // the lane's row, or column
-    const size_t at0 = base + (turned ? (size_t)j * g.M + i : (size_t)(i - lane) * g.N + j + lane);
-    const size_t step = turned ? g.M : g.N;
-    if (!lane_in) return;
 #pragma unroll
-    for (int k0 = 0; k0 < 32; k0 += 8) {
-        float p[8];
-        if (EPI == kEpiMuon) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) p[k] = k0 + k < n ? load_as_f32(to, at0 + (k0 + k) * step, dtype) : 0.f;
-        }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            if (k0 + k >= n) continue;
-            float r = turned ? v[k0 + k] : stage[(k0 + k) * kStagePitch + lane];
-            if (poisoned) r = NAN;
-            store_from_f32(to, at0 + (k0 + k) * step, dtype, EPI == kEpiMuon ? muon_param(p[k], r, lr, decay) : r);
-        }
+    for (int k = 0; k < 32; ++k) {
+        if (k >= to.n) continue;
+        float r = to.turned ? v[k] : stage[k * kStagePitch + lane];
+        if (poisoned) r = NAN;
+        store_from_f32(to.p, to.at + k * to.step, to.dtype, EPI == kEpiMuon ? muon_param(p[k], r, lr, decay) : r);
     }
 }
 
@@ -434,9 +447,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             const bool mirror = (at.j * BN) / kBM != at.i; // off the diagonal block
 #pragma unroll
             for (int c = 0; c < W / 32; ++c) {
+                float p[32];
+                fetch_params<EPI>(g, tab, tensor, at.b, i, j + 32 * c, lane, p);
                 stage32<SPLIT, EPI>(out_stage, lane, e);
                 if (c + 1 < W / 32) fetch32<SPLIT, EPI>(g, at.b, i - lane, j + 32 * (c + 1), lane, e);
-                finish32<SPLIT, EPI>(g, tab, tensor, at.b, i, j + 32 * c, lane, v + 32 * c, di, dj[c], mirror, poisoned, out_stage);
+                finish32<SPLIT, EPI>(g, tab, tensor, at.b, i, j + 32 * c, lane, v + 32 * c, p, di, dj[c], mirror, poisoned, out_stage);
             }
         }
     }

@@ -147,14 +147,6 @@ int ortho_thin_bwd(long long batch, int rows, int cols, int dtype, const void *x
 int ortho_thin_muon(const MuonTable &table, int rows, int cols, const OrthoCoefficients &co, float eps,
                     cudaStream_t stream);
 
-// --- short side <= 128 and not too long (ortho_cluster.cu): one launch, the matrix in the
-// shared memory of a cluster. The scales are those of X, A and B as OrthoPlanes have them.
-bool ortho_is_clustered(int rows, int cols);
-int ortho_cluster_fwd(long long batch, int rows, int cols, int dtype, const void *x, void *y, const OrthoCoefficients &co,
-                      float x_scale, float a_scale, float b_scale, float eps, cudaStream_t stream);
-int ortho_cluster_muon(const MuonTable &table, int rows, int cols, const OrthoCoefficients &co, float x_scale,
-                       float a_scale, float b_scale, float eps, cudaStream_t stream);
-
 // --- tiled products (ortho_gemm.cu) ----------------------------------------
 // A matrix of the iteration: value = scale * (hi + lo), both fp16, so 22
 // significand bits. Row-major, rows of `ld` elements (a multiple of 8), one
@@ -164,6 +156,21 @@ struct OrthoPlanes {
     int ld;
     long long stride;
 };
+
+// --- short side <= 128 and not too long (ortho_cluster.cu): one launch, the matrix in the
+// shared memory of a cluster. The scales are those of X, A and B as OrthoPlanes have them.
+bool ortho_is_clustered(int rows, int cols);
+// Where the first step's X, A and B go for a backward pass (x.hi = NULL: nowhere), each further step's
+// `step` halves (2 bytes) behind.
+struct ClusterKept {
+    OrthoPlanes x, a, b;
+    float *da, *db, *norms;
+    long long step;
+};
+int ortho_cluster_fwd(long long batch, int rows, int cols, int dtype, const void *x, void *y, const OrthoCoefficients &co,
+                      float x_scale, float a_scale, float b_scale, float eps, const ClusterKept &kept, cudaStream_t stream);
+int ortho_cluster_muon(const MuonTable &table, int rows, int cols, const OrthoCoefficients &co, float x_scale,
+                       float a_scale, float b_scale, float eps, cudaStream_t stream);
 
 enum OrthoEpilogue : int {
     kEpiGram,   // A: off-diagonal part and its diagonal

@@ -132,7 +132,7 @@ __device__ __forceinline__ void multiply(uint32_t d, uint32_t p, uint32_t p_lo, 
 template <typename T, typename M, bool MUON>
 __global__ void __launch_bounds__(kClusterThreads, 1)
     ortho_cluster_kernel(const __grid_constant__ ClusterShape sh, const T *x_in, T *y, const __grid_constant__ MuonTable tab,
-                         const __grid_constant__ ClusterSteps co, float eps) {
+                         const __grid_constant__ ClusterSteps co, float eps, const __grid_constant__ ClusterKept kept) {
     extern __shared__ char raw[];
     __shared__ alignas(16) float diag_a[kClusterMaxShort];
     __shared__ float diag_b[kClusterMaxShort];
@@ -300,6 +300,23 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
         }
     }
 
+    const bool keep = !MUON && kept.x.hi != nullptr;
+    if (keep && tid == 0 && rank == 0) kept.norms[b] = norm < eps ? -1.f : norm;
+    // rows [r0, r1) and columns up to `used` of a plane pair to memory, 16 bytes at a time
+    auto dump = [&](const char *hi, const char *lo, const OrthoPlanes &to, int step, int r0, int r1, int used, int col0) {
+        const int eights = (used + 7) / 8;
+        __half *out = to.hi + step * kept.step + (size_t)b * to.stride;
+        const ptrdiff_t to_lo = to.lo - to.hi;
+        for (int t = tid; t < (r1 - r0) * eights; t += kClusterThreads) {
+            const int i = r0 + t / eights, c = (t - (i - r0) * eights) * 8;
+            const uint32_t from = plane_byte(sh.m16, i, c);
+            uint4 *at = reinterpret_cast<uint4 *>(out + (size_t)i * to.ld + col0 + c);
+            *at = *reinterpret_cast<const uint4 *>(hi + from);
+            *reinterpret_cast<uint4 *>(reinterpret_cast<__half *>(at) + to_lo) = *reinterpret_cast<const uint4 *>(lo + from);
+        }
+    };
+    const int own0 = sh.blocks > 1 ? min(sh.m, (int)rank * sh.per) : 0, own1 = sh.blocks > 1 ? min(sh.m, own0 + sh.per) : sh.m;
+
     const int row = 32 * (warp % 4) + lane, turn = warp / 4; // columns 16 (turn + 4 k) ..
     const uint32_t acc = tmem + ((uint32_t)(32 * (warp % 4)) << 16);
     const bool rows_here = 32 * (warp % 4) < sh.m16; // the warp has rows (all its lanes read TMEM together)
@@ -329,6 +346,7 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
             multiply(tmem, xh, xl, xh, xl, sh.m16, sh.m16, true, sh.m16, ns16, leader);
             mma_commit(&done, leader);
         }
+        if (keep) dump(x_hi, x_lo, kept.x, step, 0, sh.m, cols, j0);
         const uint32_t owner = mine ? row / sh.per : 0; // of this row of A
         const uint32_t to = sh.blocks > 1 ? remote(smem_u32(partial + ((int)rank * sh.per + row - (int)owner * sh.per) * pitch), owner) : 0u;
         finish();
@@ -391,6 +409,12 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
             multiply(tmem, ah, al, ah, al, sh.m16, sh.m16, true, sh.m16, sh.m16, leader);
             mma_commit(&done, leader);
         }
+        if (keep) {
+            dump(a_hi, a_lo, kept.a, step, own0, own1, sh.m, 0);
+            if (rank == 0 && tid < sh.m)
+                reinterpret_cast<float *>(reinterpret_cast<__half *>(kept.da) + step * kept.step)[(size_t)b * sh.m + tid] = diag_a[tid];
+            __syncthreads(); // B takes A's place
+        }
         float o[16];
         float di = 0.f;
         if (mine) {
@@ -429,6 +453,11 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
                 multiply(tmem + c, ah, al, xh + (c >> 6) * sh.m16 * 128, xl + (c >> 6) * sh.m16 * 128, sh.m16, sh.m16, false,
                          min(256, ns16 - c), sh.m16, leader);
             mma_commit(&done, leader);
+        }
+        if (keep) {
+            dump(a_hi, a_lo, kept.b, step, own0, own1, sh.m, 0);
+            if (rank == 0 && tid < sh.m)
+                reinterpret_cast<float *>(reinterpret_cast<__half *>(kept.db) + step * kept.step)[(size_t)b * sh.m + tid] = diag_b[tid];
         }
         float f = 0.f;
         if (mine) {
@@ -549,7 +578,7 @@ bool ortho_is_clustered(int rows, int cols) { return cluster_blocks(rows, cols) 
 
 template <typename T, typename M, bool MUON>
 static int cluster_launch(long long batch, const ClusterShape &sh, const void *x, void *y, const MuonTable &tab,
-                          const ClusterSteps &steps, float eps, cudaStream_t stream) {
+                          const ClusterSteps &steps, float eps, const ClusterKept &kept, cudaStream_t stream) {
     auto *kernel = ortho_cluster_kernel<T, M, MUON>;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sh.smem) != cudaSuccess)
         return check_launch("ortho_cluster_kernel attributes");
@@ -564,7 +593,7 @@ static int cluster_launch(long long batch, const ClusterShape &sh, const void *x
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, sh, static_cast<const T *>(x), static_cast<T *>(y), tab, steps, eps);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, sh, static_cast<const T *>(x), static_cast<T *>(y), tab, steps, eps, kept);
     if (e != cudaSuccess) return set_error(kErrLaunch, "ortho_cluster_kernel: %s", cudaGetErrorString(e));
     return check_launch("ortho_cluster_kernel");
 }
@@ -589,14 +618,14 @@ static int cluster_plan(const char *what, long long batch, int rows, int cols, c
 }
 
 int ortho_cluster_fwd(long long batch, int rows, int cols, int dtype, const void *x, void *y, const OrthoCoefficients &co,
-                      float x_scale, float a_scale, float b_scale, float eps, cudaStream_t stream) {
+                      float x_scale, float a_scale, float b_scale, float eps, const ClusterKept &kept, cudaStream_t stream) {
     ClusterShape sh;
     ClusterSteps st = {};
     if (int e = cluster_plan("orthogonalize", batch, rows, cols, co, x_scale, a_scale, b_scale, &sh, &st)) return e;
     static const MuonTable none = {};
-    if (dtype == kOrthoF32) return cluster_launch<float, float, false>(batch, sh, x, y, none, st, eps, stream);
-    if (dtype == kOrthoBF16) return cluster_launch<__nv_bfloat16, float, false>(batch, sh, x, y, none, st, eps, stream);
-    return cluster_launch<__half, float, false>(batch, sh, x, y, none, st, eps, stream);
+    if (dtype == kOrthoF32) return cluster_launch<float, float, false>(batch, sh, x, y, none, st, eps, kept, stream);
+    if (dtype == kOrthoBF16) return cluster_launch<__nv_bfloat16, float, false>(batch, sh, x, y, none, st, eps, kept, stream);
+    return cluster_launch<__half, float, false>(batch, sh, x, y, none, st, eps, kept, stream);
 }
 
 int ortho_cluster_muon(const MuonTable &t, int rows, int cols, const OrthoCoefficients &co, float x_scale, float a_scale,
@@ -606,12 +635,12 @@ int ortho_cluster_muon(const MuonTable &t, int rows, int cols, const OrthoCoeffi
     const long long batch = t.first[t.n];
     if (int e = cluster_plan("muon", batch, rows, cols, co, x_scale, a_scale, b_scale, &sh, &st)) return e;
     const bool same = t.dtype == t.state_dtype;
-    if (t.dtype == kOrthoF32) return cluster_launch<float, float, true>(batch, sh, nullptr, nullptr, t, st, eps, stream);
+    if (t.dtype == kOrthoF32) return cluster_launch<float, float, true>(batch, sh, nullptr, nullptr, t, st, eps, ClusterKept{}, stream);
     if (t.dtype == kOrthoBF16)
-        return same ? cluster_launch<__nv_bfloat16, __nv_bfloat16, true>(batch, sh, nullptr, nullptr, t, st, eps, stream)
-                    : cluster_launch<__nv_bfloat16, float, true>(batch, sh, nullptr, nullptr, t, st, eps, stream);
-    return same ? cluster_launch<__half, __half, true>(batch, sh, nullptr, nullptr, t, st, eps, stream)
-                : cluster_launch<__half, float, true>(batch, sh, nullptr, nullptr, t, st, eps, stream);
+        return same ? cluster_launch<__nv_bfloat16, __nv_bfloat16, true>(batch, sh, nullptr, nullptr, t, st, eps, ClusterKept{}, stream)
+                    : cluster_launch<__nv_bfloat16, float, true>(batch, sh, nullptr, nullptr, t, st, eps, ClusterKept{}, stream);
+    return same ? cluster_launch<__half, __half, true>(batch, sh, nullptr, nullptr, t, st, eps, ClusterKept{}, stream)
+                : cluster_launch<__half, float, true>(batch, sh, nullptr, nullptr, t, st, eps, ClusterKept{}, stream);
 }
 
 } // namespace gsb

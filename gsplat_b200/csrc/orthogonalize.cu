@@ -408,13 +408,13 @@ struct OrthoPlan {
     OrthoScales s;
     int ldx, lda;
     long long px, pa; // elements of one matrix's plane
-    size_t per_matrix; // scratch bytes a matrix
-    size_t fixed;      // and for alignment
+    size_t per_matrix, fixed;       // scratch bytes: a matrix's, and for alignment
+    size_t kept_matrix, kept_fixed; // of the state that a backward pass needs
 };
 
 static size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
-static OrthoPlan ortho_plan(int rows, int cols, int dtype, const OrthoCoefficients &co, bool backward) {
+static OrthoPlan ortho_plan(int rows, int cols, int dtype, const OrthoCoefficients &co, bool backward, bool kept) {
     OrthoPlan p = {};
     p.rows = rows;
     p.cols = cols;
@@ -423,7 +423,7 @@ static OrthoPlan ortho_plan(int rows, int cols, int dtype, const OrthoCoefficien
     p.n = p.transposed ? rows : cols;
     p.steps = co.steps;
     p.backward = backward;
-    p.split = dtype != kOrthoBF16 || backward || p.n <= 128;
+    p.split = dtype != kOrthoBF16 || backward || kept || p.n <= 128;
     const size_t numel = (size_t)rows * cols;
     p.chunk_size = std::max<size_t>(8192, (numel / 512 + 3) / 4 * 4); // about 512 blocks for a large matrix
     p.chunks = (int)((numel + p.chunk_size - 1) / p.chunk_size);
@@ -432,16 +432,20 @@ static OrthoPlan ortho_plan(int rows, int cols, int dtype, const OrthoCoefficien
     p.lda = (p.m + 7) / 8 * 8;
     p.px = (long long)p.m * p.ldx;
     p.pa = (long long)p.m * p.lda;
-    const int kept = backward ? co.steps : 1;
     const size_t halves = 2 * sizeof(__half);
-    size_t bytes = 0;
-    bytes += (backward ? kept : 2) * halves * p.px;        // X
-    bytes += 2 * kept * halves * p.pa;                     // O_A, O_B
-    bytes += 2 * kept * sizeof(float) * p.m;               // diagonals
-    bytes += sizeof(double) * (size_t)p.chunks + 3 * sizeof(float);
-    if (backward) bytes += 2 * halves * p.px + 2 * halves * p.pa; // G twice, S, T
+    p.kept_matrix = co.steps * (halves * (p.px + 2 * p.pa) + 2 * sizeof(float) * p.m) + sizeof(float);
+    p.kept_fixed = 256 * (size_t)(8 * co.steps + 2);
+    size_t bytes = sizeof(double) * (size_t)p.chunks + 3 * sizeof(float);
+    if (backward)
+        bytes += 2 * halves * (p.px + p.pa); // G twice, S, T
+    else
+        bytes += 2 * halves * (p.px + p.pa) + 2 * sizeof(float) * p.m; // X twice, A, B, diagonals
     p.per_matrix = bytes;
-    p.fixed = 256 * (size_t)(8 * kept + 24);
+    p.fixed = 256 * 24;
+    if (backward && !kept) {
+        p.per_matrix += p.kept_matrix;
+        p.fixed += p.kept_fixed;
+    }
     return p;
 }
 
@@ -473,9 +477,22 @@ struct Carver {
     }
 };
 
+// What a backward pass needs of the steps: each one's X, A and B, and the norms.
 struct OrthoBuffers {
     OrthoPlanes x[kOrthoMaxSteps], a[kOrthoMaxSteps], b[kOrthoMaxSteps];
     float *da[kOrthoMaxSteps], *db[kOrthoMaxSteps];
+    float *norms;
+
+    OrthoBuffers(Carver &ws, const OrthoPlan &p, long long nb) {
+        for (int k = 0; k < p.steps; ++k) {
+            x[k] = ws.planes(nb, p.px, p.ldx);
+            a[k] = ws.planes(nb, p.pa, p.lda);
+            b[k] = ws.planes(nb, p.pa, p.lda);
+            da[k] = ws.take<float>((size_t)nb * p.m);
+            db[k] = ws.take<float>((size_t)nb * p.m);
+        }
+        norms = ws.take<float>(nb);
+    }
 };
 
 // f(T, M, is it a Muon step)
@@ -596,42 +613,57 @@ static int ortho_tiled_fwd(const OrthoPlan &p, const OrthoCoefficients &co, long
     return kOk;
 }
 
-// The steps again, each one's X, A and B kept, and then back through them:
+// B's scale where the backward pass reads it. There both products of G's step accumulate together: (B's scale)
+// (G's) = (T's)(X's). With |G| scaled to at most kPlaneTop, T's scaled bound is worst_t kPlaneTop sb / sx.
+static double backward_scale(const OrthoPlan &p) { return std::fmin(p.s.b, pow2_floor(p.s.x / p.s.worst_t)); }
+
+// The steps, each one's X, A and B kept; y may be NULL (the last product is then left out).
+static int ortho_tiled_kept(const OrthoPlan &p, const OrthoCoefficients &co, long long nb, const void *src, void *y, int dtype,
+                            const OrthoBuffers &w, float eps, double *partial, int *error, cudaStream_t stream) {
+    const double sb = backward_scale(p);
+    const MuonTable none = {};
+    if (int e = run_split(p, nb, src, dtype, none, (float)p.s.x, eps, w.norms, partial, w.x[0], error, stream)) return e;
+    for (int k = 0; k < co.steps; ++k) {
+        if (int e = run_poly(p, nb, co.c[k], sb, w.x[k], w.a[k], w.b[k], w.da[k], w.db[k], nullptr, error, stream)) return e;
+        OrthoGemm g = apply_gemm(p, nb, co.c[k][0], sb, w.x[k], w.b[k], w.db[k], error);
+        if (k + 1 < co.steps) {
+            g.out = w.x[k + 1];
+        } else if (y) {
+            g.epilogue = kEpiOut;
+            g.c[2] = (float)(1.0 / p.s.x);
+            g.y = y;
+            g.dtype = dtype;
+        } else {
+            break;
+        }
+        if (int e = ortho_gemm(g, nullptr, stream)) return e;
+    }
+    return kOk;
+}
+
+// Back through the steps, kept by the forward pass or taken again here:
 //     S = G X^T + X G^T,  T = b S + c (S A + A S),  G <- a G + B G + T X.
 // G's scale falls by the power of two above the largest slope |p'| at each
 // step, which bounds how far its norm can grow; it is measured anew before
 // that has cost it its low bits.
 static int ortho_tiled_bwd(const OrthoPlan &p, const OrthoCoefficients &co, long long nb, const void *src,
-                           const void *v, void *v_x, int dtype, float eps, char *scratch, cudaStream_t stream) {
+                           const void *v, void *v_x, int dtype, float eps, void *kept, char *scratch, cudaStream_t stream) {
     const int K = co.steps;
-    Carver ws{scratch};
-    OrthoBuffers w;
-    for (int k = 0; k < K; ++k) {
-        w.x[k] = ws.planes(nb, p.px, p.ldx);
-        w.a[k] = ws.planes(nb, p.pa, p.lda);
-        w.b[k] = ws.planes(nb, p.pa, p.lda);
-        w.da[k] = ws.take<float>((size_t)nb * p.m);
-        w.db[k] = ws.take<float>((size_t)nb * p.m);
-    }
+    Carver ws{scratch}, own{static_cast<char *>(kept)};
+    const OrthoBuffers w(kept ? own : ws, p, nb);
     OrthoPlanes gr[2] = {ws.planes(nb, p.px, p.ldx), ws.planes(nb, p.px, p.ldx)};
     const OrthoPlanes s = ws.planes(nb, p.pa, p.lda), t = ws.planes(nb, p.pa, p.lda);
     double *partial = ws.take<double>((size_t)nb * p.chunks);
-    float *norms = ws.take<float>(nb), *factor[2] = {ws.take<float>(nb), ws.take<float>(nb)};
+    float *factor[2] = {ws.take<float>(nb), ws.take<float>(nb)};
+    float *const norms = w.norms;
     int *error = ws.take<int>(1);
     const MuonTable none = {};
     const double shrink = std::exp2(std::ceil(std::log2(p.s.slope)));
-    // both products of G's step accumulate together: (B's scale)(G's) = (T's)(X's).
-    // With |G| scaled to at most kPlaneTop, T's scaled bound is worst_t kPlaneTop sb / sx.
-    const double sb = std::fmin(p.s.b, pow2_floor(p.s.x / p.s.worst_t));
-    if (int e = run_split(p, nb, src, dtype, none, (float)p.s.x, eps, norms, partial, w.x[0], error, stream)) return e;
-    for (int k = 0; k < K; ++k) {
-        if (int e = run_poly(p, nb, co.c[k], sb, w.x[k], w.a[k], w.b[k], w.da[k], w.db[k], nullptr, error, stream)) return e;
-        if (k + 1 == K) break;
-        OrthoGemm g = apply_gemm(p, nb, co.c[k][0], sb, w.x[k], w.b[k], w.db[k], error);
-        g.out = w.x[k + 1];
-        if (int e = ortho_gemm(g, nullptr, stream)) return e;
-    }
-    if (int e = run_split(p, nb, v, dtype, none, (float)kPlaneTop, 0.f, factor[0], partial, gr[K & 1], nullptr, stream)) return e;
+    const double sb = backward_scale(p);
+    if (!kept)
+        if (int e = ortho_tiled_kept(p, co, nb, src, nullptr, dtype, w, eps, partial, error, stream)) return e;
+    if (int e = run_split(p, nb, v, dtype, none, (float)kPlaneTop, 0.f, factor[0], partial, gr[K & 1], kept ? error : nullptr, stream))
+        return e;
     double grown = 1.0; // G's scale has fallen by this
     for (int k = K - 1; k >= 0; --k) {
         const OrthoPlanes &from = gr[(k + 1) & 1], &to = gr[k & 1];
@@ -714,8 +746,8 @@ static void finish_scales(OrthoPlan *p) {
     s.b = pow2_floor(kPlaneTop / std::fmax(s.top_b, 1.0));
 }
 
-static OrthoPlan make_plan(int rows, int cols, int dtype, const OrthoCoefficients &co, bool backward) {
-    OrthoPlan p = ortho_plan(rows, cols, dtype, co, backward);
+static OrthoPlan make_plan(int rows, int cols, int dtype, const OrthoCoefficients &co, bool backward, bool kept) {
+    OrthoPlan p = ortho_plan(rows, cols, dtype, co, backward, kept);
     finish_scales(&p);
     return p;
 }
@@ -728,12 +760,22 @@ static size_t plan_bytes(const OrthoPlan &p, long long batch) {
 
 using namespace gsb;
 
-extern "C" size_t gsb_orthogonalize_scratch_bytes(long long batch, int rows, int cols, int dtype, int steps, int backward) {
+extern "C" size_t gsb_orthogonalize_kept_bytes(long long batch, int rows, int cols, int steps) {
+    if (batch <= 0 || rows <= 0 || cols <= 0 || steps < 1 || steps > kOrthoMaxSteps || ortho_is_thin(rows, cols)) return 0;
+    OrthoCoefficients co = {};
+    co.steps = steps;
+    const OrthoPlan p = ortho_plan(rows, cols, kOrthoF32, co, true, true);
+    // the whole batch at once, or nothing
+    if ((size_t)batch > kScratchBudget / (p.kept_matrix + p.per_matrix) || ortho_chunk(p, batch) < batch) return 0;
+    return (size_t)batch * p.kept_matrix + p.kept_fixed;
+}
+
+extern "C" size_t gsb_orthogonalize_scratch_bytes(long long batch, int rows, int cols, int dtype, int steps, int backward, int kept) {
     if (batch <= 0 || rows <= 0 || cols <= 0 || steps < 1 || steps > kOrthoMaxSteps || ortho_is_thin(rows, cols)) return 0;
     if (!backward && ortho_is_clustered(rows, cols)) return 0;
     OrthoCoefficients co = {};
     co.steps = steps;
-    return plan_bytes(ortho_plan(rows, cols, dtype, co, backward != 0), batch);
+    return plan_bytes(ortho_plan(rows, cols, dtype, co, backward != 0, kept != 0), batch);
 }
 
 static const char *at_matrix(const void *p, long long b, int rows, int cols, int dtype) {
@@ -741,17 +783,34 @@ static const char *at_matrix(const void *p, long long b, int rows, int cols, int
 }
 
 extern "C" int gsb_orthogonalize_fwd(long long batch, int rows, int cols, int dtype, const void *x, void *y, int steps,
-                                     const float *coefficients, float eps, void *scratch, size_t scratch_bytes,
-                                     cudaStream_t stream) {
+                                     const float *coefficients, float eps, void *kept, size_t kept_bytes, void *scratch,
+                                     size_t scratch_bytes, cudaStream_t stream) {
     OrthoCoefficients co = {};
     if (int e = check_common("orthogonalize", batch, rows, cols, dtype, steps, coefficients, eps, &co)) return e;
     if (batch == 0 || rows == 0 || cols == 0) return kOk;
+    if (kept && (kept_bytes == 0 || kept_bytes < gsb_orthogonalize_kept_bytes(batch, rows, cols, steps)))
+        return set_error(kErrInvalidArgument, "orthogonalize: the kept state needs %zu bytes", gsb_orthogonalize_kept_bytes(batch, rows, cols, steps));
     if (ortho_is_thin(rows, cols)) return ortho_thin_fwd(batch, rows, cols, dtype, x, y, co, eps, stream);
-    const OrthoPlan p = make_plan(rows, cols, dtype, co, false);
-    if (ortho_is_clustered(rows, cols))
-        return ortho_cluster_fwd(batch, rows, cols, dtype, x, y, co, (float)p.s.x, (float)p.s.a, (float)p.s.b, eps, stream);
+    const OrthoPlan p = make_plan(rows, cols, dtype, co, false, kept != nullptr);
+    Carver own{static_cast<char *>(kept)};
+    if (ortho_is_clustered(rows, cols)) {
+        if (!kept)
+            return ortho_cluster_fwd(batch, rows, cols, dtype, x, y, co, (float)p.s.x, (float)p.s.a, (float)p.s.b, eps, ClusterKept{}, stream);
+        const OrthoBuffers w(own, p, batch);
+        ClusterKept k = {};
+        k.x = w.x[0], k.a = w.a[0], k.b = w.b[0];
+        k.da = w.da[0], k.db = w.db[0], k.norms = w.norms;
+        k.step = steps > 1 ? w.x[1].hi - w.x[0].hi : 0;
+        return ortho_cluster_fwd(batch, rows, cols, dtype, x, y, co, (float)p.s.x, (float)p.s.a, (float)backward_scale(p), eps, k, stream);
+    }
     if (scratch == nullptr || scratch_bytes < plan_bytes(p, batch))
         return set_error(kErrInvalidArgument, "orthogonalize: %zu scratch bytes are needed", plan_bytes(p, batch));
+    if (kept) {
+        const OrthoBuffers w(own, p, batch);
+        Carver ws{static_cast<char *>(scratch)};
+        double *partial = ws.take<double>((size_t)batch * p.chunks);
+        return ortho_tiled_kept(p, co, batch, x, y, dtype, w, eps, partial, ws.take<int>(1), stream);
+    }
     const long long chunk = ortho_chunk(p, batch);
     const MuonTable none = {};
     for (long long b = 0; b < batch; b += chunk) {
@@ -764,20 +823,22 @@ extern "C" int gsb_orthogonalize_fwd(long long batch, int rows, int cols, int dt
 }
 
 extern "C" int gsb_orthogonalize_bwd(long long batch, int rows, int cols, int dtype, const void *x, const void *v_y,
-                                     void *v_x, int steps, const float *coefficients, float eps, void *scratch,
-                                     size_t scratch_bytes, cudaStream_t stream) {
+                                     void *v_x, int steps, const float *coefficients, float eps, void *kept, size_t kept_bytes,
+                                     void *scratch, size_t scratch_bytes, cudaStream_t stream) {
     OrthoCoefficients co = {};
     if (int e = check_common("orthogonalize", batch, rows, cols, dtype, steps, coefficients, eps, &co)) return e;
     if (batch == 0 || rows == 0 || cols == 0) return kOk;
+    if (kept && (kept_bytes == 0 || kept_bytes < gsb_orthogonalize_kept_bytes(batch, rows, cols, steps)))
+        return set_error(kErrInvalidArgument, "orthogonalize: the kept state needs %zu bytes", gsb_orthogonalize_kept_bytes(batch, rows, cols, steps));
     if (ortho_is_thin(rows, cols)) return ortho_thin_bwd(batch, rows, cols, dtype, x, v_y, v_x, co, eps, stream);
-    const OrthoPlan p = make_plan(rows, cols, dtype, co, true);
+    const OrthoPlan p = make_plan(rows, cols, dtype, co, true, kept != nullptr);
     if (scratch == nullptr || scratch_bytes < plan_bytes(p, batch))
         return set_error(kErrInvalidArgument, "orthogonalize: %zu scratch bytes are needed", plan_bytes(p, batch));
-    const long long chunk = ortho_chunk(p, batch);
+    const long long chunk = kept ? batch : ortho_chunk(p, batch);
     for (long long b = 0; b < batch; b += chunk) {
         if (int e = ortho_tiled_bwd(p, co, std::min(chunk, batch - b), at_matrix(x, b, rows, cols, dtype),
                                     at_matrix(v_y, b, rows, cols, dtype),
-                                    const_cast<char *>(at_matrix(v_x, b, rows, cols, dtype)), dtype, eps,
+                                    const_cast<char *>(at_matrix(v_x, b, rows, cols, dtype)), dtype, eps, kept,
                                     static_cast<char *>(scratch), stream))
             return e;
     }
@@ -826,7 +887,7 @@ extern "C" int gsb_muon(int n_tensors, const GsbMuonTensor *tensors, int rows, i
     const bool thin = ortho_is_thin(rows, cols), clustered = !thin && ortho_is_clustered(rows, cols);
     OrthoPlan p = {};
     if (!thin) {
-        p = make_plan(rows, cols, dtype, co, false);
+        p = make_plan(rows, cols, dtype, co, false, false);
         if (!clustered && (scratch == nullptr || scratch_bytes < plan_bytes(p, total)))
             return set_error(kErrInvalidArgument, "muon: %zu scratch bytes are needed", plan_bytes(p, total));
     }

@@ -141,12 +141,16 @@ def _ortho_coefficient_array(triples, steps: int):
 
 
 @functools.lru_cache(maxsize=256)
-def _ortho_scratch_bytes(batch: int, rows: int, cols: int, dtype: int, steps: int, backward: bool) -> int:
-    return lib().gsb_orthogonalize_scratch_bytes(batch, rows, cols, dtype, steps, int(backward))
+def _ortho_scratch_bytes(batch: int, rows: int, cols: int, dtype: int, steps: int, backward: int, kept: int) -> int:
+    return lib().gsb_orthogonalize_scratch_bytes(batch, rows, cols, dtype, steps, backward, kept)
 
 
-def _ortho_scratch(batch: int, rows: int, cols: int, dtype: int, steps: int, backward: bool, device) -> Optional[Tensor]:
-    size = _ortho_scratch_bytes(batch, rows, cols, dtype, steps, backward)
+@functools.lru_cache(maxsize=256)
+def _ortho_kept_bytes(batch: int, rows: int, cols: int, steps: int) -> int:
+    return lib().gsb_orthogonalize_kept_bytes(batch, rows, cols, steps)
+
+
+def _bytes(size: int, device) -> Optional[Tensor]:
     return torch.empty(size, dtype=torch.uint8, device=device) if size else None
 
 
@@ -162,7 +166,9 @@ def orthogonalize(
     every singular value s becomes p(...p(s)) with p(s) = a s + b s^3 + c s^5. The default
     coefficients bring all but the smallest near 1 in five steps; (1.5, -0.5, 0) converges to the orthogonal
     factor itself. ``coefficients`` may also be a list with a triple for each step. Matrices are multiplied
-    with 22 significand bits, bfloat16 ones with a side above 128 with 11; the result has x's shape and type. Differentiable (once); a matrix with a NaN or an infinity becomes NaN, others of the batch are not touched
+    with 22 significand bits, bfloat16 ones with a side above 128 with 11; the result has x's shape and type. Differentiable (once; the steps' state is kept for the backward
+    pass, about 4 steps (x.numel() + 2 B M M) bytes with M the shorter side, unless that is above 1 GiB: then it takes the
+    steps again). A matrix with a NaN or an infinity becomes NaN, others of the batch are not touched
     by it. Polynomials that take a singular value in [0, 1] above 16 are refused.
     """
     if x.dim() < 2:
@@ -177,30 +183,32 @@ def orthogonalize(
     return _orthogonalize_fwd(x, steps, coefficients, eps)
 
 
-def _orthogonalize_fwd(x: Tensor, steps: int, coefficients, eps: float) -> Tensor:
+def _orthogonalize_fwd(x: Tensor, steps: int, coefficients, eps: float, keep: bool = False):
     check_cuda("x", x)
     rows, cols = x.shape[-2:]
     batch = math.prod(x.shape[:-2])
     dtype = _ORTHO_DTYPES[x.dtype]
     y = torch.empty_like(x)
     with device_guard(x.device):
-        scratch = _ortho_scratch(batch, rows, cols, dtype, steps, False, x.device)
+        kept_bytes = _ortho_kept_bytes(batch, rows, cols, steps) if keep else 0
+        scratch_bytes = _ortho_scratch_bytes(batch, rows, cols, dtype, steps, 0, int(kept_bytes > 0))
+        kept, scratch = _bytes(kept_bytes, x.device), _bytes(scratch_bytes, x.device)
         call("gsb_orthogonalize_fwd", batch, rows, cols, dtype, ptr(x), ptr(y), steps, coefficients, eps,
-             ptr(scratch), 0 if scratch is None else scratch.numel(), stream_of(x))
-    return y
+             ptr(kept), kept_bytes, ptr(scratch), scratch_bytes, stream_of(x))
+    return (y, kept) if keep else y
 
 
 class _Orthogonalize(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x: Tensor, steps: int, coefficients, eps: float) -> Tensor:
-        y = _orthogonalize_fwd(x, steps, coefficients, eps)
-        ctx.save_for_backward(x)
+        y, kept = _orthogonalize_fwd(x, steps, coefficients, eps, keep=True)
+        ctx.save_for_backward(x, kept)
         ctx.steps, ctx.coefficients, ctx.eps = steps, coefficients, eps
         return y
 
     @staticmethod
     def backward(ctx, v_y: Tensor):
-        (x,) = ctx.saved_tensors
+        x, kept = ctx.saved_tensors
         v_y = v_y.contiguous()
         check_cuda("v_y", v_y)
         rows, cols = x.shape[-2:]
@@ -208,9 +216,11 @@ class _Orthogonalize(torch.autograd.Function):
         dtype = _ORTHO_DTYPES[x.dtype]
         v_x = torch.empty_like(x)
         with device_guard(x.device):
-            scratch = _ortho_scratch(batch, rows, cols, dtype, ctx.steps, True, x.device)
+            kept_bytes = 0 if kept is None else kept.numel()
+            scratch_bytes = _ortho_scratch_bytes(batch, rows, cols, dtype, ctx.steps, 1, int(kept_bytes > 0))
+            scratch = _bytes(scratch_bytes, x.device)
             call("gsb_orthogonalize_bwd", batch, rows, cols, dtype, ptr(x), ptr(v_y), ptr(v_x), ctx.steps,
-                 ctx.coefficients, ctx.eps, ptr(scratch), 0 if scratch is None else scratch.numel(), stream_of(x))
+                 ctx.coefficients, ctx.eps, ptr(kept), kept_bytes, ptr(scratch), scratch_bytes, stream_of(x))
         if torch.is_grad_enabled():  # create_graph=True
             v_x = _DifferentiableOnce.apply(v_x, x, v_y)
         return v_x, None, None, None
@@ -310,9 +320,10 @@ def muon(
         stream = stream_of(params[0])
         for (rows, cols, dtype, state_dtype), entries in groups.items():
             arr = (_B.GsbMuonTensor * len(entries))(*entries)
-            scratch = _ortho_scratch(sum(e[3] for e in entries), rows, cols, dtype, steps, False, device)
+            scratch_bytes = _ortho_scratch_bytes(sum(e[3] for e in entries), rows, cols, dtype, steps, 0, 0)
+            scratch = _bytes(scratch_bytes, device)
             call("gsb_muon", len(entries), arr, rows, cols, dtype, state_dtype, ptr(valid), momentum, int(nesterov),
-                 steps, coefficients, eps, ptr(scratch), 0 if scratch is None else scratch.numel(), stream)
+                 steps, coefficients, eps, ptr(scratch), scratch_bytes, stream)
     torch.autograd.graph.increment_version(params + momentum_buffers)
 
 

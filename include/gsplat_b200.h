@@ -466,7 +466,10 @@ GSB_API int gsb_adam_multi(int n_groups, const GsbAdamGroup *groups, const bool 
  * (X transposed where rows > cols). Coefficients whose polynomials a s + b s^3 + c s^5 take
  * a singular value in [0, 1] above 16 are refused. Matrices are multiplied with
  * 22 significand bits; bfloat16 ones with a side above 128 with 11.
- * gsb_orthogonalize_bwd: v_x = the gradient of x for the gradient v_y of y.
+ * gsb_orthogonalize_bwd: v_x = the gradient of x for the gradient v_y of y. With a
+ * `kept` state of gsb_orthogonalize_kept_bytes (0: there is none for this shape, or it would be
+ * above 1 GiB with the scratch) that the forward call wrote, the backward call, of the
+ * same arguments, need not take the steps again; both may have NULL instead.
  * gsb_muon: for the listed tensors, each a batch of matrices of one shape (or its
  * transpose) and type: m <- m + (1 - momentum)(grad - m); u = grad + momentum (m - grad) (nesterov)
  * or m; param <- decay * param - lr * orthogonalized(u). momentum_buffer has
@@ -474,15 +477,19 @@ GSB_API int gsb_adam_multi(int n_groups, const GsbAdamGroup *groups, const bool 
  * dimension (`inner` matrices) whose entry is false is neither read nor
  * written. Tensors must not overlap.
  * Scratch: gsb_orthogonalize_scratch_bytes of the whole batch (gsb_muon: the sum
- * of the tensors' batches, backward = 0); 0 where none is needed. Calls that may run at the same time need scratch of their own. */
+ * of the tensors' batches, backward = kept = 0; kept = 1: for a call with a kept state);
+ * 0 where none is needed. Calls that may run at the same time need scratch of their own. */
+GSB_API size_t gsb_orthogonalize_kept_bytes(long long batch, int rows, int cols, int steps);
 GSB_API size_t gsb_orthogonalize_scratch_bytes(long long batch, int rows, int cols, int dtype,
-                                       int steps, int backward);
+                                       int steps, int backward, int kept);
 GSB_API int gsb_orthogonalize_fwd(long long batch, int rows, int cols, int dtype, const void *x,
-                          void *y, int steps, const float *coefficients, float eps, void *scratch,
-                          size_t scratch_bytes, cudaStream_t stream);
+                          void *y, int steps, const float *coefficients, float eps, void *kept,
+                          size_t kept_bytes, void *scratch, size_t scratch_bytes,
+                          cudaStream_t stream);
 GSB_API int gsb_orthogonalize_bwd(long long batch, int rows, int cols, int dtype, const void *x,
                           const void *v_y, void *v_x, int steps, const float *coefficients,
-                          float eps, void *scratch, size_t scratch_bytes, cudaStream_t stream);
+                          float eps, void *kept, size_t kept_bytes, void *scratch,
+                          size_t scratch_bytes, cudaStream_t stream);
 typedef struct GsbMuonTensor {
     void *param;
     const void *grad;

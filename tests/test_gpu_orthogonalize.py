@@ -122,6 +122,29 @@ def test_gradient_steps(shape, steps, coefficients):
     assert off <= N.gradient_tolerance(x, v, steps, coefficients) * exact.norm() + N.projected_away(x, v, steps, coefficients)
 
 
+@pytest.mark.parametrize("shape", [(3, 20, 40), (2, 70, 500), (2, 150, 140)])
+def test_gradient_without_kept_state(shape, monkeypatch):
+    """Where the steps' state would be too large, the backward pass takes the steps again."""
+    from gsplat_b200.cuda import _wrapper
+
+    x, v = data(shape, torch.float32, 18), data(shape, torch.float32, 19, 1.0)
+    xg = x.cuda().requires_grad_(True)
+    monkeypatch.setattr(_wrapper, "_ortho_kept_bytes", lambda *a: 0)
+    (got,) = torch.autograd.grad(gs().orthogonalize(xg), xg, v.cuda())
+    exact = N.gradient(x, v, 5, N.QUINTIC)
+    off = (got.cpu().double() - exact).norm()
+    assert off <= N.gradient_tolerance(x, v, 5, N.QUINTIC) * exact.norm() + N.projected_away(x, v, 5, N.QUINTIC)
+
+
+def test_gradient_twice_from_one_forward():
+    """A retained graph: the kept state serves both passes."""
+    for shape in ((5, 24, 40), (1, 300, 200)):
+        x, v = data(shape, torch.float32, 90).cuda().requires_grad_(True), data(shape, torch.float32, 91, 1.0).cuda()
+        y = gs().orthogonalize(x)
+        first = torch.autograd.grad(y, x, v, retain_graph=True)[0]
+        assert torch.equal(torch.autograd.grad(y, x, v)[0], first)
+
+
 def test_gradient_against_differences():
     """A central difference of the kernel's own values along one direction: its error is the third derivative's h^2
     and the rounding 2^-22 / h of a sum of values of order 1."""

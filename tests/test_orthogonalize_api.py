@@ -66,8 +66,8 @@ def triples(*c):
 def test_c_entry_points_refuse_before_any_launch():
     L, c = lib(), triples(*[N.QUINTIC] * 5)
 
-    def fwd(batch=1, rows=8, cols=8, dtype=0, steps=5, co=c, eps=1e-7, scratch=None, size=0):
-        return L.gsb_orthogonalize_fwd(batch, rows, cols, dtype, None, None, steps, co, eps, scratch, size, None)
+    def fwd(batch=1, rows=8, cols=8, dtype=0, steps=5, co=c, eps=1e-7, kept=None, kept_size=0, scratch=None, size=0):
+        return L.gsb_orthogonalize_fwd(batch, rows, cols, dtype, None, None, steps, co, eps, kept, kept_size, scratch, size, None)
 
     assert fwd(batch=-1) == -1 and b"negative" in L.gsb_last_error()
     assert fwd(dtype=3) == -2 and b"dtype" in L.gsb_last_error()
@@ -80,8 +80,9 @@ def test_c_entry_points_refuse_before_any_launch():
     # the peak lies inside: 12 s - 12 s^3 is 0 at 1 and 4.6 at 0.58, and grows from there
     assert fwd(co=triples(*[(12.0, -12.0, 0.0)] * 5)) == -1
     assert fwd(rows=200, cols=200) == -1 and b"scratch" in L.gsb_last_error()
+    assert fwd(rows=200, cols=200, kept=4096, kept_size=100) == -1 and b"kept" in L.gsb_last_error()
     assert fwd(batch=0) == 0 and fwd(rows=0) == 0 and fwd(cols=0) == 0
-    rc = L.gsb_orthogonalize_bwd(1, 200, 200, 0, None, None, None, 5, c, 1e-7, None, 0, None)
+    rc = L.gsb_orthogonalize_bwd(1, 200, 200, 0, None, None, None, 5, c, 1e-7, None, 0, None, 0, None)
     assert rc == -1 and b"scratch" in L.gsb_last_error()
     assert L.gsb_muon(1, None, 8, 8, 0, 0, None, 0.9, 1, 5, c, 1e-7, None, 0, None) == -1
     assert b"no tensor list" in L.gsb_last_error()
@@ -92,14 +93,18 @@ def test_c_entry_points_refuse_before_any_launch():
 
 def test_scratch_sizes():
     L = lib()
-    size = L.gsb_orthogonalize_scratch_bytes
+    def size(batch, rows, cols, dtype, steps, backward, kept=0):
+        return L.gsb_orthogonalize_scratch_bytes(batch, rows, cols, dtype, steps, backward, kept)
+
+    kept = L.gsb_orthogonalize_kept_bytes
     assert size(1000000, 15, 3, 0, 5, 0) == 0 and size(10, 3, 128, 1, 5, 1) == 0  # thin
     assert size(10, 64, 64, 0, 5, 0) == 0 and size(10, 64, 64, 0, 5, 1) > 0  # on chip, forward
     assert size(10, 129, 129, 0, 5, 0) > 0 and size(0, 200, 200, 0, 5, 0) == 0
     assert size(1, 512, 256, 0, 5, 0) == size(1, 256, 512, 0, 5, 0)
-    assert size(1, 256, 256, 0, 5, 1) > size(1, 256, 256, 0, 5, 0)
-    # a large batch is taken in pieces: the scratch stays near 1 GiB
-    assert size(100000, 512, 512, 0, 5, 0) < 1.1 * 2**30
+    assert size(1, 256, 256, 0, 5, 1) > size(1, 256, 256, 0, 5, 1, 1)
+    assert kept(10, 3, 15, 5) == 0 and kept(1, 256, 256, 5) > 0 and kept(1, 64, 64, 5) > 0
+    # a large batch is taken in pieces: the scratch stays near 1 GiB, and nothing is kept
+    assert size(100000, 512, 512, 0, 5, 0) < 1.1 * 2**30 and kept(100000, 512, 512, 5) == 0
 
 
 def test_model_of_roundings_is_small_and_grows_with_them():

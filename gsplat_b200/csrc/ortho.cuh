@@ -118,23 +118,31 @@ __device__ __forceinline__ bool muon_visible(const MuonTable &t, int i, long lon
 }
 
 // A launch whose blocks may set up while the launch before it in the stream ends; the kernel
-// waits for that one (griddepcontrol.wait) before it touches memory.
+// waits for that one (griddepcontrol.wait) before it touches memory. `cluster` blocks form a cluster.
 template <typename... P, typename... A>
-inline int launch_after(void (*kernel)(P...), unsigned blocks, int threads, size_t smem, cudaStream_t stream, const char *what,
-                        const A &...args) {
+inline int launch_clusters_after(void (*kernel)(P...), int cluster, unsigned blocks, int threads, size_t smem, cudaStream_t stream,
+                                 const char *what, const A &...args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(blocks);
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 0 ? 2 : 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
     if (e != cudaSuccess) return set_error(kErrLaunch, "%s: %s", what, cudaGetErrorString(e));
     return check_launch(what);
+}
+template <typename... P, typename... A>
+inline int launch_after(void (*kernel)(P...), unsigned blocks, int threads, size_t smem, cudaStream_t stream, const char *what,
+                        const A &...args) {
+    return launch_clusters_after(kernel, 0, blocks, threads, smem, stream, what, args...);
 }
 
 // --- thin matrices (ortho_thin.cu) -----------------------------------------

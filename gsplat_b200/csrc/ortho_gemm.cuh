@@ -11,6 +11,7 @@
 // A launch follows the one before it without a gap: its blocks set up while that one ends (griddepcontrol).
 #pragma once
 
+#include <algorithm>
 #include <cuda.h>
 
 #include "ortho.cuh"
@@ -267,7 +268,34 @@ template <bool SPLIT, int EPI> __device__ __forceinline__ void stage32(float *st
     __syncwarp();
 }
 
-template <bool SPLIT, int BN, int EPI>
+__device__ __forceinline__ uint32_t block_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
+}
+// The leader's (rank 0's) copy of an address of this block's shared memory, and a store to it.
+__device__ __forceinline__ uint32_t at_leader(uint32_t addr) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+    return r;
+}
+__device__ __forceinline__ void store_at(uint32_t addr, float4 v) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+
+// DEEP: the blocks of a cluster share a tile, each with a part of the depth. All but the leader leave their
+// sums in its shared memory (where its stages were), and it adds them in the order of the blocks and finishes
+// the tile; a launch then has one tile a cluster. For long contractions with few tiles (A of a
+// short matrix), whose blocks would otherwise work through the depth alone.
+template <bool SPLIT, int BN, int EPI, bool DEEP>
 __global__ void __launch_bounds__(kGemmThreads, 1)
     ortho_gemm_kernel(const __grid_constant__ OrthoGemm g, const __grid_constant__ GemmMaps maps,
                       const __grid_constant__ MuonTable tab, int per, int tiles_n, long long tiles) {
@@ -312,8 +340,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     asm volatile("griddepcontrol.wait;" ::: "memory"); // for what the launches before this one wrote
 
     const int kblocks = (g.K + kBK - 1) / kBK;
-    const int total = kblocks * g.pairs;      // stages of a tile
-    const int chunk = SPLIT ? kChunk : total; // stages of an accumulation
+    const int ranks = DEEP ? (int)cluster_size() : 1, rank = DEEP ? (int)block_rank() : 0;
+    const int all = kblocks * g.pairs;                                              // stages of a tile
+    const int begin = DEEP ? all * rank / ranks : 0, end = DEEP ? all * (rank + 1) / ranks : all; // this block's
+    const int chunk = SPLIT ? kChunk : end - begin;                                 // stages of an accumulation
+    const long long first = DEEP ? blockIdx.x / ranks : blockIdx.x, stride = DEEP ? gridDim.x / ranks : gridDim.x;
+    // whether the cluster's one tile is worked on, by all of its blocks' warps
+    const bool shared_tile = DEEP && !(tab.n > 0 && !muon_visible(tab, muon_tensor_of(tab, first / per), first / per));
     if (warp == kEpilogueWarps) {
         // the copies
         if (lane == 0) {
@@ -321,11 +354,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             uint32_t phase = 0;
             long long loads = 0;
             bool ok = true;
-            for (long long t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+            for (long long t = first; ok && t < tiles; t += stride) {
                 const TileAt at = tile_at<BN>(t, per, tiles_n, kSymmetric);
                 if (tab.n > 0 && !muon_visible(tab, muon_tensor_of(tab, at.b), at.b)) continue;
                 const int b = (int)at.b, i0 = at.i * kBM, j0 = at.j * BN;
-                for (int s = 0; s < total; ++s) {
+                for (int s = begin; s < end; ++s) {
                     const int pair = s >= kblocks, k0 = (s - pair * kblocks) * kBK;
                     ok = mbar_wait(&sh.empty[stage], phase ^ 1u, abort);
                     if (!ok) break;
@@ -358,6 +391,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                     for (unsigned i = 0; i < kWaitLimit && !mbar_try(&sh.full[l % kStages], (uint32_t)(l / kStages) & 1u); ++i) {}
             }
         }
+        if (DEEP && shared_tile) {
+            __syncwarp();
+            cluster_barrier();
+            cluster_barrier();
+        }
     } else if (warp == kEpilogueWarps + 1) {
         // the products
         const uint32_t leader = elect_leader();
@@ -366,15 +404,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         int stage = 0, acc = 0;
         uint32_t phase = 0, acc_phase = 0;
         bool ok = true;
-        for (long long t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+        for (long long t = first; ok && t < tiles; t += stride) {
             const TileAt at = tile_at<BN>(t, per, tiles_n, kSymmetric);
             if (tab.n > 0 && !muon_visible(tab, muon_tensor_of(tab, at.b), at.b)) continue;
-            for (int s0 = 0; ok && s0 < total; s0 += chunk) {
+            for (int s0 = begin; ok && s0 < end; s0 += chunk) {
                 ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_empty[acc], acc_phase ^ 1u, abort));
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t d = tmem + acc * BN;
-                const int s1 = min(total, s0 + chunk);
+                const int s1 = min(end, s0 + chunk);
                 for (int s = s0; s < s1; ++s) {
                     ok = __all_sync(0xffffffffu, mbar_wait(&sh.full[stage], phase, abort));
                     if (!ok) break;
@@ -402,6 +440,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                 if (acc == 0) acc_phase ^= 1u;
             }
         }
+        if (DEEP && shared_tile) {
+            __syncwarp();
+            cluster_barrier();
+            cluster_barrier();
+        }
     } else {
         // the epilogue: warp w has rows 32 (w % 4) .., columns W (w / 4) ..
         const int row = 32 * (warp % 4) + lane, half = warp / 4;
@@ -410,7 +453,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         int acc = 0;
         uint32_t acc_phase = 0;
         bool ok = true;
-        for (long long t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+        for (long long t = first; ok && t < tiles; t += stride) {
             const TileAt at = tile_at<BN>(t, per, tiles_n, kSymmetric);
             const int tensor = tab.n > 0 ? muon_tensor_of(tab, at.b) : 0;
             if (tab.n > 0 && !muon_visible(tab, tensor, at.b)) continue;
@@ -425,7 +468,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             }
             fetch32<SPLIT, EPI>(g, at.b, i - lane, j, lane, e);
             float v[W];
-            for (int s0 = 0; s0 < total; s0 += chunk) {
+            for (int s0 = begin; s0 < end; s0 += chunk) {
                 ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[acc], acc_phase, abort));
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -435,13 +478,37 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                     float u[32];
                     tmem_load32(src + c, u);
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) v[c + k] = s0 == 0 ? u[k] : v[c + k] + u[k];
+                    for (int k = 0; k < 32; ++k) v[c + k] = s0 == begin ? u[k] : v[c + k] + u[k];
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.acc_empty[acc]);
                 acc ^= 1;
                 if (acc == 0) acc_phase ^= 1u;
+            }
+            if (DEEP) { // rank r's sums at r - 1 of [ranks - 1][warp][W / 4][lane], four columns each
+                const uint32_t sums = stage0 + (uint32_t)(warp * (W / 4) * 32 + lane) * 16;
+                constexpr uint32_t block = kEpilogueWarps * (W / 4) * 32 * 16;
+                __syncwarp();
+                cluster_barrier(); // the leader's stages are done with
+                if (rank > 0) {
+                    const uint32_t to = at_leader(sums) + (rank - 1) * block;
+#pragma unroll
+                    for (int c = 0; c < W; c += 4) store_at(to + c / 4 * 512, make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]));
+                }
+                cluster_barrier();
+                if (rank > 0) break;
+                for (int r = 1; r < ranks; ++r) {
+#pragma unroll
+                    for (int c = 0; c < W; c += 4) {
+                        float4 f;
+                        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                     : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w)
+                                     : "r"(sums + (r - 1) * block + c / 4 * 512)
+                                     : "memory");
+                        v[c] += f.x, v[c + 1] += f.y, v[c + 2] += f.z, v[c + 3] += f.w;
+                    }
+                }
             }
             if (!ok) break;
             const bool mirror = (at.j * BN) / kBM != at.i; // off the diagonal block
@@ -467,8 +534,25 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 template <bool SPLIT, int BN, int EPI>
 static int launch_one(const OrthoGemm &g, const GemmMaps &maps, const MuonTable &tab, int per, int tn, long long tiles,
                       int sms, cudaStream_t stream) {
-    auto *kernel = ortho_gemm_kernel<SPLIT, BN, EPI>;
     constexpr int smem = Stages<SPLIT, BN>::smem;
+    // Blocks that share a tile's depth: as many as there are SMs for, as fit their sums beside each other in the
+    // leader's stages, and as have 2 us of products each (4 or 12 stages), which is what meeting costs. With
+    // more tiles than the GPU has clusters of SMs (8), a power of two: other sizes leave SMs of each without work.
+    constexpr int most = Stages<SPLIT, BN>::n * Stages<SPLIT, BN>::bytes / (kBM * BN * 4) + 1;
+    const int stages = (g.K + kBK - 1) / kBK * g.pairs;
+    int ranks = (int)std::min<long long>({sms / tiles, stages / (SPLIT ? 4 : 12), most, 8});
+    if (tiles > 8 && ranks > 1) ranks = ranks >= 4 ? 4 : 2;
+    constexpr bool kDeep = BN == 64 && (EPI == kEpiGram || EPI == kEpiSym);
+    if constexpr (kDeep) {
+        if (ranks > 1) {
+            auto *kernel = ortho_gemm_kernel<SPLIT, BN, EPI, true>;
+            if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+                return check_launch("ortho_gemm_kernel attributes");
+            return launch_clusters_after(kernel, ranks, (unsigned)(tiles * ranks), kGemmThreads, smem, stream, "ortho_gemm_kernel", g, maps,
+                                         tab, per, tn, tiles);
+        }
+    }
+    auto *kernel = ortho_gemm_kernel<SPLIT, BN, EPI, false>;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
         return check_launch("ortho_gemm_kernel attributes");
     return launch_after(kernel, (unsigned)(tiles < sms ? tiles : sms), kGemmThreads, smem, stream, "ortho_gemm_kernel", g, maps, tab,

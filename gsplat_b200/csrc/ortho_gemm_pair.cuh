@@ -22,20 +22,6 @@ template <bool SPLIT> struct PairStages {
     static constexpr int smem = n * bytes + kOutStage + 1024;
 };
 
-__device__ __forceinline__ uint32_t pair_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void pair_sync() {
-    asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
-}
-// The leader's copy of one of this block's shared variables.
-__device__ __forceinline__ uint32_t at_leader(const void *p) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
-    return r;
-}
 __device__ __forceinline__ void arrive_at(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -72,7 +58,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     __shared__ GemmShared sh;
     const uint32_t stage0 = (smem_u32(raw) + 1023u) & ~1023u;
     const int warp = uniform_warp(), lane = threadIdx.x % 32;
-    const uint32_t rank = pair_rank();
+    const uint32_t rank = block_rank();
     const long long first = blockIdx.x / 2, pairs = gridDim.x / 2;
     volatile int *abort = &sh.abort;
 
@@ -99,7 +85,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     }
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    pair_sync();
+    cluster_barrier();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -124,7 +110,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                     ok = mbar_wait(&sh.empty[stage], phase ^ 1u, abort);
                     if (!ok) break;
                     uint32_t dst = stage0 + stage * Stage::bytes;
-                    const uint32_t bar = at_leader(&sh.full[stage]);
+                    const uint32_t bar = at_leader(smem_u32(&sh.full[stage]));
                     if (rank == 0) mbar_expect(&sh.full[stage], 2 * Stage::bytes);
                     tma_load_pair(dst, &maps.p_hi[pair], k0, i0, b, bar);
                     if (SPLIT) tma_load_pair(dst + Stage::plane, &maps.p_lo[pair], k0, i0, b, bar);
@@ -201,7 +187,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         const int row = 32 * (warp % 4) + lane, half = warp / 4;
         float *out_stage = reinterpret_cast<float *>(raw + (stage0 - smem_u32(raw)) + kStages * Stage::bytes) + warp * 32 * kStagePitch;
         const bool poisoned = !E::to_planes && *(volatile const int *)g.error != 0;
-        const uint32_t acc_empty[2] = {at_leader(&sh.acc_empty[0]), at_leader(&sh.acc_empty[1])};
+        const uint32_t acc_empty[2] = {at_leader(smem_u32(&sh.acc_empty[0])), at_leader(smem_u32(&sh.acc_empty[1]))};
         int acc = 0;
         uint32_t acc_phase = 0;
         bool ok = true;
@@ -267,7 +253,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     if (threadIdx.x == 0 && sh.abort) atomicExch(g.error, 1);
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    pair_sync(); // neither block leaves while the other may reach its shared memory
+    cluster_barrier(); // neither block leaves while the other may reach its shared memory
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (warp == kEpilogueWarps + 1)
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * kPair) : "memory");

@@ -103,7 +103,7 @@ struct MuonTable {
     void *momentum[kOrthoMaxTensors];
     float lr[kOrthoMaxTensors], decay[kOrthoMaxTensors]; // decay = 1 - lr * weight_decay
     int inner[kOrthoMaxTensors];         // matrices per leading row
-    bool transposed[kOrthoMaxTensors];   // the tensor's matrices are [long, short] (tiled path)
+    bool transposed[kOrthoMaxTensors];   // the tensor's matrices are [long, short]
     long long skipped[kOrthoMaxTensors]; // the tensor's matrices before its first one here
     long long first[kOrthoMaxTensors + 1];
 };
@@ -167,7 +167,7 @@ struct OrthoPlanes {
 
 // --- short side <= 128 and not too long (ortho_cluster.cu): one launch, the matrix in the
 // shared memory of a cluster. The scales are those of X, A and B as OrthoPlanes have them.
-bool ortho_is_clustered(int rows, int cols);
+int ortho_is_clustered(int rows, int cols); // the blocks of a matrix's cluster, or 0
 // Where the first step's X, A and B go for a backward pass (x.hi = NULL: nowhere), each further step's
 // `step` halves (2 bytes) behind.
 struct ClusterKept {
@@ -177,8 +177,9 @@ struct ClusterKept {
 };
 int ortho_cluster_fwd(long long batch, int rows, int cols, int dtype, const void *x, void *y, const OrthoCoefficients &co,
                       float x_scale, float a_scale, float b_scale, float eps, const ClusterKept &kept, cudaStream_t stream);
-int ortho_cluster_muon(const MuonTable &table, int rows, int cols, const OrthoCoefficients &co, float x_scale,
-                       float a_scale, float b_scale, float eps, cudaStream_t stream);
+// The table's tensors, of sizes[t] = {rows, columns} each, all with the same clusters.
+int ortho_cluster_muon(const MuonTable &table, const int sizes[][2], const OrthoCoefficients &co, float x_scale, float a_scale,
+                       float b_scale, float eps, cudaStream_t stream);
 
 enum OrthoEpilogue : int {
     kEpiGram,   // A: off-diagonal part and its diagonal

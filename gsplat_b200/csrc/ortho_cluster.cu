@@ -112,26 +112,40 @@ __device__ __forceinline__ void planes_put16(char *hi, char *lo, int rows, int r
     }
 }
 
-// One warp: D[128, n] = P Q over `depth`, hi and lo planes of both; P and Q depth-major from their
-// first row (X X^T, A A), or Q column-major (B X). `rows`: of the planes.
-__device__ __forceinline__ void multiply(uint32_t d, uint32_t p, uint32_t p_lo, uint32_t q, uint32_t q_lo, int rows_p,
-                                         int rows_q, bool q_k_major, int n, int depth, uint32_t leader) {
-    const uint32_t idesc = mma_desc(n, q_k_major);
-    const uint32_t chunk_p = rows_p * 128, chunk_q = rows_q * 128;
-    const uint64_t ph = operand_desc(p, true, 0), pl = operand_desc(p_lo, true, 0);
-    const uint64_t qh = operand_desc(q, q_k_major, chunk_q), ql = operand_desc(q_lo, q_k_major, chunk_q);
-    for (int k = 0; k < depth; k += 16) { // 16 bytes a unit of the descriptors' addresses
-        const uint32_t po = ((k >> 6) * chunk_p + ((k >> 4) & 3) * 32) >> 4;
-        const uint32_t qo = (q_k_major ? (k >> 6) * chunk_q + ((k >> 4) & 3) * 32 : k * 128) >> 4;
-        mma_f16(d, ph + po, qh + qo, idesc, k > 0, leader);
-        mma_f16(d, ph + po, ql + qo, idesc, true, leader);
-        mma_f16(d, pl + po, qh + qo, idesc, true, leader);
+// The descriptors of a product of planes and what a step of 64 of its depth adds to them, in 16-byte units: P
+// depth-major; Q depth-major from its first row (X X^T, A A), or column-major (B X). `rows`: of the planes.
+struct Operands {
+    uint64_t p, p_lo, q, q_lo;
+    uint32_t p_block, q_block, q_step; // of 64 deep, and of 16 within
+};
+__device__ __forceinline__ Operands operands(uint32_t p, uint32_t p_lo, uint32_t q, uint32_t q_lo, int rows, bool q_k_major) {
+    const uint32_t chunk = rows * 128;
+    return {operand_desc(p, true, 0), operand_desc(p_lo, true, 0), operand_desc(q, q_k_major, chunk), operand_desc(q_lo, q_k_major, chunk),
+            chunk / 16, q_k_major ? chunk / 16 : 64 * 128 / 16, q_k_major ? 2u : 128u};
+}
+// One warp: D[128, n] = P Q over `depth` (a multiple of 16).
+__device__ __forceinline__ void multiply(uint32_t d, Operands o, uint32_t idesc, int depth, uint32_t leader) {
+    for (int k = 0; k < depth; k += 64) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (k + 16 * i >= depth) break;
+            mma_f16(d, o.p + 2 * i, o.q + i * o.q_step, idesc, k > 0 || i > 0, leader);
+            mma_f16(d, o.p + 2 * i, o.q_lo + i * o.q_step, idesc, true, leader);
+            mma_f16(d, o.p_lo + 2 * i, o.q + i * o.q_step, idesc, true, leader);
+        }
+        o.p += o.p_block, o.p_lo += o.p_block;
+        o.q += o.q_block, o.q_lo += o.q_block;
     }
 }
 
+// The shapes of a launch's tensors; all have the same number of blocks a cluster.
+template <bool MUON> struct ClusterShapes {
+    ClusterShape of[MUON ? kOrthoMaxTensors : 1];
+};
+
 template <typename T, typename M, bool MUON>
 __global__ void __launch_bounds__(kClusterThreads, 1)
-    ortho_cluster_kernel(const __grid_constant__ ClusterShape sh, const T *x_in, T *y, const __grid_constant__ MuonTable tab,
+    ortho_cluster_kernel(const __grid_constant__ ClusterShapes<MUON> shapes, const T *x_in, T *y, const __grid_constant__ MuonTable tab,
                          const __grid_constant__ ClusterSteps co, float eps, const __grid_constant__ ClusterKept kept) {
     extern __shared__ char raw[];
     __shared__ alignas(16) float diag_a[kClusterMaxShort];
@@ -141,9 +155,11 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
     __shared__ uint32_t tmem_at;
     __shared__ int abort_flag;
     const int tid = threadIdx.x, warp = uniform_warp(), lane = tid % 32;
-    const uint32_t rank = sh.blocks > 1 ? cluster_rank() : 0;
-    const long long b = blockIdx.x / sh.blocks;
+    const int blocks = shapes.of[0].blocks;
+    const uint32_t rank = blocks > 1 ? cluster_rank() : 0;
+    const long long b = blockIdx.x / blocks;
     const int tensor = MUON ? muon_tensor_of(tab, b) : 0;
+    const ClusterShape &sh = shapes.of[tensor];
     if (MUON && !muon_visible(tab, tensor, b)) return; // the whole cluster alike
 
     char *base = reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
@@ -228,6 +244,7 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
         reinterpret_cast<uint4 *>(base)[i] = make_uint4(0, 0, 0, 0);
     // the norm: sums in 64 bits, in a fixed order
     double s = 0.0;
+    float4 g0[U], m0[U]; // the first turn's values stay for the second pass, which is all of a small slab
     for (int e0 = tid; e0 < moves; e0 += U * kClusterThreads) {
         float4 g[U], m[U];
 #pragma unroll
@@ -236,6 +253,7 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
             int i, j;
             g[u] = m[u] = make_float4(0, 0, 0, 0);
             if (e < moves) g[u] = fetch(place(e, i, j), e < fours, m[u]);
+            if (e0 == tid) g0[u] = g[u], m0[u] = m[u];
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -277,7 +295,8 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
             const int e = e0 + u * kClusterThreads;
             if (e < moves) {
                 at[u] = place(e, i[u], j[u]);
-                g[u] = fetch(at[u], e < fours, m[u]);
+                if (e0 == tid) g[u] = g0[u], m[u] = m0[u];
+                else g[u] = fetch(at[u], e < fours, m[u]);
             }
         }
 #pragma unroll
@@ -324,6 +343,9 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
     const uint32_t xh = smem_u32(x_hi), xl = smem_u32(x_lo), ah = smem_u32(a_hi), al = smem_u32(a_lo);
     const int ns16 = (sh.ns + 15) / 16 * 16;
     const uint32_t leader = elect_leader();
+    const Operands gram = operands(xh, xl, xh, xl, sh.m16, true), square = operands(ah, al, ah, al, sh.m16, true),
+                   apply = operands(ah, al, xh, xl, sh.m16, false);
+    const uint32_t idesc_a = mma_desc(sh.m16, true);
     uint32_t phase = 0;
     // what was written to shared memory is multiplied, and every thread waits for the product
     auto begin = [&] {
@@ -343,7 +365,7 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
         // A
         begin();
         if (warp == 0) {
-            multiply(tmem, xh, xl, xh, xl, sh.m16, sh.m16, true, sh.m16, ns16, leader);
+            multiply(tmem, gram, idesc_a, ns16, leader);
             mma_commit(&done, leader);
         }
         if (keep) dump(x_hi, x_lo, kept.x, step, 0, sh.m, cols, j0);
@@ -406,7 +428,7 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
         // B
         begin();
         if (warp == 0) {
-            multiply(tmem, ah, al, ah, al, sh.m16, sh.m16, true, sh.m16, sh.m16, leader);
+            multiply(tmem, square, idesc_a, sh.m16, leader);
             mma_commit(&done, leader);
         }
         if (keep) {
@@ -449,9 +471,11 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
         // X
         begin();
         if (warp == 0) {
-            for (int c = 0; c < ns16; c += 256)
-                multiply(tmem + c, ah, al, xh + (c >> 6) * sh.m16 * 128, xl + (c >> 6) * sh.m16 * 128, sh.m16, sh.m16, false,
-                         min(256, ns16 - c), sh.m16, leader);
+            Operands part = apply;
+            for (int c = 0; c < ns16; c += 256) {
+                multiply(tmem + c, part, mma_desc(min(256, ns16 - c), false), sh.m16, leader);
+                part.q += 4 * part.p_block, part.q_lo += 4 * part.p_block; // four blocks of 64 columns on
+            }
             mma_commit(&done, leader);
         }
         if (keep) {
@@ -574,73 +598,100 @@ static int cluster_blocks(int rows, int cols) {
     return 0;
 }
 
-bool ortho_is_clustered(int rows, int cols) { return cluster_blocks(rows, cols) > 0; }
+int ortho_is_clustered(int rows, int cols) { return cluster_blocks(rows, cols); }
 
 template <typename T, typename M, bool MUON>
-static int cluster_launch(long long batch, const ClusterShape &sh, const void *x, void *y, const MuonTable &tab,
+static int cluster_launch(long long batch, const ClusterShapes<MUON> &shapes, size_t smem, const void *x, void *y, const MuonTable &tab,
                           const ClusterSteps &steps, float eps, const ClusterKept &kept, cudaStream_t stream) {
     auto *kernel = ortho_cluster_kernel<T, M, MUON>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sh.smem) != cudaSuccess)
+    const int blocks = shapes.of[0].blocks;
+    if (batch * blocks > 0x7fffffffll) return set_error(kErrInvalidArgument, "orthogonalize: too many matrices");
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         return check_launch("ortho_cluster_kernel attributes");
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(batch * sh.blocks));
+    cfg.gridDim = dim3((unsigned)(batch * blocks));
     cfg.blockDim = dim3(kClusterThreads);
-    cfg.dynamicSmemBytes = sh.smem;
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = sh.blocks;
+    attr[0].val.clusterDim.x = blocks;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, sh, static_cast<const T *>(x), static_cast<T *>(y), tab, steps, eps, kept);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, shapes, static_cast<const T *>(x), static_cast<T *>(y), tab, steps, eps, kept);
     if (e != cudaSuccess) return set_error(kErrLaunch, "ortho_cluster_kernel: %s", cudaGetErrorString(e));
     return check_launch("ortho_cluster_kernel");
 }
 
-static int cluster_plan(const char *what, long long batch, int rows, int cols, const OrthoCoefficients &co, float x_scale,
-                        float a_scale, float b_scale, ClusterShape *sh, ClusterSteps *steps) {
-    *sh = cluster_shape(rows, cols, cluster_blocks(rows, cols));
-    sh->x_scale = x_scale;
-    sh->to_a = a_scale / (x_scale * x_scale);
-    sh->to_d = 1.f / (x_scale * x_scale);
-    sh->unscale_b = 1.f / b_scale;
-    sh->unscale_x = 1.f / x_scale;
-    steps->n = co.steps;
+// More blocks a cluster than a matrix needs, where there are SMs for them and a block's slab stays at least 128
+// columns: below that the exchange of A costs more than the shorter slab saves ([128, 128] 54 us in one
+// block, 72 in two; [64, 512] 77 us in one, 56 in four).
+static int cluster_widen(const int sizes[][2], int n, long long batch) {
+    int blocks = cluster_blocks(sizes[0][0], sizes[0][1]), sms = 148, dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    auto wide = [&] {
+        for (int i = 0; i < n; ++i)
+            if (cluster_shape(sizes[i][0], sizes[i][1], blocks).ns < 256) return false;
+        return true;
+    };
+    while (2 * blocks <= kClusterMax && batch * 2 * blocks <= sms && wide()) blocks *= 2;
+    return blocks;
+}
+
+static ClusterShape cluster_plan(int rows, int cols, int blocks, float x_scale, float a_scale, float b_scale) {
+    ClusterShape sh = cluster_shape(rows, cols, blocks);
+    sh.x_scale = x_scale;
+    sh.to_a = a_scale / (x_scale * x_scale);
+    sh.to_d = 1.f / (x_scale * x_scale);
+    sh.unscale_b = 1.f / b_scale;
+    sh.unscale_x = 1.f / x_scale;
+    return sh;
+}
+static ClusterSteps cluster_steps(const OrthoCoefficients &co, float a_scale, float b_scale) {
+    ClusterSteps steps = {};
+    steps.n = co.steps;
     for (int k = 0; k < co.steps; ++k) {
         const float a = co.c[k][0], b = co.c[k][1], c = co.c[k][2];
         const float v[7] = {a, b * (b_scale / a_scale), c * (b_scale / a_scale), c * (b_scale / (a_scale * a_scale)), b, c,
                             c / (a_scale * a_scale)};
-        std::copy(v, v + 7, steps->c[k]);
+        std::copy(v, v + 7, steps.c[k]);
     }
-    if (batch * sh->blocks > 0x7fffffffll) return set_error(kErrInvalidArgument, "%s: too many matrices", what);
-    return kOk;
+    return steps;
 }
 
 int ortho_cluster_fwd(long long batch, int rows, int cols, int dtype, const void *x, void *y, const OrthoCoefficients &co,
                       float x_scale, float a_scale, float b_scale, float eps, const ClusterKept &kept, cudaStream_t stream) {
-    ClusterShape sh;
-    ClusterSteps st = {};
-    if (int e = cluster_plan("orthogonalize", batch, rows, cols, co, x_scale, a_scale, b_scale, &sh, &st)) return e;
+    ClusterShapes<false> sh = {};
+    const int sizes[1][2] = {{rows, cols}};
+    sh.of[0] = cluster_plan(rows, cols, cluster_widen(sizes, 1, batch), x_scale, a_scale, b_scale);
+    const ClusterSteps st = cluster_steps(co, a_scale, b_scale);
     static const MuonTable none = {};
-    if (dtype == kOrthoF32) return cluster_launch<float, float, false>(batch, sh, x, y, none, st, eps, kept, stream);
-    if (dtype == kOrthoBF16) return cluster_launch<__nv_bfloat16, float, false>(batch, sh, x, y, none, st, eps, kept, stream);
-    return cluster_launch<__half, float, false>(batch, sh, x, y, none, st, eps, kept, stream);
+    const size_t smem = sh.of[0].smem;
+    if (dtype == kOrthoF32) return cluster_launch<float, float, false>(batch, sh, smem, x, y, none, st, eps, kept, stream);
+    if (dtype == kOrthoBF16) return cluster_launch<__nv_bfloat16, float, false>(batch, sh, smem, x, y, none, st, eps, kept, stream);
+    return cluster_launch<__half, float, false>(batch, sh, smem, x, y, none, st, eps, kept, stream);
 }
 
-int ortho_cluster_muon(const MuonTable &t, int rows, int cols, const OrthoCoefficients &co, float x_scale, float a_scale,
-                       float b_scale, float eps, cudaStream_t stream) {
-    ClusterShape sh;
-    ClusterSteps st = {};
+int ortho_cluster_muon(const MuonTable &t, const int sizes[][2], const OrthoCoefficients &co, float x_scale, float a_scale, float b_scale,
+                       float eps, cudaStream_t stream) {
+    ClusterShapes<true> sh = {};
+    size_t smem = 0;
+    const int blocks = cluster_widen(sizes, t.n, t.first[t.n]);
+    for (int i = 0; i < t.n; ++i) {
+        sh.of[i] = cluster_plan(sizes[i][0], sizes[i][1], blocks, x_scale, a_scale, b_scale);
+        smem = std::max(smem, sh.of[i].smem);
+    }
+    const ClusterSteps st = cluster_steps(co, a_scale, b_scale);
+    const ClusterKept none = {};
     const long long batch = t.first[t.n];
-    if (int e = cluster_plan("muon", batch, rows, cols, co, x_scale, a_scale, b_scale, &sh, &st)) return e;
     const bool same = t.dtype == t.state_dtype;
-    if (t.dtype == kOrthoF32) return cluster_launch<float, float, true>(batch, sh, nullptr, nullptr, t, st, eps, ClusterKept{}, stream);
+    if (t.dtype == kOrthoF32) return cluster_launch<float, float, true>(batch, sh, smem, nullptr, nullptr, t, st, eps, none, stream);
     if (t.dtype == kOrthoBF16)
-        return same ? cluster_launch<__nv_bfloat16, __nv_bfloat16, true>(batch, sh, nullptr, nullptr, t, st, eps, ClusterKept{}, stream)
-                    : cluster_launch<__nv_bfloat16, float, true>(batch, sh, nullptr, nullptr, t, st, eps, ClusterKept{}, stream);
-    return same ? cluster_launch<__half, __half, true>(batch, sh, nullptr, nullptr, t, st, eps, ClusterKept{}, stream)
-                : cluster_launch<__half, float, true>(batch, sh, nullptr, nullptr, t, st, eps, ClusterKept{}, stream);
+        return same ? cluster_launch<__nv_bfloat16, __nv_bfloat16, true>(batch, sh, smem, nullptr, nullptr, t, st, eps, none, stream)
+                    : cluster_launch<__nv_bfloat16, float, true>(batch, sh, smem, nullptr, nullptr, t, st, eps, none, stream);
+    return same ? cluster_launch<__half, __half, true>(batch, sh, smem, nullptr, nullptr, t, st, eps, none, stream)
+                : cluster_launch<__half, float, true>(batch, sh, smem, nullptr, nullptr, t, st, eps, none, stream);
 }
 
 } // namespace gsb

@@ -868,29 +868,67 @@ static MuonTable table_part(const MuonTable &all, long long from, long long n, i
     return t;
 }
 
-extern "C" int gsb_muon(int n_tensors, const GsbMuonTensor *tensors, int rows, int cols, int dtype, int state_dtype,
-                        const bool *valid, float momentum, int nesterov, int steps, const float *coefficients, float eps,
-                        void *scratch, size_t scratch_bytes, cudaStream_t stream) {
-    OrthoCoefficients co = {};
-    if (int e = check_common("muon", 0, rows, cols, dtype, steps, coefficients, eps, &co)) return e;
-    if (state_dtype != dtype && state_dtype != kOrthoF32)
-        return set_error(kErrUnsupported, "muon: the momentum buffer has the parameter's type or float32");
+// How a tensor of a Muon step is computed, and what it is computed together with: thin matrices with those
+// of their shape, clustered ones with those of their cluster's size, tiled ones with those of their shape or its transpose.
+enum MuonKind : int { kMuonThin, kMuonClustered, kMuonTiled };
+struct MuonKey {
+    int kind, a, b;
+    bool operator==(const MuonKey &o) const { return kind == o.kind && a == o.a && b == o.b; }
+};
+static MuonKey muon_key(const GsbMuonTensor &t) {
+    if (ortho_is_thin(t.rows, t.cols)) return {kMuonThin, t.rows, t.cols};
+    if (const int blocks = ortho_is_clustered(t.rows, t.cols)) return {kMuonClustered, blocks, 0};
+    return {kMuonTiled, std::min(t.rows, t.cols), std::max(t.rows, t.cols)};
+}
+static bool muon_empty(const GsbMuonTensor &t) { return t.batch == 0 || t.rows == 0 || t.cols == 0; }
+// Whether tensor i is the first of its key.
+static bool muon_leads(const GsbMuonTensor *tensors, int i, const MuonKey &key) {
+    if (muon_empty(tensors[i])) return false;
+    for (int j = 0; j < i; ++j)
+        if (!muon_empty(tensors[j]) && muon_key(tensors[j]) == key) return false;
+    return true;
+}
+static long long muon_matrices(const GsbMuonTensor *tensors, int n, const MuonKey &key) {
+    long long total = 0;
+    for (int i = 0; i < n; ++i)
+        if (!muon_empty(tensors[i]) && muon_key(tensors[i]) == key) total += tensors[i].batch;
+    return total;
+}
+static int check_tensors(int n_tensors, const GsbMuonTensor *tensors) {
     if (n_tensors < 0) return set_error(kErrInvalidArgument, "muon: negative tensor count");
     if (n_tensors > 0 && tensors == nullptr) return set_error(kErrInvalidArgument, "muon: no tensor list");
-    long long total = 0;
     for (int i = 0; i < n_tensors; ++i) {
-        if (tensors[i].batch < 0 || tensors[i].inner < 1)
-            return set_error(kErrInvalidArgument, "muon: tensor %d: batch %lld, inner %d", i, tensors[i].batch, tensors[i].inner);
-        total += tensors[i].batch;
+        const GsbMuonTensor &t = tensors[i];
+        if (t.batch < 0 || t.rows < 0 || t.cols < 0 || t.inner < 1)
+            return set_error(kErrInvalidArgument, "muon: tensor %d: %lld x [%d, %d], inner %d", i, t.batch, t.rows, t.cols, t.inner);
     }
-    if (total == 0 || rows == 0 || cols == 0) return kOk;
-    const bool thin = ortho_is_thin(rows, cols), clustered = !thin && ortho_is_clustered(rows, cols);
-    OrthoPlan p = {};
-    if (!thin) {
-        p = make_plan(rows, cols, dtype, co, false, false);
-        if (!clustered && (scratch == nullptr || scratch_bytes < plan_bytes(p, total)))
-            return set_error(kErrInvalidArgument, "muon: %zu scratch bytes are needed", plan_bytes(p, total));
+    return kOk;
+}
+
+extern "C" size_t gsb_muon_scratch_bytes(int n_tensors, const GsbMuonTensor *tensors, int dtype, int steps) {
+    if (check_tensors(n_tensors, tensors) != kOk || steps < 1 || steps > kOrthoMaxSteps) return 0;
+    OrthoCoefficients co = {};
+    co.steps = steps;
+    size_t most = 0;
+    for (int i = 0; i < n_tensors; ++i) {
+        const MuonKey key = muon_key(tensors[i]);
+        if (key.kind == kMuonTiled && muon_leads(tensors, i, key))
+            most = std::max(most, plan_bytes(ortho_plan(key.a, key.b, dtype, co, false, false), muon_matrices(tensors, n_tensors, key)));
     }
+    return most;
+}
+
+extern "C" int gsb_muon(int n_tensors, const GsbMuonTensor *tensors, int dtype, int state_dtype, const bool *valid, float momentum,
+                        int nesterov, int steps, const float *coefficients, float eps, void *scratch, size_t scratch_bytes,
+                        cudaStream_t stream) {
+    OrthoCoefficients co = {};
+    if (int e = check_common("muon", 0, 0, 0, dtype, steps, coefficients, eps, &co)) return e;
+    if (state_dtype != dtype && state_dtype != kOrthoF32)
+        return set_error(kErrUnsupported, "muon: the momentum buffer has the parameter's type or float32");
+    if (int e = check_tensors(n_tensors, tensors)) return e;
+    const size_t needed = gsb_muon_scratch_bytes(n_tensors, tensors, dtype, steps);
+    if (needed > 0 && (scratch == nullptr || scratch_bytes < needed))
+        return set_error(kErrInvalidArgument, "muon: %zu scratch bytes are needed", needed);
     MuonTable t = {};
     t.dtype = dtype;
     t.state_dtype = state_dtype;
@@ -898,42 +936,52 @@ extern "C" int gsb_muon(int n_tensors, const GsbMuonTensor *tensors, int rows, i
     t.mu = momentum;
     t.one_minus_mu = (float)(1.0 - (double)momentum);
     t.valid = valid;
-    auto run = [&](bool turned) -> int { // the tensors gathered in t
-        if (t.n == 0) return kOk;
-        int e = kOk;
-        const int r = turned ? cols : rows, c = turned ? rows : cols;
-        if (thin) {
-            e = ortho_thin_muon(t, r, c, co, eps, stream);
-        } else if (clustered) {
-            e = ortho_cluster_muon(t, r, c, co, (float)p.s.x, (float)p.s.a, (float)p.s.b, eps, stream);
-        } else {
-            const long long here = t.first[t.n], chunk = ortho_chunk(p, total);
-            for (long long b = 0; b < here && e == kOk; b += chunk) {
-                const long long n = std::min(chunk, here - b);
-                e = ortho_tiled_fwd(p, co, n, nullptr, nullptr, dtype, table_part(t, b, n, rows, cols), eps,
-                                    static_cast<char *>(scratch), stream);
+    int sizes[kOrthoMaxTensors][2]; // rows and columns of the tensors in t
+    for (int i = 0; i < n_tensors; ++i) {
+        const MuonKey key = muon_key(tensors[i]);
+        if (!muon_leads(tensors, i, key)) continue;
+        OrthoPlan p = {};
+        long long chunk = 0;
+        if (key.kind != kMuonThin) p = make_plan(tensors[i].rows, tensors[i].cols, dtype, co, false, false);
+        if (key.kind == kMuonTiled) {
+            p = make_plan(key.a, key.b, dtype, co, false, false);
+            chunk = ortho_chunk(p, muon_matrices(tensors, n_tensors, key));
+        }
+        auto run = [&]() -> int { // the tensors gathered in t
+            if (t.n == 0) return kOk;
+            int e = kOk;
+            if (key.kind == kMuonThin) {
+                e = ortho_thin_muon(t, key.a, key.b, co, eps, stream);
+            } else if (key.kind == kMuonClustered) {
+                e = ortho_cluster_muon(t, sizes, co, (float)p.s.x, (float)p.s.a, (float)p.s.b, eps, stream);
+            } else {
+                const long long here = t.first[t.n];
+                for (long long b = 0; b < here && e == kOk; b += chunk) {
+                    const long long n = std::min(chunk, here - b);
+                    e = ortho_tiled_fwd(p, co, n, nullptr, nullptr, dtype, table_part(t, b, n, key.a, key.b), eps,
+                                        static_cast<char *>(scratch), stream);
+                }
             }
-        }
-        t.n = 0;
-        return e;
-    };
-    // the tiled path takes both orientations together, the others one after the other
-    for (int pass = 0; pass < (thin || clustered ? 2 : 1); ++pass) {
-        for (int i = 0; i < n_tensors; ++i) {
-            const bool turned = tensors[i].turned != 0;
-            if (tensors[i].batch == 0 || ((thin || clustered) && turned != (pass == 1))) continue;
-            t.param[t.n] = tensors[i].param;
-            t.grad[t.n] = tensors[i].grad;
-            t.momentum[t.n] = tensors[i].momentum_buffer;
-            t.lr[t.n] = tensors[i].lr;
-            t.decay[t.n] = tensors[i].decay;
-            t.inner[t.n] = tensors[i].inner;
-            t.transposed[t.n] = turned != (rows > cols);
-            t.first[t.n + 1] = t.first[t.n] + tensors[i].batch;
+            t.n = 0;
+            return e;
+        };
+        for (int j = i; j < n_tensors; ++j) {
+            const GsbMuonTensor &u = tensors[j];
+            if (muon_empty(u) || !(muon_key(u) == key)) continue;
+            t.param[t.n] = u.param;
+            t.grad[t.n] = u.grad;
+            t.momentum[t.n] = u.momentum_buffer;
+            t.lr[t.n] = u.lr;
+            t.decay[t.n] = u.decay;
+            t.inner[t.n] = u.inner;
+            t.transposed[t.n] = u.rows > u.cols;
+            t.first[t.n + 1] = t.first[t.n] + u.batch;
+            sizes[t.n][0] = u.rows;
+            sizes[t.n][1] = u.cols;
             if (++t.n == kOrthoMaxTensors)
-                if (int e = run(pass == 1)) return e;
+                if (int e = run()) return e;
         }
-        if (int e = run(pass == 1)) return e;
+        if (int e = run()) return e;
     }
     return kOk;
 }

@@ -63,8 +63,9 @@ class GsbMuonTensor(ctypes.Structure):
         ("grad", P),
         ("momentum_buffer", P),
         ("batch", I64),
+        ("rows", I32),
+        ("cols", I32),
         ("inner", I32),
-        ("turned", I32),
         ("lr", F32),
         ("decay", F32),
     ]
@@ -174,7 +175,8 @@ SIGNATURES = {
     "gsb_orthogonalize_scratch_bytes": (SZ, [I64, I32, I32, I32, I32, I32, I32]),
     "gsb_orthogonalize_fwd": (I32, [I64, I32, I32, I32, P, P, I32, P, F32, P, SZ, P, SZ, P]),
     "gsb_orthogonalize_bwd": (I32, [I64, I32, I32, I32, P, P, P, I32, P, F32, P, SZ, P, SZ, P]),
-    "gsb_muon": (I32, [I32, ctypes.POINTER(GsbMuonTensor), I32, I32, I32, I32, P, F32, I32, I32, P, F32, P, SZ, P]),
+    "gsb_muon_scratch_bytes": (SZ, [I32, ctypes.POINTER(GsbMuonTensor), I32, I32]),
+    "gsb_muon": (I32, [I32, ctypes.POINTER(GsbMuonTensor), I32, I32, P, F32, I32, I32, P, F32, P, SZ, P]),
 }
 
 

@@ -257,7 +257,8 @@ def muon(
     ``nesterov``, else m; param = param (1 - lr weight_decay) - lr ``orthogonalize(u)``. Gradients have
     their parameter's type (float32, bfloat16 or float16), buffers that type or float32. As in :func:`adam`, ``valid``
     masks the leading dimension, which all params then share (three dimensions or more): masked matrices keep their parameter
-    and momentum. Tensors of one type and one shape (or its transpose) go through the kernels together. A tensor must not be listed
+    and momentum. Tensors of one shape (or its transpose), and
+    small matrices of any, go through the kernels together. A tensor must not be listed
     twice or overlap another.
     """
     if isinstance(params, Tensor):
@@ -306,8 +307,8 @@ def muon(
         rows, cols = shape[-2:]
         batch = numel // (rows * cols)
         inner = batch // shape[0] if len(shape) > 2 else 1
-        key = (cols, rows, dtype, state_dtype) if rows > cols else (rows, cols, dtype, state_dtype)
-        groups.setdefault(key, []).append((at_p, at_g, at_m, batch, inner, rows > cols, rate, 1.0 - rate * weight_decay))
+        groups.setdefault((dtype, state_dtype), []).append(
+            (at_p, at_g, at_m, batch, rows, cols, inner, rate, 1.0 - rate * weight_decay))
     read_end = write_end = 0
     for start, end, read_only in sorted(spans):
         if start < write_end or (not read_only and start < read_end):
@@ -318,12 +319,13 @@ def muon(
             write_end = max(write_end, end)
     with device_guard(device):
         stream = stream_of(params[0])
-        for (rows, cols, dtype, state_dtype), entries in groups.items():
-            arr = (_B.GsbMuonTensor * len(entries))(*entries)
-            scratch_bytes = _ortho_scratch_bytes(sum(e[3] for e in entries), rows, cols, dtype, steps, 0, 0)
+        for (dtype, state_dtype), entries in groups.items():
+            n = len(entries)
+            arr = (_B.GsbMuonTensor * n)(*entries)
+            scratch_bytes = lib().gsb_muon_scratch_bytes(n, arr, dtype, steps)
             scratch = _bytes(scratch_bytes, device)
-            call("gsb_muon", len(entries), arr, rows, cols, dtype, state_dtype, ptr(valid), momentum, int(nesterov),
-                 steps, coefficients, eps, ptr(scratch), scratch_bytes, stream)
+            call("gsb_muon", n, arr, dtype, state_dtype, ptr(valid), momentum, int(nesterov), steps, coefficients, eps,
+                 ptr(scratch), scratch_bytes, stream)
     torch.autograd.graph.increment_version(params + momentum_buffers)
 
 

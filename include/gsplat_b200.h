@@ -470,15 +470,13 @@ GSB_API int gsb_adam_multi(int n_groups, const GsbAdamGroup *groups, const bool 
  * `kept` state of gsb_orthogonalize_kept_bytes (0: there is none for this shape, or it would be
  * above 1 GiB with the scratch) that the forward call wrote, the backward call, of the
  * same arguments, need not take the steps again; both may have NULL instead.
- * gsb_muon: for the listed tensors, each a batch of matrices of one shape (or its
- * transpose) and type: m <- m + (1 - momentum)(grad - m); u = grad + momentum (m - grad) (nesterov)
+ * gsb_muon: for the listed tensors of one type, each a batch of matrices: m <- m + (1 - momentum)(grad - m); u = grad + momentum (m - grad) (nesterov)
  * or m; param <- decay * param - lr * orthogonalized(u). momentum_buffer has
  * the type of param or float32 (state_dtype). valid (optional): a row of a tensor's leading
  * dimension (`inner` matrices) whose entry is false is neither read nor
  * written. Tensors must not overlap.
- * Scratch: gsb_orthogonalize_scratch_bytes of the whole batch (gsb_muon: the sum
- * of the tensors' batches, backward = kept = 0; kept = 1: for a call with a kept state);
- * 0 where none is needed. Calls that may run at the same time need scratch of their own. */
+ * Scratch: gsb_orthogonalize_scratch_bytes of the whole batch (kept = 1: for a call with a
+ * kept state), gsb_muon_scratch_bytes of the list; 0 where none is needed. Calls that may run at the same time need scratch of their own. */
 GSB_API size_t gsb_orthogonalize_kept_bytes(long long batch, int rows, int cols, int steps);
 GSB_API size_t gsb_orthogonalize_scratch_bytes(long long batch, int rows, int cols, int dtype,
                                        int steps, int backward, int kept);
@@ -495,13 +493,15 @@ typedef struct GsbMuonTensor {
     const void *grad;
     void *momentum_buffer;
     long long batch; /* matrices */
+    int rows;
+    int cols;
     int inner;       /* matrices of one row of the leading dimension */
-    int turned;      /* the tensor's matrices are [cols, rows] */
     float lr;
     float decay;     /* 1 - lr * weight_decay */
 } GsbMuonTensor;
-GSB_API int gsb_muon(int n_tensors, const GsbMuonTensor *tensors, int rows, int cols, int dtype,
-             int state_dtype, const bool *valid, float momentum, int nesterov, int steps,
+GSB_API size_t gsb_muon_scratch_bytes(int n_tensors, const GsbMuonTensor *tensors, int dtype, int steps);
+GSB_API int gsb_muon(int n_tensors, const GsbMuonTensor *tensors, int dtype, int state_dtype,
+             const bool *valid, float momentum, int nesterov, int steps,
              const float *coefficients, float eps, void *scratch, size_t scratch_bytes,
              cudaStream_t stream);
 

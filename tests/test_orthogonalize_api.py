@@ -84,11 +84,20 @@ def test_c_entry_points_refuse_before_any_launch():
     assert fwd(batch=0) == 0 and fwd(rows=0) == 0 and fwd(cols=0) == 0
     rc = L.gsb_orthogonalize_bwd(1, 200, 200, 0, None, None, None, 5, c, 1e-7, None, 0, None, 0, None)
     assert rc == -1 and b"scratch" in L.gsb_last_error()
-    assert L.gsb_muon(1, None, 8, 8, 0, 0, None, 0.9, 1, 5, c, 1e-7, None, 0, None) == -1
-    assert b"no tensor list" in L.gsb_last_error()
-    assert L.gsb_muon(0, None, 8, 8, 0, 1, None, 0.9, 1, 5, c, 1e-7, None, 0, None) == -2
-    assert b"momentum buffer" in L.gsb_last_error()
-    assert L.gsb_muon(0, None, 8, 8, 1, 0, None, 0.9, 1, 5, c, 1e-7, None, 0, None) == 0
+    def muon(n=0, tensors=None, dtype=0, state=0, scratch=None, size=0):
+        return L.gsb_muon(n, tensors, dtype, state, None, 0.9, 1, 5, c, 1e-7, scratch, size, None)
+
+    assert muon(n=1) == -1 and b"no tensor list" in L.gsb_last_error()
+    assert muon(n=-1) == -1 and b"negative" in L.gsb_last_error()
+    assert muon(state=1) == -2 and b"momentum buffer" in L.gsb_last_error()
+    assert muon(dtype=1) == 0  # nothing to do
+    from gsplat_b200.cuda._backend import GsbMuonTensor
+
+    big = (GsbMuonTensor * 2)((None, None, None, 1, 200, 300, 1, 0.1, 1.0), (None, None, None, 0, 300, 200, 1, 0.1, 1.0))
+    assert muon(2, big) == -1 and b"scratch" in L.gsb_last_error()
+    assert L.gsb_muon_scratch_bytes(2, big, 0, 5) == L.gsb_orthogonalize_scratch_bytes(1, 200, 300, 0, 5, 0, 0)
+    for bad in ((None, None, None, -1, 8, 8, 1, 0.1, 1.0), (None, None, None, 1, -8, 8, 1, 0.1, 1.0), (None, None, None, 1, 8, 8, 0, 0.1, 1.0)):
+        assert muon(1, (GsbMuonTensor * 1)(bad)) == -1 and b"tensor 0" in L.gsb_last_error()
 
 
 def test_scratch_sizes():

@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(kThinThreads)
 }
 
 // Momentum, orthogonalisation and the parameters' step in one pass. Matrices of
-// hidden rows are neither read nor written.
+// hidden rows keep their values.
 template <typename T, typename M, int S>
 __global__ void __launch_bounds__(kThinThreads)
     thin_muon_kernel(ThinShape sh, const __grid_constant__ MuonTable tab, const __grid_constant__ OrthoCoefficients co, float eps) {
@@ -524,7 +524,7 @@ __device__ __forceinline__ void pair_iterate(uint64_t x[P][S], const OrthoCoeffi
 template <typename T, int P, int S>
 __global__ void __launch_bounds__(kStackThreads)
     stack_fwd_kernel(StackShape sh, const T *__restrict__ x_in, T *__restrict__ y, const __grid_constant__ OrthoCoefficients co, float eps) {
-    extern __shared__ float stage[];
+    extern __shared__ __align__(16) float stage[];
     const long long b0 = (long long)blockIdx.x * kStackThreads;
     const int n = (int)min((long long)kStackThreads, sh.batch - b0);
     const size_t base = (size_t)b0 * sh.E;
@@ -547,7 +547,7 @@ template <typename T, int P, int S>
 __global__ void __launch_bounds__(kStackThreads)
     stack_bwd_kernel(StackShape sh, const T *__restrict__ x_in, const T *__restrict__ v_y, T *__restrict__ v_x,
                      const __grid_constant__ OrthoCoefficients co, float eps) {
-    extern __shared__ float stage[];
+    extern __shared__ __align__(16) float stage[];
     const int threads = blockDim.x;
     uint64_t *kept = reinterpret_cast<uint64_t *>(stage + ((threads * sh.pitch + 1) & ~1)) + threadIdx.x;
     const long long b0 = (long long)blockIdx.x * threads;
@@ -628,7 +628,7 @@ template <typename T, typename M, int P, int S>
 __global__ void __launch_bounds__(kStackThreads)
     stack_muon_kernel(StackShape sh, const __grid_constant__ MuonTable tab, const __grid_constant__ StackBlocks blocks,
                       const __grid_constant__ OrthoCoefficients co, float eps) {
-    extern __shared__ float stage[];
+    extern __shared__ __align__(16) float stage[];
     __shared__ short list[kStackSpan];
     __shared__ bool visible[kStackSpan + 1];
     __shared__ int warp_count[kStackThreads / 32];
@@ -661,20 +661,6 @@ __global__ void __launch_bounds__(kStackThreads)
     M *mom = static_cast<M *>(tab.momentum[t]) + base;
     T *param = static_cast<T *>(tab.param[t]) + base;
     const int total = n * sh.E;
-    // Turn `at` of the moves: quad i and which of its values are a visible matrix's. Without hidden
-    // matrices the quads are taken as they lie; else each listed matrix's quads in turn, the
-    // first and the last of which it may share with a neighbour.
-    const int per = (sh.E + 6) / 4, turns = !blocks.vec[t] ? 0 : all ? total / 4 : count * per;
-    auto quad_at = [&](int at, unsigned &seen) -> int {
-        if (all) {
-            seen = 15u;
-            return at;
-        }
-        const int l = (int)__umulhi((uint32_t)at, sh.magic_quads), first = list[l] * sh.E, i = first / 4 + at - l * per;
-        const int from = first - 4 * i, to = first + sh.E - 4 * i; // of the quad, 0 to 4
-        seen = to <= 0 ? 0u : (15u >> max(0, 4 - to)) & (15u << max(0, from));
-        return i;
-    };
     auto one_in = [&](int e) {
         const int q = stack_matrix(sh, e);
         if (!visible[q]) return;
@@ -690,52 +676,79 @@ __global__ void __launch_bounds__(kStackThreads)
     using VT = typename Quad<T>::type;
     using VM = typename Quad<M>::type;
     constexpr int U = 4; // quads on their way at once
+    auto updated = [&](float4 g, float4 &m) -> float4 {
+        m = make_float4(muon_momentum(g.x, m.x, tab.one_minus_mu), muon_momentum(g.y, m.y, tab.one_minus_mu),
+                        muon_momentum(g.z, m.z, tab.one_minus_mu), muon_momentum(g.w, m.w, tab.one_minus_mu));
+        return make_float4(muon_update(g.x, m.x, tab.mu, tab.nesterov), muon_update(g.y, m.y, tab.mu, tab.nesterov),
+                           muon_update(g.z, m.z, tab.mu, tab.nesterov), muon_update(g.w, m.w, tab.mu, tab.nesterov));
+    };
+    // With hidden matrices, each listed one's quads in turn (turn `at` of `turns`): quad i, the values of it that are the
+    // matrix's, and their place on the stage. A quad that it shares is read whole and written value by value.
+    const int per = (sh.E + 6) / 4, turns = !blocks.vec[t] || all ? 0 : count * per, quads = blocks.vec[t] && all ? total / 4 : 0;
+    struct Part {
+        int i;
+        unsigned seen;
+        float *stage;
+    };
+    auto part = [&](int at) -> Part {
+        const int l = (int)__umulhi((uint32_t)at, sh.magic_quads), q = list[l], first = q * sh.E, i = first / 4 + at - l * per;
+        const int from = first - 4 * i, to = first + sh.E - 4 * i; // of the quad, 0 to 4
+        return {i, to <= 0 ? 0u : (15u >> max(0, 4 - to)) & (15u << max(0, from)), stage + 4 * i + (sh.pitch != sh.E ? q : 0)};
+    };
+    for (int i0 = threadIdx.x; i0 < quads; i0 += U * kStackThreads) {
+        float4 g[U], m[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (i0 + u * kStackThreads < quads) {
+                g[u] = Quad<T>::get(reinterpret_cast<const VT *>(grad)[i0 + u * kStackThreads]);
+                m[u] = Quad<M>::get(reinterpret_cast<const VM *>(mom)[i0 + u * kStackThreads]);
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (i0 + u * kStackThreads < quads) {
+                const float4 w = updated(g[u], m[u]);
+                reinterpret_cast<VM *>(mom)[i0 + u * kStackThreads] = Quad<M>::put(m[u]);
+                stage_put(sh, stage, i0 + u * kStackThreads, w);
+            }
+    }
     for (int a0 = threadIdx.x; a0 < turns; a0 += U * kStackThreads) {
         float4 g[U], m[U];
-        unsigned seen[U];
-        int quad[U];
+        Part at[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            seen[u] = 0u;
-            if (a0 + u * kStackThreads < turns) quad[u] = quad_at(a0 + u * kStackThreads, seen[u]);
-            const int i = quad[u];
-            if (seen[u] == 15u) {
-                g[u] = Quad<T>::get(reinterpret_cast<const VT *>(grad)[i]);
-                m[u] = Quad<M>::get(reinterpret_cast<const VM *>(mom)[i]);
-            } else if (seen[u]) {
-                if (seen[u] & 1u) g[u].x = to_f32(grad[4 * i]), m[u].x = to_f32(mom[4 * i]);
-                if (seen[u] & 2u) g[u].y = to_f32(grad[4 * i + 1]), m[u].y = to_f32(mom[4 * i + 1]);
-                if (seen[u] & 4u) g[u].z = to_f32(grad[4 * i + 2]), m[u].z = to_f32(mom[4 * i + 2]);
-                if (seen[u] & 8u) g[u].w = to_f32(grad[4 * i + 3]), m[u].w = to_f32(mom[4 * i + 3]);
+            at[u] = a0 + u * kStackThreads < turns ? part(a0 + u * kStackThreads) : Part{0, 0u, stage};
+            if (at[u].seen && 4 * at[u].i + 3 < total) {
+                g[u] = Quad<T>::get(reinterpret_cast<const VT *>(grad)[at[u].i]);
+                m[u] = Quad<M>::get(reinterpret_cast<const VM *>(mom)[at[u].i]);
             }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int i = quad[u];
-            if (!seen[u]) continue;
-            float4 w;
-            m[u].x = muon_momentum(g[u].x, m[u].x, tab.one_minus_mu);
-            m[u].y = muon_momentum(g[u].y, m[u].y, tab.one_minus_mu);
-            m[u].z = muon_momentum(g[u].z, m[u].z, tab.one_minus_mu);
-            m[u].w = muon_momentum(g[u].w, m[u].w, tab.one_minus_mu);
-            w.x = muon_update(g[u].x, m[u].x, tab.mu, tab.nesterov);
-            w.y = muon_update(g[u].y, m[u].y, tab.mu, tab.nesterov);
-            w.z = muon_update(g[u].z, m[u].z, tab.mu, tab.nesterov);
-            w.w = muon_update(g[u].w, m[u].w, tab.mu, tab.nesterov);
-            if (seen[u] == 15u) {
-                stage_put(sh, stage, i, w);
-                reinterpret_cast<VM *>(mom)[i] = Quad<M>::put(m[u]);
+            const unsigned seen = at[u].seen;
+            if (!seen) continue;
+            if (4 * at[u].i + 3 >= total) { // the tensor's last values
+#pragma unroll 1
+                for (int e = 4 * at[u].i; e < total; ++e) one_in(e);
+                continue;
+            }
+            const float4 w = updated(g[u], m[u]);
+            float *own = at[u].stage;
+            M *to = mom + 4 * at[u].i;
+            if (seen & 1u) own[0] = w.x;
+            if (seen & 2u) own[1] = w.y;
+            if (seen & 4u) own[2] = w.z;
+            if (seen & 8u) own[3] = w.w;
+            if (seen == 15u) {
+                *reinterpret_cast<VM *>(to) = Quad<M>::put(m[u]);
             } else {
-                // all of its values here belong to the listed matrix
-                float *own = stage + 4 * i + (sh.pitch != sh.E ? list[__umulhi((uint32_t)(a0 + u * kStackThreads), sh.magic_quads)] : 0);
-                if (seen[u] & 1u) mom[4 * i] = from_f32<M>(m[u].x), own[0] = w.x;
-                if (seen[u] & 2u) mom[4 * i + 1] = from_f32<M>(m[u].y), own[1] = w.y;
-                if (seen[u] & 4u) mom[4 * i + 2] = from_f32<M>(m[u].z), own[2] = w.z;
-                if (seen[u] & 8u) mom[4 * i + 3] = from_f32<M>(m[u].w), own[3] = w.w;
+                if (seen & 1u) to[0] = from_f32<M>(m[u].x);
+                if (seen & 2u) to[1] = from_f32<M>(m[u].y);
+                if (seen & 4u) to[2] = from_f32<M>(m[u].z);
+                if (seen & 8u) to[3] = from_f32<M>(m[u].w);
             }
         }
     }
-    for (int e = (!blocks.vec[t] ? 0 : all ? 4 * turns : total) + threadIdx.x; e < total; e += kStackThreads) one_in(e);
+    for (int e = (!blocks.vec[t] ? 0 : all ? 4 * quads : total) + threadIdx.x; e < total; e += kStackThreads) one_in(e);
     __syncthreads();
     for (int i = threadIdx.x; i < count; i += kStackThreads) {
         float *own = stage + list[i] * sh.pitch;
@@ -747,47 +760,53 @@ __global__ void __launch_bounds__(kStackThreads)
     }
     __syncthreads();
     const float lr = tab.lr[t], decay = tab.decay[t];
+    for (int i0 = threadIdx.x; i0 < quads; i0 += U * kStackThreads) {
+        float4 p[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (i0 + u * kStackThreads < quads) p[u] = Quad<T>::get(reinterpret_cast<const VT *>(param)[i0 + u * kStackThreads]);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (i0 + u * kStackThreads < quads) {
+                const float4 o = stage_get(sh, stage, i0 + u * kStackThreads);
+                reinterpret_cast<VT *>(param)[i0 + u * kStackThreads] =
+                    Quad<T>::put(make_float4(muon_param(p[u].x, o.x, lr, decay), muon_param(p[u].y, o.y, lr, decay),
+                                             muon_param(p[u].z, o.z, lr, decay), muon_param(p[u].w, o.w, lr, decay)));
+            }
+    }
     for (int a0 = threadIdx.x; a0 < turns; a0 += U * kStackThreads) {
         float4 p[U];
-        unsigned seen[U];
-        int quad[U];
+        Part at[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            seen[u] = 0u;
-            if (a0 + u * kStackThreads < turns) quad[u] = quad_at(a0 + u * kStackThreads, seen[u]);
-            const int i = quad[u];
-            if (seen[u] == 15u) {
-                p[u] = Quad<T>::get(reinterpret_cast<const VT *>(param)[i]);
-            } else if (seen[u]) {
-                if (seen[u] & 1u) p[u].x = to_f32(param[4 * i]);
-                if (seen[u] & 2u) p[u].y = to_f32(param[4 * i + 1]);
-                if (seen[u] & 4u) p[u].z = to_f32(param[4 * i + 2]);
-                if (seen[u] & 8u) p[u].w = to_f32(param[4 * i + 3]);
-            }
+            at[u] = a0 + u * kStackThreads < turns ? part(a0 + u * kStackThreads) : Part{0, 0u, stage};
+            if (at[u].seen && 4 * at[u].i + 3 < total) p[u] = Quad<T>::get(reinterpret_cast<const VT *>(param)[at[u].i]);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int i = quad[u];
-            if (!seen[u]) continue;
-            // a partial quad's values belong to the listed matrix; what lies beside them is not used
-            const float *own = stage + 4 * i;
-            if (seen[u] != 15u && sh.pitch != sh.E) own += list[__umulhi((uint32_t)(a0 + u * kStackThreads), sh.magic_quads)];
-            const float4 o = seen[u] == 15u ? stage_get(sh, stage, i) : make_float4(own[0], own[1], own[2], own[3]);
-            p[u].x = muon_param(p[u].x, o.x, lr, decay);
-            p[u].y = muon_param(p[u].y, o.y, lr, decay);
-            p[u].z = muon_param(p[u].z, o.z, lr, decay);
-            p[u].w = muon_param(p[u].w, o.w, lr, decay);
-            if (seen[u] == 15u) {
-                reinterpret_cast<VT *>(param)[i] = Quad<T>::put(p[u]);
+            const unsigned seen = at[u].seen;
+            if (!seen) continue;
+            if (4 * at[u].i + 3 >= total) {
+#pragma unroll 1
+                for (int e = 4 * at[u].i; e < total; ++e) one_out(e);
+                continue;
+            }
+            // beside the matrix's values lie others, or the room behind the stage, which are not used
+            const float *own = at[u].stage;
+            T *to = param + 4 * at[u].i;
+            const float4 w = make_float4(muon_param(p[u].x, own[0], lr, decay), muon_param(p[u].y, own[1], lr, decay),
+                                         muon_param(p[u].z, own[2], lr, decay), muon_param(p[u].w, own[3], lr, decay));
+            if (seen == 15u) {
+                *reinterpret_cast<VT *>(to) = Quad<T>::put(w);
             } else {
-                if (seen[u] & 1u) param[4 * i] = from_f32<T>(p[u].x);
-                if (seen[u] & 2u) param[4 * i + 1] = from_f32<T>(p[u].y);
-                if (seen[u] & 4u) param[4 * i + 2] = from_f32<T>(p[u].z);
-                if (seen[u] & 8u) param[4 * i + 3] = from_f32<T>(p[u].w);
+                if (seen & 1u) to[0] = from_f32<T>(w.x);
+                if (seen & 2u) to[1] = from_f32<T>(w.y);
+                if (seen & 4u) to[2] = from_f32<T>(w.z);
+                if (seen & 8u) to[3] = from_f32<T>(w.w);
             }
         }
     }
-    for (int e = (!blocks.vec[t] ? 0 : all ? 4 * turns : total) + threadIdx.x; e < total; e += kStackThreads) one_out(e);
+    for (int e = (!blocks.vec[t] ? 0 : all ? 4 * quads : total) + threadIdx.x; e < total; e += kStackThreads) one_out(e);
 }
 
 inline ThinShape thin_shape(long long batch, int rows, int cols) {

@@ -473,8 +473,7 @@ GSB_API int gsb_adam_multi(int n_groups, const GsbAdamGroup *groups, const bool 
  * gsb_muon: for the listed tensors of one type, each a batch of matrices: m <- m + (1 - momentum)(grad - m); u = grad + momentum (m - grad) (nesterov)
  * or m; param <- decay * param - lr * orthogonalized(u). momentum_buffer has
  * the type of param or float32 (state_dtype). valid (optional): a row of a tensor's leading
- * dimension (`inner` matrices) whose entry is false is neither read nor
- * written. Tensors must not overlap.
+ * dimension (`inner` matrices) whose entry is false keeps its values. Tensors must not overlap.
  * Scratch: gsb_orthogonalize_scratch_bytes of the whole batch (kept = 1: for a call with a
  * kept state), gsb_muon_scratch_bytes of the list; 0 where none is needed. Calls that may run at the same time need scratch of their own. */
 GSB_API size_t gsb_orthogonalize_kept_bytes(long long batch, int rows, int cols, int steps);

@@ -146,21 +146,46 @@ __device__ __forceinline__ OutAt out_at(const OrthoGemm &g, const MuonTable &tab
     r.n = r.turned ? (i < g.M ? g.N - j : 0) : (lane < g.N - j ? g.M - (i - lane) : 0);
     return r;
 }
-// The parameters there, read together before they are needed.
+// The parameters there, as they are stored (a 16-bit type in the low half), read together before they are needed: a
+// conversion beside each would wait for it.
 template <int EPI>
 __device__ __forceinline__ void fetch_params(const OrthoGemm &g, const MuonTable &tab, int tensor, long long b, int i, int j, int lane,
-                                             float p[32]) {
+                                             uint32_t p[32]) {
     if (EPI != kEpiMuon) return;
     const OutAt from = out_at<EPI>(g, tab, tensor, b, i, j, lane);
+    if (from.dtype == kOrthoF32) {
+        const uint32_t *at = static_cast<const uint32_t *>(from.p) + from.at;
 #pragma unroll
-    for (int k = 0; k < 32; ++k) p[k] = k < from.n ? load_as_f32(from.p, from.at + k * from.step, from.dtype) : 0.f;
+        for (int k = 0; k < 32; ++k) p[k] = k < from.n ? at[k * from.step] : 0u;
+    } else {
+        const unsigned short *at = static_cast<const unsigned short *>(from.p) + from.at;
+#pragma unroll
+        for (int k = 0; k < 32; ++k) p[k] = k < from.n ? at[k * from.step] : 0u;
+    }
+}
+template <typename T> __device__ __forceinline__ float stored_as(uint32_t v);
+template <> __device__ __forceinline__ float stored_as<float>(uint32_t v) { return __uint_as_float(v); }
+template <> __device__ __forceinline__ float stored_as<__nv_bfloat16>(uint32_t v) { return __uint_as_float(v << 16); }
+template <> __device__ __forceinline__ float stored_as<__half>(uint32_t v) { return __half2float(__ushort_as_half((unsigned short)v)); }
+
+template <typename T, bool MUON>
+__device__ __forceinline__ void put_out(const OutAt &to, const float v[32], const uint32_t p[32], const float *stage, int lane, float lr,
+                                        float decay, bool poisoned) {
+    T *at = static_cast<T *>(to.p) + to.at;
+#pragma unroll
+    for (int k = 0; k < 32; ++k) {
+        if (k >= to.n) continue;
+        float r = to.turned ? v[k] : stage[k * kStagePitch + lane];
+        if (poisoned) r = NAN;
+        at[k * to.step] = from_f32<T>(MUON ? muon_param(stored_as<T>(p[k]), r, lr, decay) : r);
+    }
 }
 
 // The epilogue of 32 columns from j of a lane's row i, the accumulator's values in v. di, dj: the diagonal
 // at the row, and at the lane's one of the columns. stage: the warp's shared memory, with the element-wise operand.
 template <bool SPLIT, int EPI>
 __device__ __forceinline__ void finish32(const OrthoGemm &g, const MuonTable &tab, int tensor, long long b, int i, int j, int lane,
-                                         float v[32], const float p[32], float di, float dj, bool mirror, bool poisoned, float *stage) {
+                                         float v[32], const uint32_t p[32], float di, float dj, bool mirror, bool poisoned, float *stage) {
     using E = Epilogue<SPLIT, EPI>;
     const bool in_rows = i < g.M;
 #pragma unroll
@@ -230,13 +255,9 @@ __device__ __forceinline__ void finish32(const OrthoGemm &g, const MuonTable &ta
         for (int k = 0; k < 32; ++k) stage[lane * kStagePitch + k] = v[k];
         __syncwarp();
     }
-#pragma unroll
-    for (int k = 0; k < 32; ++k) {
-        if (k >= to.n) continue;
-        float r = to.turned ? v[k] : stage[k * kStagePitch + lane];
-        if (poisoned) r = NAN;
-        store_from_f32(to.p, to.at + k * to.step, to.dtype, EPI == kEpiMuon ? muon_param(p[k], r, lr, decay) : r);
-    }
+    if (to.dtype == kOrthoF32) put_out<float, EPI == kEpiMuon>(to, v, p, stage, lane, lr, decay, poisoned);
+    else if (to.dtype == kOrthoBF16) put_out<__nv_bfloat16, EPI == kEpiMuon>(to, v, p, stage, lane, lr, decay, poisoned);
+    else put_out<__half, EPI == kEpiMuon>(to, v, p, stage, lane, lr, decay, poisoned);
 }
 
 // The operand e of the warp's 32 rows and 32 columns from j, four lanes to a row; nothing past the matrix.
@@ -514,7 +535,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             const bool mirror = (at.j * BN) / kBM != at.i; // off the diagonal block
 #pragma unroll
             for (int c = 0; c < W / 32; ++c) {
-                float p[32];
+                uint32_t p[32];
                 fetch_params<EPI>(g, tab, tensor, at.b, i, j + 32 * c, lane, p);
                 stage32<SPLIT, EPI>(out_stage, lane, e);
                 if (c + 1 < W / 32) fetch32<SPLIT, EPI>(g, at.b, i - lane, j + 32 * (c + 1), lane, e);
@@ -531,18 +552,24 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     if (threadIdx.x == 0 && sh.abort) atomicExch(g.error, 1);
 }
 
+// Blocks that share a tile's depth: as many as there are SMs for, as fit their sums beside each other in the
+// leader's stages, and as have 2 us of products each (4 or 12 stages), which is what meeting costs. With
+// more tiles than the GPU has groups of SMs that a cluster must fit in (8), a power of two, and fours on 7/8 of the
+// SMs: the groups' sizes leave some of them without work.
+template <bool SPLIT, int BN> static int tile_ranks(const OrthoGemm &g, long long tiles, int sms) {
+    if (g.epilogue != kEpiGram && g.epilogue != kEpiSym) return 1;
+    constexpr int most = Stages<SPLIT, BN>::n * Stages<SPLIT, BN>::bytes / (kBM * BN * 4) + 1;
+    const int stages = (g.K + kBK - 1) / kBK * g.pairs;
+    const int ranks = (int)std::min<long long>({sms / tiles, stages / (SPLIT ? 4 : 12), most, 8});
+    return ranks < 2 ? 1 : tiles <= 8 ? ranks : ranks >= 4 && 4 * tiles <= sms * 7 / 8 ? 4 : 2;
+}
+
 template <bool SPLIT, int BN, int EPI>
 static int launch_one(const OrthoGemm &g, const GemmMaps &maps, const MuonTable &tab, int per, int tn, long long tiles,
                       int sms, cudaStream_t stream) {
     constexpr int smem = Stages<SPLIT, BN>::smem;
-    // Blocks that share a tile's depth: as many as there are SMs for, as fit their sums beside each other in the
-    // leader's stages, and as have 2 us of products each (4 or 12 stages), which is what meeting costs. With
-    // more tiles than the GPU has clusters of SMs (8), a power of two: other sizes leave SMs of each without work.
-    constexpr int most = Stages<SPLIT, BN>::n * Stages<SPLIT, BN>::bytes / (kBM * BN * 4) + 1;
-    const int stages = (g.K + kBK - 1) / kBK * g.pairs;
-    int ranks = (int)std::min<long long>({sms / tiles, stages / (SPLIT ? 4 : 12), most, 8});
-    if (tiles > 8 && ranks > 1) ranks = ranks >= 4 ? 4 : 2;
-    constexpr bool kDeep = BN == 64 && (EPI == kEpiGram || EPI == kEpiSym);
+    const int ranks = tile_ranks<SPLIT, BN>(g, tiles, sms);
+    constexpr bool kDeep = EPI == kEpiGram || EPI == kEpiSym;
     if constexpr (kDeep) {
         if (ranks > 1) {
             auto *kernel = ortho_gemm_kernel<SPLIT, BN, EPI, true>;

@@ -210,7 +210,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             };
             auto finish = [&](int c, float *v) {
                 const float dj = E::col_diag && j + c + lane < g.N ? g.diag_in[(size_t)at.b * g.M + j + c + lane] : 0.f;
-                float p[32];
+                uint32_t p[32];
                 fetch_params<EPI>(g, tab, tensor, at.b, i, j + c, lane, p);
                 stage32<SPLIT, EPI>(out_stage, lane, e);
                 if (c + 32 < W) fetch32<SPLIT, EPI>(g, at.b, i - lane, j + c + 32, lane, e);

@@ -516,9 +516,17 @@ static int run_split(const OrthoPlan &p, long long nb, const void *x, int dtype,
         using T = decltype(tv);
         using M = decltype(mv);
         constexpr bool kMuon = decltype(muon)::value;
-        if (int e = launch_after(ortho_norm_kernel<T, M, kMuon>, (unsigned)(nb * p.chunks), kNormThreads, 0, stream, "ortho_norm_kernel",
-                                 x, tab, (size_t)p.rows * p.cols, p.chunk_size, p.chunks, partial, error))
+        // the call's first launch (it resets the error word) follows the stream's order in full: what a launch before it did not
+        // wait for may be our input
+        const auto blocks = (unsigned)(nb * p.chunks);
+        const size_t numel = (size_t)p.rows * p.cols;
+        if (error) {
+            ortho_norm_kernel<T, M, kMuon><<<blocks, kNormThreads, 0, stream>>>(x, tab, numel, p.chunk_size, p.chunks, partial, error);
+            if (int e = check_launch("ortho_norm_kernel")) return e;
+        } else if (int e = launch_after(ortho_norm_kernel<T, M, kMuon>, blocks, kNormThreads, 0, stream, "ortho_norm_kernel", x, tab, numel,
+                                        p.chunk_size, p.chunks, partial, error)) {
             return e;
+        }
         const int tr = (p.rows + kSplitTile - 1) / kSplitTile, tc = (p.cols + kSplitTile - 1) / kSplitTile;
         return launch_after(ortho_split_kernel<T, M, kMuon>, (unsigned)(nb * tr * tc), kNormThreads, 0, stream, "ortho_split_kernel",
                             x, tab, p.rows, p.cols, p.transposed, (const double *)partial, p.chunks, scale, eps, norm_out, out, tr, tc);

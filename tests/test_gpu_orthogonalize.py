@@ -16,7 +16,7 @@ MANY = [(8200, 1, 1), (9000, 3, 3), (8193, 15, 3), (8300, 2, 7), (8195, 4, 25), 
 SHAPES = MANY + [(1, 1, 1), (3, 1, 7), (2, 7, 1), (1, 1, 300), (5, 2, 3), (70, 3, 3), (33, 15, 3), (9, 3, 16), (4, 4, 128),
           (2, 129, 4), (3, 5, 5), (2, 5, 131), (2, 64, 64), (1, 64, 35), (2, 100, 128), (1, 128, 128), (2, 128, 129),
           (1, 129, 127), (3, 16, 16), (2, 17, 1000), (2, 1000, 77), (1, 100, 700), (1, 128, 1024),
-          (1, 1100, 128), (1, 5, 2300), (2, 48, 95), (2, 257, 65), (1, 300, 300), (1, 130, 517), (1, 513, 384)]
+          (1, 1100, 128), (1, 5, 2300), (2, 48, 95), (1, 3, 20000), (1, 6000, 20), (1, 200, 4100), (2, 257, 65), (1, 300, 300), (1, 130, 517), (1, 513, 384)]
 
 
 def gs():
@@ -256,6 +256,42 @@ def test_muon_valid(shape):
         assert torch.equal(tp.cpu()[~valid], p[~valid]) and torch.equal(tm.cpu()[~valid], m[~valid])
         if valid.any():
             check_step(p[valid], g[valid], m[valid], tp.cpu()[valid], tm.cpu()[valid], None, 0.1, 0.9, 0.0, True)
+
+
+def test_muon_refusals():
+    p, g, m = (torch.randn(6, 4, 5, device="cuda") for _ in range(3))
+    ok = dict(momentum=0.9)
+    with pytest.raises(ValueError, match="overlap"):
+        gs().muon([p, p], [g, g], [m, m.clone()], None, 0.1, **ok)  # the same parameter twice
+    with pytest.raises(ValueError, match="overlap"):
+        gs().muon(p, p, m, None, 0.1, **ok)
+    with pytest.raises(ValueError, match="overlap"):
+        gs().muon([p[:4], p[2:]], [g[:4], g[2:]], [m[:4], m[:4].clone()], None, 0.1, **ok)
+    gs().muon([p, p.clone()], [g, g], [m, m.clone()], None, 0.1, **ok)  # a gradient may serve two
+    with pytest.raises(ValueError, match="alike"):
+        gs().muon(p, g[:5], m, None, 0.1, **ok)
+    with pytest.raises(TypeError):
+        gs().muon(p, g.half(), m, None, 0.1, **ok)
+    with pytest.raises(TypeError):
+        gs().muon(p, g, m.half(), None, 0.1, **ok)
+    with pytest.raises(RuntimeError, match="contiguous"):
+        gs().muon(p.mT, g.mT, m.mT, None, 0.1, **ok)
+    for valid in (torch.ones(5, dtype=torch.bool, device="cuda"), torch.ones(6, device="cuda"), torch.ones(6, 1, dtype=torch.bool, device="cuda")):
+        with pytest.raises(ValueError, match="valid"):
+            gs().muon(p, g, m, valid, 0.1, **ok)
+    with pytest.raises(ValueError, match="valid"):
+        gs().muon(p[0].contiguous(), g[0].contiguous(), m[0].contiguous(), torch.ones(4, dtype=torch.bool, device="cuda"), 0.1, **ok)
+    with pytest.raises(RuntimeError, match="singular value"):
+        gs().orthogonalize(p, coefficients=(2.0, 0.0, 0.0))
+
+
+def test_param_used_by_a_living_graph_is_noticed():
+    """A step in place counts as a modification: a backward pass that still needs the old values raises."""
+    w = torch.nn.Parameter(torch.randn(20, 20, device="cuda"))
+    loss = (w * w).sum()
+    gs().muon(w, torch.randn(20, 20, device="cuda"), torch.zeros(20, 20, device="cuda"), None, 0.1, 0.9)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
 
 
 def test_muon_list_of_shapes_matches_one_by_one():

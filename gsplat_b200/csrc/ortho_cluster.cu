@@ -123,18 +123,30 @@ __device__ __forceinline__ Operands operands(uint32_t p, uint32_t p_lo, uint32_t
     return {operand_desc(p, true, 0), operand_desc(p_lo, true, 0), operand_desc(q, q_k_major, chunk), operand_desc(q_lo, q_k_major, chunk),
             chunk / 16, q_k_major ? chunk / 16 : 64 * 128 / 16, q_k_major ? 2u : 128u};
 }
-// One warp: D[128, n] = P Q over `depth` (a multiple of 16).
-__device__ __forceinline__ void multiply(uint32_t d, Operands o, uint32_t idesc, int depth, uint32_t leader) {
+// One warp: D[128, n] = P Q over `depth` (a multiple of 16). The small products (hi lo and lo hi) come first: the
+// accumulator truncates at every addition, relative to the sum so far, and so only a third of the
+// additions are to a large one.
+__device__ __forceinline__ void multiply(uint32_t d, const Operands &o, uint32_t idesc, int depth, uint32_t leader) {
+    Operands at = o;
     for (int k = 0; k < depth; k += 64) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if (k + 16 * i >= depth) break;
-            mma_f16(d, o.p + 2 * i, o.q + i * o.q_step, idesc, k > 0 || i > 0, leader);
-            mma_f16(d, o.p + 2 * i, o.q_lo + i * o.q_step, idesc, true, leader);
-            mma_f16(d, o.p_lo + 2 * i, o.q + i * o.q_step, idesc, true, leader);
+            mma_f16(d, at.p + 2 * i, at.q_lo + i * o.q_step, idesc, k > 0 || i > 0, leader);
+            mma_f16(d, at.p_lo + 2 * i, at.q + i * o.q_step, idesc, true, leader);
         }
-        o.p += o.p_block, o.p_lo += o.p_block;
-        o.q += o.q_block, o.q_lo += o.q_block;
+        at.p += o.p_block, at.p_lo += o.p_block;
+        at.q += o.q_block, at.q_lo += o.q_block;
+    }
+    at = o;
+    for (int k = 0; k < depth; k += 64) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (k + 16 * i >= depth) break;
+            mma_f16(d, at.p + 2 * i, at.q + i * o.q_step, idesc, true, leader);
+        }
+        at.p += o.p_block;
+        at.q += o.q_block;
     }
 }
 

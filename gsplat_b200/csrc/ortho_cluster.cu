@@ -177,8 +177,7 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
     char *base = reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     const int x_plane = sh.m16 * sh.ns64 * 2, a_plane = sh.m16 * sh.mk * 2;
     char *x_hi = base, *x_lo = x_hi + x_plane, *a_hi = x_lo + x_plane, *a_lo = a_hi + a_plane;
-    float *partial = reinterpret_cast<float *>(a_lo + a_plane); // several blocks: [blocks, per, m16 + 4]
-    const int pitch = sh.m16 + 4;
+    float *partial = reinterpret_cast<float *>(a_lo + a_plane); // several blocks: [blocks][m16 / 4][per], four columns each
     volatile int *abort = &abort_flag;
 
     const int j0 = (int)rank * sh.ns, cols = max(0, min(sh.ns, sh.n - j0)); // this block's columns
@@ -382,7 +381,7 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
         }
         if (keep) dump(x_hi, x_lo, kept.x, step, 0, sh.m, cols, j0);
         const uint32_t owner = mine ? row / sh.per : 0; // of this row of A
-        const uint32_t to = sh.blocks > 1 ? remote(smem_u32(partial + ((int)rank * sh.per + row - (int)owner * sh.per) * pitch), owner) : 0u;
+        const uint32_t to = sh.blocks > 1 ? remote(smem_u32(partial) + ((int)rank * (sh.m16 / 4) * sh.per + row - (int)owner * sh.per) * 16, owner) : 0u;
         finish();
         if (rows_here)
             for (int c = 16 * turn; c < sh.m16; c += 64) {
@@ -393,7 +392,7 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
                 if (sh.blocks > 1) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        remote_store4(to + (c + 4 * k) * 4, make_uint4(__float_as_uint(v[4 * k]), __float_as_uint(v[4 * k + 1]),
+                        remote_store4(to + (c / 4 + k) * sh.per * 16, make_uint4(__float_as_uint(v[4 * k]), __float_as_uint(v[4 * k + 1]),
                                                                        __float_as_uint(v[4 * k + 2]), __float_as_uint(v[4 * k + 3])));
                 } else {
                     float on = 0.f;
@@ -408,32 +407,44 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
             }
         if (sh.blocks > 1) {
             cluster_sync();
-            // add up this block's rows, in the order of the blocks, and give them to all
-            const int r0 = (int)rank * sh.per, rows = max(0, min(sh.m16, r0 + sh.per) - r0), eights = sh.m16 / 8;
-            for (int t = tid; t < rows * eights; t += kClusterThreads) {
-                const int i = t / eights, c = (t - i * eights) * 8;
+            // add up this block's rows, in the order of the blocks, then give them to all
+            const int r0 = (int)rank * sh.per, rows = max(0, min(sh.m16, r0 + sh.per) - r0), pieces = rows * (sh.m16 / 8);
+            for (int t = tid; t < pieces; t += kClusterThreads) {
+                const int c8 = t / rows, i = t - c8 * rows, c = c8 * 8;
                 float v[8] = {};
-#pragma unroll 4
+#pragma unroll 8
                 for (int r = 0; r < sh.blocks; ++r) {
-                    const float4 *p = reinterpret_cast<const float4 *>(partial + (r * sh.per + i) * pitch + c);
-                    const float4 f = p[0], g = p[1];
+                    const float4 *p = reinterpret_cast<const float4 *>(partial) + (r * (sh.m16 / 4) + c / 4) * sh.per + i;
+                    const float4 f = p[0], g = p[sh.per];
                     v[0] += f.x, v[1] += f.y, v[2] += f.z, v[3] += f.w;
                     v[4] += g.x, v[5] += g.y, v[6] += g.z, v[7] += g.w;
                 }
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    if (c + k == r0 + i)
-                        for (int r = 0; r < sh.blocks; ++r) remote_store_f32(remote(smem_u32(&diag_a[r0 + i]), r), v[k] * sh.to_d);
+                    if (c + k == r0 + i) diag_a[r0 + i] = v[k] * sh.to_d;
                     v[k] = c + k == r0 + i ? 0.f : v[k] * sh.to_a;
                 }
                 uint4 hi, lo;
                 split8(v, hi, lo);
                 const uint32_t at = plane_byte(sh.m16, r0 + i, c);
-                for (int r = 0; r < sh.blocks; ++r) {
-                    remote_store4(remote(ah + at, r), hi);
-                    remote_store4(remote(al + at, r), lo);
-                }
+                *reinterpret_cast<uint4 *>(a_hi + at) = hi;
+                *reinterpret_cast<uint4 *>(a_lo + at) = lo;
             }
+            __syncthreads();
+            // as they lie: 128 bytes of a row, then the next row's, so that a warp's pieces reach the other block together
+            const int line = rows * 128, all = 2 * (sh.mk / 64) * line; // bytes of a plane's block of 64 columns; of both planes'
+            for (int u = tid * 16; u < all; u += kClusterThreads * 16) {
+                int rest = u, offset = r0 * 128;
+                while (rest >= line) rest -= line, offset += sh.m16 * 128; // at most 3 times: lo follows hi
+                const uint32_t at = offset + rest;
+                const uint4 piece = *reinterpret_cast<const uint4 *>(a_hi + at);
+#pragma unroll
+                for (int o = 1; o < kClusterMax; ++o)
+                    if (o < sh.blocks) remote_store4(remote(ah + at, (rank + o) & (sh.blocks - 1)), piece);
+            }
+            if (tid < rows)
+                for (int o = 1; o < sh.blocks; ++o)
+                    remote_store_f32(remote(smem_u32(&diag_a[r0 + tid]), (rank + o) & (sh.blocks - 1)), diag_a[r0 + tid]);
             asm volatile("fence.proxy.async.shared::cluster;" ::: "memory");
             cluster_sync();
         }
@@ -593,7 +604,7 @@ static ClusterShape cluster_shape(int rows, int cols, int blocks) {
     while (s.columns < std::max(s.m16, s.ns)) s.columns *= 2;
     const size_t planes = 4 * (size_t)s.m16 * (s.ns64 + s.mk);
     // a 128-row operand reads past a plane of fewer rows: into what follows, whose rows of the product are not read
-    size_t smem = 1024 + planes + std::max<size_t>(blocks > 1 ? 4 * (size_t)s.per * blocks * (s.m16 + 4) : 0, (size_t)(128 - s.m16) * 128);
+    size_t smem = 1024 + planes + std::max<size_t>(blocks > 1 ? 4 * (size_t)s.per * blocks * s.m16 : 0, (size_t)(128 - s.m16) * 128);
     // blocks that share an SM must find their TMEM columns free: as large a part of its shared memory as of its TMEM
     smem = std::max(smem, kClusterSmem * s.columns / 512 - kClusterStatic);
     s.smem = smem;

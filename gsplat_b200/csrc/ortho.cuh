@@ -67,18 +67,6 @@ template <> struct Quad<__nv_bfloat16> {
     }
 };
 
-// One value of a type known at run time (uniform over the launch).
-__device__ __forceinline__ float load_as_f32(const void *p, size_t i, int dtype) {
-    if (dtype == kOrthoF32) return static_cast<const float *>(p)[i];
-    if (dtype == kOrthoBF16) return to_f32(static_cast<const __nv_bfloat16 *>(p)[i]);
-    return to_f32(static_cast<const __half *>(p)[i]);
-}
-__device__ __forceinline__ void store_from_f32(void *p, size_t i, int dtype, float v) {
-    if (dtype == kOrthoF32) static_cast<float *>(p)[i] = v;
-    else if (dtype == kOrthoBF16) static_cast<__nv_bfloat16 *>(p)[i] = from_f32<__nv_bfloat16>(v);
-    else static_cast<__half *>(p)[i] = from_f32<__half>(v);
-}
-
 // Momentum and the matrix that is orthogonalised, in 32 bits: m <- m + (1 - mu)(g - m),
 // u = g + mu (m - g) (Nesterov) or m.
 __device__ __forceinline__ float muon_momentum(float g, float m, float one_minus_mu) {

@@ -3,7 +3,8 @@
 // the first read to the last write.
 //
 // What bounds such a matrix is not its products but the chain of them: 15 launches of
-// the tiled kernel took 165 us for a stack of 64 x 64. Here a step is
+// the tiled kernel took 165 us for a stack of 64 x 64, this takes 25 ([77, 1000] x 12 54, [128, 1024] 69; a step of 64 x 64 3.8,
+// a third each for A, B and X: 0.7 until the product is there, 0.4 for its end). Here a step is
 //   A = X X^T      each block multiplies its slab; with several blocks the partial
 //                  sums are exchanged through distributed shared memory (each block adds up some rows
 //                  of A, in the order of the blocks, and gives them to all)

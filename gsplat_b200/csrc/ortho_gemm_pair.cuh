@@ -2,6 +2,8 @@
 // (tcgen05 cta_group::2). Each holds 128 rows of P and 128 of Q's 256 columns, and reads half as many operand
 // bytes from its shared memory for a product as with a tile of its own: a 128 x 128 tile
 // wants 126 bytes a cycle for its operands and 85 to 123 for the copies that fill its stages, of an SM's 128.
+// Measured at 4096 x 4096: A 150 us, B 170, X 305 split (72% of cycles with the tensor cores at work; three products each),
+// and 68 for X of 2048 x 8192 with hi alone, where the L2's bytes bound it.
 // The rest is as in ortho_gemm.cuh: the leader (rank 0) issues the products for both; the copies of both are
 // counted on the leader's barriers, and its commits free the stages and hand over the accumulators of both.
 #pragma once
@@ -10,7 +12,8 @@
 
 namespace gsb {
 
-constexpr int kPair = 256; // rows and columns of a tile
+constexpr int kPair = 256;   // rows and columns of a tile
+constexpr int kPairChunk = 8; // stages between two readings of the accumulator, split (4 cost 8% of a product)
 
 // Split sums go on in 128 registers of an epilogue thread, more than three warpgroups at 168 leave it: the
 // warpgroup of the copies and products gives 112 of its own. 2 x 224 + 56 = 3 x 168.
@@ -92,7 +95,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 
     const int kblocks = (g.K + kBK - 1) / kBK;
     const int total = kblocks * g.pairs;
-    const int chunk = SPLIT ? kChunk : total;
+    const int chunk = SPLIT ? kPairChunk : total;
     if (warp >= kEpilogueWarps) {
     if (SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegisters));
     if (warp == kEpilogueWarps) {

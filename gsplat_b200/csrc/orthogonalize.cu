@@ -889,19 +889,29 @@ static MuonKey muon_key(const GsbMuonTensor &t) {
     return {kMuonTiled, std::min(t.rows, t.cols), std::max(t.rows, t.cols)};
 }
 static bool muon_empty(const GsbMuonTensor &t) { return t.batch == 0 || t.rows == 0 || t.cols == 0; }
-// Whether tensor i is the first of its key.
-static bool muon_leads(const GsbMuonTensor *tensors, int i, const MuonKey &key) {
-    if (muon_empty(tensors[i])) return false;
-    for (int j = 0; j < i; ++j)
-        if (!muon_empty(tensors[j]) && muon_key(tensors[j]) == key) return false;
-    return true;
-}
-static long long muon_matrices(const GsbMuonTensor *tensors, int n, const MuonKey &key) {
-    long long total = 0;
-    for (int i = 0; i < n; ++i)
-        if (!muon_empty(tensors[i]) && muon_key(tensors[i]) == key) total += tensors[i].batch;
-    return total;
-}
+// A list is taken in slices, whose keys are worked out once; tensors of different slices are not computed together.
+constexpr int kMuonSlice = 256;
+struct MuonSlice {
+    int n;
+    const GsbMuonTensor *tensors;
+    MuonKey keys[kMuonSlice];
+
+    MuonSlice(const GsbMuonTensor *all, int from, int count) : n(std::min(count - from, kMuonSlice)), tensors(all + from) {
+        for (int i = 0; i < n; ++i) keys[i] = muon_empty(tensors[i]) ? MuonKey{-1, 0, 0} : muon_key(tensors[i]);
+    }
+    bool leads(int i) const { // whether tensor i is the first of its key
+        if (keys[i].kind < 0) return false;
+        for (int j = 0; j < i; ++j)
+            if (keys[j] == keys[i]) return false;
+        return true;
+    }
+    long long matrices(const MuonKey &key) const {
+        long long total = 0;
+        for (int i = 0; i < n; ++i)
+            if (keys[i] == key) total += tensors[i].batch;
+        return total;
+    }
+};
 static int check_tensors(int n_tensors, const GsbMuonTensor *tensors) {
     if (n_tensors < 0) return set_error(kErrInvalidArgument, "muon: negative tensor count");
     if (n_tensors > 0 && tensors == nullptr) return set_error(kErrInvalidArgument, "muon: no tensor list");
@@ -918,10 +928,13 @@ extern "C" size_t gsb_muon_scratch_bytes(int n_tensors, const GsbMuonTensor *ten
     OrthoCoefficients co = {};
     co.steps = steps;
     size_t most = 0;
-    for (int i = 0; i < n_tensors; ++i) {
-        const MuonKey key = muon_key(tensors[i]);
-        if (key.kind == kMuonTiled && muon_leads(tensors, i, key))
-            most = std::max(most, plan_bytes(ortho_plan(key.a, key.b, dtype, co, false, false), muon_matrices(tensors, n_tensors, key)));
+    for (int from = 0; from < n_tensors; from += kMuonSlice) {
+        const MuonSlice slice(tensors, from, n_tensors);
+        for (int i = 0; i < slice.n; ++i) {
+            const MuonKey &key = slice.keys[i];
+            if (key.kind == kMuonTiled && slice.leads(i))
+                most = std::max(most, plan_bytes(ortho_plan(key.a, key.b, dtype, co, false, false), slice.matrices(key)));
+        }
     }
     return most;
 }
@@ -945,51 +958,54 @@ extern "C" int gsb_muon(int n_tensors, const GsbMuonTensor *tensors, int dtype, 
     t.one_minus_mu = (float)(1.0 - (double)momentum);
     t.valid = valid;
     int sizes[kOrthoMaxTensors][2]; // rows and columns of the tensors in t
-    for (int i = 0; i < n_tensors; ++i) {
-        const MuonKey key = muon_key(tensors[i]);
-        if (!muon_leads(tensors, i, key)) continue;
-        OrthoPlan p = {};
-        long long chunk = 0;
-        if (key.kind != kMuonThin) p = make_plan(tensors[i].rows, tensors[i].cols, dtype, co, false, false);
-        if (key.kind == kMuonTiled) {
-            p = make_plan(key.a, key.b, dtype, co, false, false);
-            chunk = ortho_chunk(p, muon_matrices(tensors, n_tensors, key));
-        }
-        auto run = [&]() -> int { // the tensors gathered in t
-            if (t.n == 0) return kOk;
-            int e = kOk;
-            if (key.kind == kMuonThin) {
-                e = ortho_thin_muon(t, key.a, key.b, co, eps, stream);
-            } else if (key.kind == kMuonClustered) {
-                e = ortho_cluster_muon(t, sizes, co, (float)p.s.x, (float)p.s.a, (float)p.s.b, eps, stream);
-            } else {
-                const long long here = t.first[t.n];
-                for (long long b = 0; b < here && e == kOk; b += chunk) {
-                    const long long n = std::min(chunk, here - b);
-                    e = ortho_tiled_fwd(p, co, n, nullptr, nullptr, dtype, table_part(t, b, n, key.a, key.b), eps,
-                                        static_cast<char *>(scratch), stream);
-                }
+    for (int from = 0; from < n_tensors; from += kMuonSlice) {
+        const MuonSlice slice(tensors, from, n_tensors);
+        for (int i = 0; i < slice.n; ++i) {
+            if (!slice.leads(i)) continue;
+            const MuonKey key = slice.keys[i];
+            OrthoPlan p = {};
+            long long chunk = 0;
+            if (key.kind != kMuonThin) p = make_plan(slice.tensors[i].rows, slice.tensors[i].cols, dtype, co, false, false);
+            if (key.kind == kMuonTiled) {
+                p = make_plan(key.a, key.b, dtype, co, false, false);
+                chunk = ortho_chunk(p, slice.matrices(key));
             }
-            t.n = 0;
-            return e;
-        };
-        for (int j = i; j < n_tensors; ++j) {
-            const GsbMuonTensor &u = tensors[j];
-            if (muon_empty(u) || !(muon_key(u) == key)) continue;
-            t.param[t.n] = u.param;
-            t.grad[t.n] = u.grad;
-            t.momentum[t.n] = u.momentum_buffer;
-            t.lr[t.n] = u.lr;
-            t.decay[t.n] = u.decay;
-            t.inner[t.n] = u.inner;
-            t.transposed[t.n] = u.rows > u.cols;
-            t.first[t.n + 1] = t.first[t.n] + u.batch;
-            sizes[t.n][0] = u.rows;
-            sizes[t.n][1] = u.cols;
-            if (++t.n == kOrthoMaxTensors)
-                if (int e = run()) return e;
+            auto run = [&]() -> int { // the tensors gathered in t
+                if (t.n == 0) return kOk;
+                int e = kOk;
+                if (key.kind == kMuonThin) {
+                    e = ortho_thin_muon(t, key.a, key.b, co, eps, stream);
+                } else if (key.kind == kMuonClustered) {
+                    e = ortho_cluster_muon(t, sizes, co, (float)p.s.x, (float)p.s.a, (float)p.s.b, eps, stream);
+                } else {
+                    const long long here = t.first[t.n];
+                    for (long long b = 0; b < here && e == kOk; b += chunk) {
+                        const long long n = std::min(chunk, here - b);
+                        e = ortho_tiled_fwd(p, co, n, nullptr, nullptr, dtype, table_part(t, b, n, key.a, key.b), eps,
+                                            static_cast<char *>(scratch), stream);
+                    }
+                }
+                t.n = 0;
+                return e;
+            };
+            for (int j = i; j < slice.n; ++j) {
+                const GsbMuonTensor &u = slice.tensors[j];
+                if (!(slice.keys[j] == key)) continue;
+                t.param[t.n] = u.param;
+                t.grad[t.n] = u.grad;
+                t.momentum[t.n] = u.momentum_buffer;
+                t.lr[t.n] = u.lr;
+                t.decay[t.n] = u.decay;
+                t.inner[t.n] = u.inner;
+                t.transposed[t.n] = u.rows > u.cols;
+                t.first[t.n + 1] = t.first[t.n] + u.batch;
+                sizes[t.n][0] = u.rows;
+                sizes[t.n][1] = u.cols;
+                if (++t.n == kOrthoMaxTensors)
+                    if (int e = run()) return e;
+            }
+            if (int e = run()) return e;
         }
-        if (int e = run()) return e;
     }
     return kOk;
 }

@@ -307,12 +307,12 @@ def test_muon_list_of_shapes_matches_one_by_one():
 
 
 def test_muon_many_tensors():
-    """More tensors of a shape than one launch takes."""
+    """More tensors of a shape than one launch takes, or one slice of the list."""
     for shape in ((3, 3), (20, 24)):
-        ps, grads, ms = ([data(shape, torch.float32, 100 + 3 * i + j, 0.1) for i in range(71)] for j in range(3))
+        ps, grads, ms = ([data(shape, torch.float32, 100 + 3 * i + j, 0.1) for i in range(300)] for j in range(3))
         tp, tm = [p.cuda() for p in ps], [m.cuda() for m in ms]
         gs().muon(tp, [g.cuda() for g in grads], tm, None, 0.02, 0.9)
-        for i in (0, 31, 32, 63, 64, 70):
+        for i in (0, 31, 32, 63, 64, 70, 255, 256, 299):
             check_step(ps[i], grads[i], ms[i], tp[i].cpu(), tm[i].cpu(), None, 0.02, 0.9, 0.0, True)
 
 

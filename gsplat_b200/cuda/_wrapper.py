@@ -165,11 +165,14 @@ def orthogonalize(
     X = x / max(|x|_F, eps), then ``steps`` (1 to 32) times A = X X^T, X = a X + (b A + c A A) X:
     every singular value s becomes p(...p(s)) with p(s) = a s + b s^3 + c s^5. The default
     coefficients bring all but the smallest near 1 in five steps; (1.5, -0.5, 0) converges to the orthogonal
-    factor itself. ``coefficients`` may also be a list with a triple for each step. Matrices are multiplied
-    with 22 significand bits, bfloat16 ones with a side above 128 with 11; the result has x's shape and type. Differentiable (once; the steps' state is kept for the backward
-    pass, about 4 steps (x.numel() + 2 B M M) bytes with M the shorter side, unless that is above 1 GiB: then it takes the
-    steps again). A matrix with a NaN or an infinity becomes NaN, others of the batch are not touched
-    by it. Polynomials that take a singular value in [0, 1] above 16 are refused.
+    factor itself. ``coefficients`` may also be a list with a triple for each step. Polynomials that
+    take a singular value in [0, 1] above 16 are refused. Matrices are multiplied with 22 significand
+    bits, bfloat16 ones with a side above 128 with 11 where no gradient is wanted; the result has x's
+    shape and type. A matrix with a NaN or an infinity becomes NaN, and no other of the batch.
+
+    Differentiable once. The steps' state is kept for the backward pass, about
+    4 steps (x.numel() + 2 B M M) bytes for B matrices of shorter side M (none where it is at most 4 and the
+    longer at most 128); where that would be above 1 GiB the backward pass takes the steps again.
     """
     if x.dim() < 2:
         raise ValueError(f"x must be [..., M, N], got {tuple(x.shape)}")
@@ -255,11 +258,10 @@ def muon(
 
     For every matrix: m += (1 - momentum) (grad - m); u = grad + momentum (m - grad) with
     ``nesterov``, else m; param = param (1 - lr weight_decay) - lr ``orthogonalize(u)``. Gradients have
-    their parameter's type (float32, bfloat16 or float16), buffers that type or float32. As in :func:`adam`, ``valid``
-    masks the leading dimension, which all params then share (three dimensions or more): masked matrices keep their parameter
-    and momentum. Tensors of one shape (or its transpose), and
-    small matrices of any, go through the kernels together. A tensor must not be listed
-    twice or overlap another.
+    their parameter's type (float32, bfloat16 or float16), buffers that type or float32. As in :func:`adam`,
+    ``valid`` masks the leading dimension, which all params then share (three dimensions or more): masked
+    matrices keep their parameter and momentum. Tensors of one shape (or its transpose), and small
+    matrices of any, go through the kernels together. A tensor must not be listed twice or overlap another.
     """
     if isinstance(params, Tensor):
         params, param_grads, momentum_buffers = [params], [param_grads], [momentum_buffers]

@@ -465,17 +465,18 @@ GSB_API int gsb_adam_multi(int n_groups, const GsbAdamGroup *groups, const bool 
  *   `coefficients` (host, [steps, 3]): A = X X^T, X <- a X + (b A + c A A) X
  * (X transposed where rows > cols). Coefficients whose polynomials a s + b s^3 + c s^5 take
  * a singular value in [0, 1] above 16 are refused. Matrices are multiplied with
- * 22 significand bits; bfloat16 ones with a side above 128 with 11.
+ * 22 significand bits; bfloat16 ones with a side above 128 with 11, unless a state is kept.
  * gsb_orthogonalize_bwd: v_x = the gradient of x for the gradient v_y of y. With a
  * `kept` state of gsb_orthogonalize_kept_bytes (0: there is none for this shape, or it would be
  * above 1 GiB with the scratch) that the forward call wrote, the backward call, of the
  * same arguments, need not take the steps again; both may have NULL instead.
- * gsb_muon: for the listed tensors of one type, each a batch of matrices: m <- m + (1 - momentum)(grad - m); u = grad + momentum (m - grad) (nesterov)
- * or m; param <- decay * param - lr * orthogonalized(u). momentum_buffer has
+ * gsb_muon: for the listed tensors of one type, each a batch of matrices:
+ * m <- m + (1 - momentum)(grad - m); u = grad + momentum (m - grad) (nesterov) or m; param <- decay * param - lr * orthogonalized(u). momentum_buffer has
  * the type of param or float32 (state_dtype). valid (optional): a row of a tensor's leading
  * dimension (`inner` matrices) whose entry is false keeps its values. Tensors must not overlap.
  * Scratch: gsb_orthogonalize_scratch_bytes of the whole batch (kept = 1: for a call with a
- * kept state), gsb_muon_scratch_bytes of the list; 0 where none is needed. Calls that may run at the same time need scratch of their own. */
+ * kept state), gsb_muon_scratch_bytes of the list; 0 where none is needed. Calls that
+ * may run at the same time need scratch of their own. */
 GSB_API size_t gsb_orthogonalize_kept_bytes(long long batch, int rows, int cols, int steps);
 GSB_API size_t gsb_orthogonalize_scratch_bytes(long long batch, int rows, int cols, int dtype,
                                        int steps, int backward, int kept);

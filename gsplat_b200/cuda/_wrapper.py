@@ -253,11 +253,12 @@ def muon(
     steps: int = 5,
     coefficients=MUON_COEFFICIENTS,
     eps: float = 1e-7,
+    update_scale=1.0,
 ) -> None:
-    """One Muon step, in place, of one tensor or of a list (``lr`` then one number or a list).
+    """One Muon step, in place, of one tensor or of a list (``lr`` and ``update_scale`` then one number or a list).
 
     For every matrix: m += (1 - momentum) (grad - m); u = grad + momentum (m - grad) with
-    ``nesterov``, else m; param = param (1 - lr weight_decay) - lr ``orthogonalize(u)``. Gradients have
+    ``nesterov``, else m; param = param (1 - lr weight_decay) - lr update_scale ``orthogonalize(u)``. Gradients have
     their parameter's type (float32, bfloat16 or float16), buffers that type or float32. As in :func:`adam`,
     ``valid`` masks the leading dimension, which all params then share (three dimensions or more): masked
     matrices keep their parameter and momentum. Tensors of one shape (or its transpose), and small
@@ -267,8 +268,12 @@ def muon(
         params, param_grads, momentum_buffers = [params], [param_grads], [momentum_buffers]
     params, param_grads, momentum_buffers = list(params), list(param_grads), list(momentum_buffers)
     lrs = [float(v) for v in lr] if isinstance(lr, (list, tuple)) else [float(lr)] * len(params)
-    if not len(params) == len(param_grads) == len(momentum_buffers) == len(lrs):
-        raise ValueError("params, param_grads, momentum_buffers and lr must have the same length")
+    if isinstance(update_scale, (list, tuple)):
+        update_scales = [float(v) for v in update_scale]
+    else:
+        update_scales = [float(update_scale)] * len(params)
+    if not len(params) == len(param_grads) == len(momentum_buffers) == len(lrs) == len(update_scales):
+        raise ValueError("params, param_grads, momentum_buffers, lr and update_scale must have the same length")
     if not 0.0 <= momentum < 1.0:
         raise ValueError(f"momentum must be in [0, 1), got {momentum}")
     if not eps > 0:
@@ -283,7 +288,7 @@ def muon(
     groups = {}
     spans = []
     index = params[0].get_device()
-    for p, g, m, rate in zip(params, param_grads, momentum_buffers, lrs):
+    for p, g, m, rate, scale in zip(params, param_grads, momentum_buffers, lrs, update_scales):
         for name, t in (("param", p), ("param_grad", g), ("momentum_buffer", m)):
             if not (t.is_cuda and t.is_contiguous()):
                 check_cuda(name, t)
@@ -310,7 +315,7 @@ def muon(
         batch = numel // (rows * cols)
         inner = batch // shape[0] if len(shape) > 2 else 1
         groups.setdefault((dtype, state_dtype), []).append(
-            (at_p, at_g, at_m, batch, rows, cols, inner, rate, 1.0 - rate * weight_decay))
+            (at_p, at_g, at_m, batch, rows, cols, inner, rate * scale, 1.0 - rate * weight_decay))
     read_end = write_end = 0
     for start, end, read_only in sorted(spans):
         if start < write_end or (not read_only and start < read_end):

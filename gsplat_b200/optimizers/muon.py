@@ -15,8 +15,9 @@ from ..cuda._wrapper import MUON_COEFFICIENTS, muon
 
 
 class Muon(torch.optim.Optimizer):
-    """``adjust_lr_fn`` scales the learning rate by the matrix's shape: None or ``"original"``:
-    sqrt(max(1, M / N)); ``"match_rms_adamw"``: 0.2 sqrt(max(M, N)), the root mean square of an Adam step.
+    """``adjust_lr_fn`` scales the update by the matrix's shape: None or ``"original"``:
+    sqrt(max(1, M / N)); ``"match_rms_adamw"``: 0.2 sqrt(max(M, N)), the root mean square of an Adam step. The weight
+    decay goes by the learning rate alone: param (1 - lr weight_decay).
     ``momentum_dtype``: the type of the momentum buffers (None: the parameter's; or torch.float32)."""
 
     def __init__(self, params, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True,
@@ -39,7 +40,7 @@ class Muon(torch.optim.Optimizer):
         if visibility is not None:
             visibility = visibility.contiguous()
         for group in self.param_groups:
-            params, grads, buffers, lrs = [], [], [], []
+            params, grads, buffers, scales = [], [], [], []
             for p in group["params"]:
                 if p.grad is None:
                     continue
@@ -53,9 +54,9 @@ class Muon(torch.optim.Optimizer):
                 params.append(p)
                 grads.append(grad.contiguous())
                 buffers.append(state["momentum_buffer"])
-                lrs.append(group["lr"] * _shape_factor(group["adjust_lr_fn"], *p.shape[-2:]))
-            muon(params, grads, buffers, visibility, lrs, group["momentum"], group["weight_decay"], group["nesterov"],
-                 group["ns_steps"], group["ns_coefficients"], group["eps"])
+                scales.append(_shape_factor(group["adjust_lr_fn"], *p.shape[-2:]))
+            muon(params, grads, buffers, visibility, group["lr"], group["momentum"], group["weight_decay"], group["nesterov"],
+                 group["ns_steps"], group["ns_coefficients"], group["eps"], scales)
 
 
 def _shape_factor(rule, rows: int, cols: int) -> float:

@@ -496,8 +496,8 @@ typedef struct GsbMuonTensor {
     int rows;
     int cols;
     int inner;       /* matrices of one row of the leading dimension */
-    float lr;
-    float decay;     /* 1 - lr * weight_decay */
+    float lr;        /* of the update, with the factor of the matrix's shape where there is one */
+    float decay;     /* 1 - (learning rate) * weight_decay; without that factor */
 } GsbMuonTensor;
 GSB_API size_t gsb_muon_scratch_bytes(int n_tensors, const GsbMuonTensor *tensors, int dtype, int steps);
 GSB_API int gsb_muon(int n_tensors, const GsbMuonTensor *tensors, int dtype, int state_dtype,

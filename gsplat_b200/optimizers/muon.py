@@ -35,6 +35,22 @@ class Muon(torch.optim.Optimizer):
                 if p.dim() < 2:
                     raise ValueError(f"Muon takes matrices [..., M, N], got a parameter {tuple(p.shape)}")
 
+    def load_state_dict(self, state_dict):
+        """As torch's, which casts all state to the parameter's type; the momentum buffers are taken from the saved state
+        again, in the group's ``momentum_dtype``. A state of ``torch.optim.Muon`` has none: this optimizer's stays."""
+        loaded = []
+        hook = self.register_load_state_dict_pre_hook(lambda _, state: loaded.append(state))  # sees what earlier hooks return
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            hook.remove()
+        for group, saved in zip(self.param_groups, loaded[-1]["param_groups"]):
+            group.setdefault("momentum_dtype", self.defaults["momentum_dtype"])
+            for p, key in zip(group["params"], saved["params"]):
+                buffer = loaded[-1]["state"].get(key, {}).get("momentum_buffer")
+                if buffer is not None:
+                    self.state[p]["momentum_buffer"] = buffer.to(p.device, group["momentum_dtype"] or p.dtype).contiguous()
+
     @torch.no_grad()
     def step(self, visibility=None):
         if visibility is not None:

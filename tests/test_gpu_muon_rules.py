@@ -1,5 +1,6 @@
 """The Muon class and muon()'s arguments on the GPU against 64-bit implementations."""
 
+import copy
 import math
 
 import pytest
@@ -46,3 +47,24 @@ def test_update_scale_of_one_tensor_and_of_a_list():
     assert torch.equal(one, tp[1])
     with pytest.raises(ValueError, match="same length"):
         gs().muon(tp, [g.cuda() for g in grads], [m.cuda() for m in ms], None, 0.1, 0.9, update_scale=[1.0])
+
+
+def test_visibility_and_checkpoint():
+    """Per-splat SH bands under a visibility mask, with the momentum in 32 bits, and a checkpoint of it."""
+    sh = torch.nn.Parameter(data((30, 15, 3), torch.bfloat16, 60, 1.0).cuda())
+    opt = gs().Muon([sh], lr=0.1, momentum_dtype=torch.float32)
+    before = sh.detach().clone()
+    sh.grad = data((30, 15, 3), torch.bfloat16, 61).cuda()
+    vis = torch.arange(30, device="cuda") % 2 == 0
+    opt.step(vis)
+    assert torch.equal(sh.detach()[~vis], before[~vis]) and (sh.detach()[vis] != before[vis]).flatten(1).any(1).all()
+    buffer = opt.state[sh]["momentum_buffer"]
+    assert buffer.dtype == torch.float32 and (buffer[~vis] == 0).all()
+    q = torch.nn.Parameter(sh.detach().clone())
+    other = gs().Muon([q], lr=0.5, momentum_dtype=torch.float32)
+    other.load_state_dict(copy.deepcopy(opt.state_dict()))
+    assert torch.equal(other.state[q]["momentum_buffer"], buffer)
+    q.grad = sh.grad.clone()
+    opt.step(vis)
+    other.step(vis)
+    assert torch.equal(q.detach(), sh.detach()) and torch.equal(other.state[q]["momentum_buffer"], buffer)

@@ -50,3 +50,48 @@ def test_update_is_scaled_by_the_shape(plain, shape, rule):
     gsplat_b200.Muon([ours], **args).step()
     torch.optim.Muon([theirs], **args).step()
     assert N.distance(ours.detach(), theirs.detach()) < 0.2
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("momentum_dtype", [None, torch.float32])
+def test_checkpoint_keeps_the_momentum(plain, dtype, momentum_dtype):
+    """A saved and loaded state has the buffers' type and every bit of them, also through a file's copy."""
+    import copy
+
+    gen = torch.Generator().manual_seed(2)
+    args = dict(lr=0.01, momentum_dtype=momentum_dtype)
+    ps = [torch.nn.Parameter(torch.randn(6, 5, generator=gen).to(dtype)) for _ in range(3)]
+    opt = gsplat_b200.Muon([dict(params=ps[:2]), dict(params=ps[2:], lr=0.5)], **args)
+    for p in ps[:2]:
+        p.grad = torch.randn(6, 5, generator=gen).to(dtype)
+    opt.step()
+    want = [opt.state[p]["momentum_buffer"] for p in ps[:2]]
+    assert all(w.dtype == (momentum_dtype or dtype) for w in want)
+    qs = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    other = gsplat_b200.Muon([dict(params=qs[:2]), dict(params=qs[2:])], **args)
+    other.register_load_state_dict_pre_hook(lambda _, state: copy.deepcopy(state))  # a user's hook may replace the state
+    other.load_state_dict(copy.deepcopy(opt.state_dict()))
+    for q, w in zip(qs, want):
+        got = other.state[q]["momentum_buffer"]
+        assert got.dtype == w.dtype and torch.equal(got, w) and got.data_ptr() != w.data_ptr()
+    assert "momentum_buffer" not in other.state[qs[2]] and other.param_groups[1]["lr"] == 0.5
+    for p, q in zip(ps, qs):
+        p.grad = torch.randn(6, 5, generator=gen).to(dtype)
+        q.grad = p.grad.clone()
+    opt.step(), other.step()
+    assert all(torch.equal(p, q) for p, q in zip(ps, qs))
+
+
+def test_state_of_torch_muon_is_taken(plain):
+    ps = [torch.nn.Parameter(torch.ones(4, 6, dtype=torch.bfloat16)) for _ in range(2)]
+    theirs = torch.optim.Muon(ps, lr=0.3)
+    ps[0].grad = torch.ones(4, 6, dtype=torch.bfloat16)
+    theirs.step()
+    opt = gsplat_b200.Muon([torch.nn.Parameter(p.detach().clone()) for p in ps], momentum_dtype=torch.float32)
+    opt.load_state_dict(theirs.state_dict())
+    a, b = opt.param_groups[0]["params"]
+    assert opt.param_groups[0]["lr"] == 0.3 and opt.state[a]["momentum_buffer"].dtype == torch.float32
+    assert torch.equal(opt.state[a]["momentum_buffer"], theirs.state[ps[0]]["momentum_buffer"].float())
+    b.grad = torch.ones(4, 6, dtype=torch.bfloat16)
+    opt.step()
+    assert opt.state[b]["momentum_buffer"].dtype == torch.float32

@@ -170,7 +170,7 @@ def orthogonalize(
     bits, bfloat16 ones with a side above 128 with 11 where no gradient is wanted; the result has x's
     shape and type. A matrix with a NaN or an infinity becomes NaN, and no other of the batch.
 
-    Differentiable once. The steps' state is kept for the backward pass, about
+    Differentiable once, in reverse mode. The steps' state is kept for the backward pass, about
     4 steps (x.numel() + 2 B M M) bytes for B matrices of shorter side M (none where it is at most 4 and the
     longer at most 128); where that would be above 1 GiB the backward pass takes the steps again.
     """
@@ -179,6 +179,8 @@ def orthogonalize(
     _ortho_dtype("x", x)
     if not eps > 0:
         raise ValueError(f"eps must be positive, got {eps}")
+    if torch.autograd.forward_ad.unpack_dual(x).tangent is not None:
+        raise NotImplementedError("orthogonalize has no forward-mode derivative")
     x = x.contiguous()
     coefficients = _ortho_coefficients(coefficients, steps)
     if x.requires_grad and torch.is_grad_enabled():

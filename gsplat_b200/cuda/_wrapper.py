@@ -126,7 +126,10 @@ def _ortho_coefficients(coefficients, steps: int):
     """``coefficients`` (one (a, b, c) for every step, or a list of them) as a C array of steps triples."""
     if not 1 <= steps <= 32:
         raise ValueError(f"steps must be 1 to 32, got {steps}")
-    triples = tuple(tuple(v) if isinstance(v, (list, tuple)) else v for v in coefficients)
+    if hasattr(coefficients, "tolist"):
+        coefficients = coefficients.tolist()
+    # numbers before the cache sees them: a tensor is hashed by its identity, and may change
+    triples = tuple(tuple(map(float, v)) if isinstance(v, (list, tuple)) else float(v) for v in coefficients)
     return _ortho_coefficient_array(triples, steps)
 
 
@@ -136,7 +139,7 @@ def _ortho_coefficient_array(triples, steps: int):
         triples = [triples] * steps
     if len(triples) != steps or any(not isinstance(t, tuple) or len(t) != 3 for t in triples):
         raise ValueError(f"coefficients must be (a, b, c) or a list of steps = {steps} such triples")
-    flat = [float(v) for t in triples for v in t]
+    flat = [v for t in triples for v in t]
     return (ctypes.c_float * len(flat))(*flat)
 
 

@@ -31,3 +31,18 @@ def test_forward_mode_is_refused(launches):
     with pytest.raises(NotImplementedError):
         torch.func.jvp(gsplat_b200.orthogonalize, (x,), (torch.ones_like(x),))
     assert len(launches) == 1
+
+
+@pytest.mark.parametrize("nested", [False, True])
+def test_coefficients_are_read_at_each_call(launches, nested):
+    """Of tensors that change in place (an annealed schedule), as of new numbers."""
+    triple = [torch.tensor(1.5), torch.tensor(-0.5), torch.tensor(0.0)]
+    coefficients = [triple, (3.0, -2.0, 0.0)] if nested else triple
+    rest = [3.0, -2.0, 0.0] if nested else []
+    x = torch.randn(3, 3)
+    gsplat_b200.orthogonalize(x, len(rest) // 3 + 1, coefficients)
+    triple[0].fill_(2.0)
+    gsplat_b200.orthogonalize(x, len(rest) // 3 + 1, coefficients)
+    gsplat_b200.orthogonalize(x, 1, torch.tensor([1.25, -0.25, 0.0]))
+    gsplat_b200.orthogonalize(x, 2, torch.tensor([[1.25, -0.25, 0.0], [1.0, 0.0, 0.5]]))
+    assert launches == [[1.5, -0.5, 0.0] + rest, [2.0, -0.5, 0.0] + rest, [1.25, -0.25, 0.0], [1.25, -0.25, 0.0, 1.0, 0.0, 0.5]]

@@ -129,7 +129,8 @@ def _ortho_coefficients(coefficients, steps: int):
     if hasattr(coefficients, "tolist"):
         coefficients = coefficients.tolist()
     # numbers before the cache sees them: a tensor is hashed by its identity, and may change
-    triples = tuple(tuple(map(float, v)) if isinstance(v, (list, tuple)) else float(v) for v in coefficients)
+    triples = tuple([v if type(v) is float else tuple(map(float, v)) if isinstance(v, (list, tuple)) else float(v)
+                     for v in coefficients])
     return _ortho_coefficient_array(triples, steps)
 
 
@@ -151,6 +152,11 @@ def _ortho_scratch_bytes(batch: int, rows: int, cols: int, dtype: int, steps: in
 @functools.lru_cache(maxsize=256)
 def _ortho_kept_bytes(batch: int, rows: int, cols: int, steps: int) -> int:
     return lib().gsb_orthogonalize_kept_bytes(batch, rows, cols, steps)
+
+
+def _forward_ad_level() -> int:
+    """The entered level of forward-mode differentiation, below 0 if there is none (then a look at x is saved)."""
+    return getattr(torch.autograd.forward_ad, "_current_level", 0)
 
 
 def _bytes(size: int, device) -> Optional[Tensor]:
@@ -182,7 +188,7 @@ def orthogonalize(
     _ortho_dtype("x", x)
     if not eps > 0:
         raise ValueError(f"eps must be positive, got {eps}")
-    if torch.autograd.forward_ad.unpack_dual(x).tangent is not None:
+    if _forward_ad_level() >= 0 and torch.autograd.forward_ad.unpack_dual(x).tangent is not None:
         raise NotImplementedError("orthogonalize has no forward-mode derivative")
     x = x.contiguous()
     coefficients = _ortho_coefficients(coefficients, steps)

@@ -79,6 +79,20 @@ __device__ __forceinline__ float muon_param(float p, float o, float lr, float de
     return fmaf(-lr, o, p * decay);
 }
 
+// How a matrix is divided by its norm, a sum in 64 bits: x * pre / div. Where the norm nears the ends of a float's range
+// or passes them (FLT_MAX in several entries is a norm above it), a power of two brings it back.
+struct Divisor {
+    float pre, div;
+    bool small; // the norm is below eps, which takes its place
+};
+__device__ __forceinline__ Divisor divisor_of(double norm, float eps) {
+    Divisor d;
+    d.small = (float)norm < eps;
+    d.pre = d.small ? 1.f : norm > 0x1p120 ? 0x1p-40f : norm < 0x1p-100 ? 0x1p60f : 1.f;
+    d.div = d.small ? eps : (float)(norm * (double)d.pre);
+    return d;
+}
+
 // The tensors of one Muon step that share a shape: [batch_t, rows, cols] each.
 // Matrix b of the launch belongs to the tensor t with first[t] <= b < first[t + 1].
 struct MuonTable {
@@ -160,7 +174,8 @@ int ortho_is_clustered(int rows, int cols); // the blocks of a matrix's cluster,
 // `step` halves (2 bytes) behind.
 struct ClusterKept {
     OrthoPlanes x, a, b;
-    float *da, *db, *norms;
+    float *da, *db;
+    double *norms;
     long long step;
 };
 int ortho_cluster_fwd(long long batch, int rows, int cols, int dtype, const void *x, void *y, const OrthoCoefficients &co,

@@ -290,9 +290,10 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
         s = 0.0;
         for (int r = 0; r < sh.blocks; ++r) s += remote_load_f64(remote(smem_u32(&block_total), r));
     }
-    const float norm = (float)sqrt(s), div = norm < eps ? eps : norm;
+    const double norm = sqrt(s);
+    const Divisor d = divisor_of(norm, eps);
     auto put = [&](int i, int j, float v) {
-        v = v / div * sh.x_scale;
+        v = v * d.pre / d.div * sh.x_scale;
         const __half h = __float2half_rn(v);
         const uint32_t p = plane_byte(sh.m16, i, j);
         *reinterpret_cast<__half *>(x_hi + p) = h;
@@ -332,7 +333,7 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
     }
 
     const bool keep = !MUON && kept.x.hi != nullptr;
-    if (keep && tid == 0 && rank == 0) kept.norms[b] = norm < eps ? -1.f : norm;
+    if (keep && tid == 0 && rank == 0) kept.norms[b] = d.small ? -1.0 : norm;
     // rows [r0, r1) and columns up to `used` of a plane pair to memory, 16 bytes at a time
     auto dump = [&](const char *hi, const char *lo, const OrthoPlanes &to, int step, int r0, int r1, int used, int col0) {
         const int eights = (used + 7) / 8;

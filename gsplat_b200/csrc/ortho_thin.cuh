@@ -101,14 +101,14 @@ template <int S> __device__ __forceinline__ void apply(float x[kThinRows][S], co
     }
 }
 
-// The Frobenius norm over the group, summed in 64 bits (any finite input).
-template <int S> __device__ __forceinline__ float frobenius(const float x[kThinRows][S], int group) {
+// The Frobenius norm over the group, in 64 bits (any finite input).
+template <int S> __device__ __forceinline__ double frobenius(const float x[kThinRows][S], int group) {
     double s = 0.0;
 #pragma unroll
     for (int r = 0; r < kThinRows; ++r)
 #pragma unroll
         for (int j = 0; j < S; ++j) s = fma((double)x[r][j], (double)x[r][j], s);
-    return (float)sqrt(group_sum(s, group));
+    return sqrt(group_sum(s, group));
 }
 
 struct ThinShape {
@@ -138,12 +138,11 @@ __global__ void __launch_bounds__(kThinThreads)
             const int l = r * sh.group + lane;
             x[r][j] = live && l < sh.L ? to_f32(x_in[base + l * sh.row_step + j * sh.col_step]) : 0.f;
         }
-    const float norm = frobenius<S>(x, sh.group);
-    const float d = norm < eps ? eps : norm;
+    const Divisor d = divisor_of(frobenius<S>(x, sh.group), eps);
 #pragma unroll
     for (int r = 0; r < kThinRows; ++r)
 #pragma unroll
-        for (int j = 0; j < S; ++j) x[r][j] = x[r][j] / d;
+        for (int j = 0; j < S; ++j) x[r][j] = x[r][j] * d.pre / d.div;
     thin_iterate<S>(x, co, sh.group);
 #pragma unroll
     for (int r = 0; r < kThinRows; ++r)
@@ -175,12 +174,11 @@ __global__ void __launch_bounds__(kThinThreads)
             x[r][j] = in ? to_f32(x_in[at]) : 0.f;
             g[r][j] = in ? to_f32(v_y[at]) : 0.f;
         }
-    const float norm = frobenius<S>(x, sh.group);
-    const float d = norm < eps ? eps : norm;
+    const Divisor d = divisor_of(frobenius<S>(x, sh.group), eps);
 #pragma unroll
     for (int r = 0; r < kThinRows; ++r)
 #pragma unroll
-        for (int j = 0; j < S; ++j) x[r][j] = x[r][j] / d;
+        for (int j = 0; j < S; ++j) x[r][j] = x[r][j] * d.pre / d.div;
     for (int k = 0; k < co.steps; ++k) {
 #pragma unroll
         for (int r = 0; r < kThinRows; ++r)
@@ -223,14 +221,14 @@ __global__ void __launch_bounds__(kThinThreads)
 #pragma unroll
         for (int j = 0; j < S; ++j) dot = fmaf(g[r][j], x[r][j], dot);
     dot = group_sum(dot, sh.group);
-    if (norm < eps) dot = 0.f;
+    if (d.small) dot = 0.f;
 #pragma unroll
     for (int r = 0; r < kThinRows; ++r)
 #pragma unroll
         for (int j = 0; j < S; ++j) {
             const int l = r * sh.group + lane;
             if (live && l < sh.L)
-                v_x[base + l * sh.row_step + j * sh.col_step] = from_f32<T>(fmaf(-x[r][j], dot, g[r][j]) / d);
+                v_x[base + l * sh.row_step + j * sh.col_step] = from_f32<T>(fmaf(-x[r][j], dot, g[r][j]) / d.div * d.pre);
         }
 }
 
@@ -264,12 +262,11 @@ __global__ void __launch_bounds__(kThinThreads)
                 x[r][j] = muon_update(g, m, tab.mu, tab.nesterov);
             }
         }
-    const float norm = frobenius<S>(x, sh.group);
-    const float d = norm < eps ? eps : norm;
+    const Divisor d = divisor_of(frobenius<S>(x, sh.group), eps);
 #pragma unroll
     for (int r = 0; r < kThinRows; ++r)
 #pragma unroll
-        for (int j = 0; j < S; ++j) x[r][j] = x[r][j] / d;
+        for (int j = 0; j < S; ++j) x[r][j] = x[r][j] * d.pre / d.div;
     thin_iterate<S>(x, co, sh.group);
     const float lr = tab.lr[t], decay = tab.decay[t];
 #pragma unroll

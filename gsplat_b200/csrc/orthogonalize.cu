@@ -152,13 +152,13 @@ __device__ __forceinline__ float4 planes_get4(const OrthoPlanes &p, size_t at) {
 }
 
 // planes <- factor * source, in the orientation whose rows are the shorter side.
-// eps > 0: factor = scale / max(norm, eps), and norm_out gets the norm, negated
+// eps > 0: factor = scale / max(norm, eps), and norm_out gets the norm, or -1
 // below eps. eps = 0: factor = the power of two that brings the norm to (scale / 2, scale], and
 // norm_out gets the factor. A block takes 64 x 64 values, a thread four rows of four.
 template <typename T, typename M, bool MUON>
 __global__ void __launch_bounds__(kNormThreads)
     ortho_split_kernel(const void *x, const __grid_constant__ MuonTable tab, int rows, int cols, int transposed,
-                       const double *partial, int chunks, float scale, float eps, float *norm_out, OrthoPlanes out,
+                       const double *partial, int chunks, float scale, float eps, double *norm_out, OrthoPlanes out,
                        int tiles_r, int tiles_c) {
     __shared__ float tile[kSplitTile][kSplitTile + 1];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -195,17 +195,20 @@ __global__ void __launch_bounds__(kNormThreads)
             if (col + 3 < cols) g[u].w = src.get1(e + 3, m[u].w);
         }
     }
-    const float norm = (float)sqrt(sum_partials(partial, b, chunks));
-    float div, mul;
+    const double norm = sqrt(sum_partials(partial, b, chunks));
+    float pre, div, mul;
     if (eps > 0.f) {
-        div = norm < eps ? eps : norm;
+        const Divisor d = divisor_of(norm, eps);
+        pre = d.pre;
+        div = d.div;
         mul = scale;
-        if (ti == 0 && threadIdx.x == 0) norm_out[b] = norm < eps ? -1.f : norm;
-    } else {
-        const int e = norm > 0.f && norm < INFINITY ? min(max(ilogb(norm) + 1, -100), 126) : 0;
+        if (ti == 0 && threadIdx.x == 0) norm_out[b] = d.small ? -1.0 : norm;
+    } else { // in two factors: their product may lie outside of a float's range
+        const int e = norm > 0.0 && norm < (double)INFINITY ? ilogb(norm) + 1 : 0;
+        pre = (float)ldexp(1.0, -(e / 2));
         div = 1.f;
-        mul = scale * exp2f((float)-e);
-        if (ti == 0 && threadIdx.x == 0) norm_out[b] = mul;
+        mul = (float)ldexp((double)scale, e / 2 - e);
+        if (ti == 0 && threadIdx.x == 0) norm_out[b] = ldexp((double)scale, -e);
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -223,7 +226,7 @@ __global__ void __launch_bounds__(kNormThreads)
                 if (col + 3 < cols) to[3] = from_f32<M>(m[u].w);
             }
         }
-        w = make_float4(w.x / div * mul, w.y / div * mul, w.z / div * mul, w.w / div * mul);
+        w = make_float4(w.x * pre / div * mul, w.y * pre / div * mul, w.z * pre / div * mul, w.w * pre / div * mul);
         if (!turned) {
             planes_put4(out, (size_t)b * out.stride + (size_t)row * out.ld + col, w);
         } else {
@@ -268,14 +271,14 @@ __global__ void __launch_bounds__(kNormThreads)
 // G's planes brought back to a norm in (scale / 2, scale] by a power of two, which its
 // factor takes too. <G, G> in `partial`.
 __global__ void __launch_bounds__(kNormThreads)
-    ortho_rescale_kernel(OrthoPlanes g, int m, int n, int chunks, const double *partial, float scale, const float *factor_in,
-                         float fallen, float *factor_out) {
+    ortho_rescale_kernel(OrthoPlanes g, int m, int n, int chunks, const double *partial, float scale, const double *factor_in,
+                         float fallen, double *factor_out) {
     const long long b = blockIdx.x / chunks;
     const int chunk = (int)(blockIdx.x % chunks);
     const float norm = (float)sqrt(sum_partials(partial, b, chunks));
     const int e = norm > 0.f && norm < INFINITY ? min(max(ilogb(norm) + 1, -100), 126) : ilogb(scale);
     const float mul = scale * exp2f((float)-e);
-    if (chunk == 0 && threadIdx.x == 0) factor_out[b] = factor_in[b] * fallen * mul;
+    if (chunk == 0 && threadIdx.x == 0) factor_out[b] = factor_in[b] * (double)fallen * (double)mul;
     for (int i = chunk; i < m; i += chunks)
         for (int j = threadIdx.x; j < n; j += kNormThreads) {
             const size_t at = (size_t)b * g.stride + (size_t)i * g.ld + j;
@@ -290,7 +293,7 @@ __global__ void __launch_bounds__(kNormThreads)
 template <typename T>
 __global__ void __launch_bounds__(kNormThreads)
     ortho_grad_out_kernel(OrthoPlanes g, OrthoPlanes x, int rows, int cols, int transposed, const double *partial,
-                          int chunks, const float *norms, const float *g_factor, float g_scale, float x_scale, float eps,
+                          int chunks, const double *norms, const double *g_factor, float g_scale, float x_scale, float eps,
                           T *v_x, int tiles_r, int tiles_c, const int *error) {
     __shared__ float tile[kSplitTile][kSplitTile + 1];
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -310,13 +313,19 @@ __global__ void __launch_bounds__(kNormThreads)
         }
     }
     const double dot = sum_partials(partial, b, chunks);
-    const float norm = norms[b];
-    const bool small = norm < 0.f;
+    const double norm = norms[b], factor = g_factor[b];
+    const bool small = norm < 0.0;
     const float along = small ? 0.f : (float)(dot / ((double)x_scale * x_scale));
-    const float div = small ? eps : norm;
-    const float f = g_factor[b]; // f and g_scale are powers of two; one after the other keeps both in range
+    const double by = small ? (double)eps : norm;
+    // in 32 bits, one after the other (the factor and g_scale are powers of two), where that keeps all in range; else in 64
+    const bool middle = by > 0x1p-100 && by < 0x1p120 && factor >= 0x1p-112 && factor <= 0x1p114;
+    const float div = (float)by, f = (float)factor;
+    const double all = 1.0 / ((double)g_scale * factor * by);
     const bool poisoned = *error != 0;
-    auto value = [&](float gw, float xw) { return poisoned ? NAN : fmaf(-xw, along, gw) / g_scale / f / div; };
+    auto value = [&](float gw, float xw) {
+        const float v = fmaf(-xw, along, gw);
+        return poisoned ? NAN : middle ? v / g_scale / f / div : (float)((double)v * all);
+    };
     T *out = v_x + (size_t)b * rows * cols;
     const bool quads = cols % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (4 * sizeof(T)) == 0;
     auto put = [&](int row, int col, float4 v) {
@@ -433,9 +442,9 @@ static OrthoPlan ortho_plan(int rows, int cols, int dtype, const OrthoCoefficien
     p.px = (long long)p.m * p.ldx;
     p.pa = (long long)p.m * p.lda;
     const size_t halves = 2 * sizeof(__half);
-    p.kept_matrix = co.steps * (halves * (p.px + 2 * p.pa) + 2 * sizeof(float) * p.m) + sizeof(float);
+    p.kept_matrix = co.steps * (halves * (p.px + 2 * p.pa) + 2 * sizeof(float) * p.m) + sizeof(double);
     p.kept_fixed = 256 * (size_t)(8 * co.steps + 2);
-    size_t bytes = sizeof(double) * (size_t)p.chunks + 3 * sizeof(float);
+    size_t bytes = sizeof(double) * (size_t)(p.chunks + 2); // sums, and norms or two factors
     if (backward)
         bytes += 2 * halves * (p.px + p.pa); // G twice, S, T
     else
@@ -481,7 +490,7 @@ struct Carver {
 struct OrthoBuffers {
     OrthoPlanes x[kOrthoMaxSteps], a[kOrthoMaxSteps], b[kOrthoMaxSteps];
     float *da[kOrthoMaxSteps], *db[kOrthoMaxSteps];
-    float *norms;
+    double *norms;
 
     OrthoBuffers(Carver &ws, const OrthoPlan &p, long long nb) {
         for (int k = 0; k < p.steps; ++k) {
@@ -491,7 +500,7 @@ struct OrthoBuffers {
             da[k] = ws.take<float>((size_t)nb * p.m);
             db[k] = ws.take<float>((size_t)nb * p.m);
         }
-        norms = ws.take<float>(nb);
+        norms = ws.take<double>(nb);
     }
 };
 
@@ -511,7 +520,7 @@ template <typename F> static int with_source(int dtype, const MuonTable &tab, F 
 }
 
 static int run_split(const OrthoPlan &p, long long nb, const void *x, int dtype, const MuonTable &tab, float scale, float eps,
-                     float *norm_out, double *partial, const OrthoPlanes &out, int *error, cudaStream_t stream) {
+                     double *norm_out, double *partial, const OrthoPlanes &out, int *error, cudaStream_t stream) {
     return with_source(dtype, tab, [&](auto tv, auto mv, auto muon) {
         using T = decltype(tv);
         using M = decltype(mv);
@@ -600,7 +609,7 @@ static int ortho_tiled_fwd(const OrthoPlan &p, const OrthoCoefficients &co, long
     const OrthoPlanes a = ws.planes(nb, p.pa, p.lda), b = ws.planes(nb, p.pa, p.lda);
     float *da = ws.take<float>((size_t)nb * p.m), *db = ws.take<float>((size_t)nb * p.m);
     double *partial = ws.take<double>((size_t)nb * p.chunks);
-    float *norms = ws.take<float>(nb);
+    double *norms = ws.take<double>(nb);
     int *error = ws.take<int>(1);
     const MuonTable *t = tab.n > 0 ? &tab : nullptr;
     if (int e = run_split(p, nb, src, dtype, tab, (float)p.s.x, eps, norms, partial, x[0], error, stream)) return e;
@@ -662,8 +671,8 @@ static int ortho_tiled_bwd(const OrthoPlan &p, const OrthoCoefficients &co, long
     OrthoPlanes gr[2] = {ws.planes(nb, p.px, p.ldx), ws.planes(nb, p.px, p.ldx)};
     const OrthoPlanes s = ws.planes(nb, p.pa, p.lda), t = ws.planes(nb, p.pa, p.lda);
     double *partial = ws.take<double>((size_t)nb * p.chunks);
-    float *factor[2] = {ws.take<float>(nb), ws.take<float>(nb)};
-    float *const norms = w.norms;
+    double *factor[2] = {ws.take<double>(nb), ws.take<double>(nb)};
+    double *const norms = w.norms;
     int *error = ws.take<int>(1);
     const MuonTable none = {};
     const double shrink = std::exp2(std::ceil(std::log2(p.s.slope)));
@@ -721,8 +730,8 @@ static int ortho_tiled_bwd(const OrthoPlan &p, const OrthoCoefficients &co, long
     return with_source(dtype, none, [&](auto tv, auto, auto) {
         using T = decltype(tv);
         return launch_after(ortho_grad_out_kernel<T>, (unsigned)(nb * tr * tc), kNormThreads, 0, stream, "ortho_grad_out_kernel", gr[0],
-                            w.x[0], p.rows, p.cols, p.transposed, (const double *)partial, p.chunks, (const float *)norms,
-                            (const float *)factor[0], (float)grown, (float)p.s.x, eps, static_cast<T *>(v_x), tr, tc, (const int *)error);
+                            w.x[0], p.rows, p.cols, p.transposed, (const double *)partial, p.chunks, (const double *)norms,
+                            (const double *)factor[0], (float)grown, (float)p.s.x, eps, static_cast<T *>(v_x), tr, tc, (const int *)error);
     });
 }
 

@@ -795,6 +795,14 @@ extern "C" size_t gsb_orthogonalize_scratch_bytes(long long batch, int rows, int
     return plan_bytes(ortho_plan(rows, cols, dtype, co, backward != 0, kept != 0), batch);
 }
 
+static int check_kept(long long batch, int rows, int cols, int steps, const void *kept, size_t kept_bytes) {
+    if (kept == nullptr) return kOk;
+    const size_t needed = gsb_orthogonalize_kept_bytes(batch, rows, cols, steps);
+    if (needed == 0) return set_error(kErrInvalidArgument, "orthogonalize: no state is kept of %lld x [%d, %d]", batch, rows, cols);
+    if (kept_bytes < needed) return set_error(kErrInvalidArgument, "orthogonalize: the kept state needs %zu bytes", needed);
+    return kOk;
+}
+
 static const char *at_matrix(const void *p, long long b, int rows, int cols, int dtype) {
     return static_cast<const char *>(p) + (size_t)b * rows * cols * (dtype == kOrthoF32 ? 4 : 2);
 }
@@ -805,8 +813,7 @@ extern "C" int gsb_orthogonalize_fwd(long long batch, int rows, int cols, int dt
     OrthoCoefficients co = {};
     if (int e = check_common("orthogonalize", batch, rows, cols, dtype, steps, coefficients, eps, &co)) return e;
     if (batch == 0 || rows == 0 || cols == 0) return kOk;
-    if (kept && (kept_bytes == 0 || kept_bytes < gsb_orthogonalize_kept_bytes(batch, rows, cols, steps)))
-        return set_error(kErrInvalidArgument, "orthogonalize: the kept state needs %zu bytes", gsb_orthogonalize_kept_bytes(batch, rows, cols, steps));
+    if (int e = check_kept(batch, rows, cols, steps, kept, kept_bytes)) return e;
     if (ortho_is_thin(rows, cols)) return ortho_thin_fwd(batch, rows, cols, dtype, x, y, co, eps, stream);
     const OrthoPlan p = make_plan(rows, cols, dtype, co, false, kept != nullptr);
     Carver own{static_cast<char *>(kept)};
@@ -845,8 +852,7 @@ extern "C" int gsb_orthogonalize_bwd(long long batch, int rows, int cols, int dt
     OrthoCoefficients co = {};
     if (int e = check_common("orthogonalize", batch, rows, cols, dtype, steps, coefficients, eps, &co)) return e;
     if (batch == 0 || rows == 0 || cols == 0) return kOk;
-    if (kept && (kept_bytes == 0 || kept_bytes < gsb_orthogonalize_kept_bytes(batch, rows, cols, steps)))
-        return set_error(kErrInvalidArgument, "orthogonalize: the kept state needs %zu bytes", gsb_orthogonalize_kept_bytes(batch, rows, cols, steps));
+    if (int e = check_kept(batch, rows, cols, steps, kept, kept_bytes)) return e;
     if (ortho_is_thin(rows, cols)) return ortho_thin_bwd(batch, rows, cols, dtype, x, v_y, v_x, co, eps, stream);
     const OrthoPlan p = make_plan(rows, cols, dtype, co, true, kept != nullptr);
     if (scratch == nullptr || scratch_bytes < plan_bytes(p, batch))

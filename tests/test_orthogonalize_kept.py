@@ -1,0 +1,46 @@
+"""CPU checks of the C entry points' kept state: it is refused before any launch where there is none or it is too short."""
+
+import ctypes
+
+import pytest
+import torch
+
+from tests import _newton_schulz as N
+
+# the calls carry pointers to nothing: only where no GPU could follow them
+pytestmark = pytest.mark.skipif(torch.cuda.is_available(), reason="for machines without a GPU")
+
+
+def lib():
+    from gsplat_b200.cuda import _backend
+
+    return _backend.lib()
+
+
+# with a valid scratch size and pointers that are never followed: only the refusal keeps these calls from a launch
+SOMEWHERE = 1 << 20
+
+
+def both(batch, rows, cols, kept, size):
+    L, c = lib(), (ctypes.c_float * 15)(*(list(N.QUINTIC) * 5))
+    fwd = L.gsb_orthogonalize_fwd(batch, rows, cols, 0, None, None, 5, c, 1e-7, kept, size, SOMEWHERE, 1 << 40, None)
+    message = L.gsb_last_error()
+    bwd = L.gsb_orthogonalize_bwd(batch, rows, cols, 0, None, None, None, 5, c, 1e-7, kept, size, SOMEWHERE, 1 << 40, None)
+    return fwd, bwd, message
+
+
+@pytest.mark.parametrize("batch,rows,cols", [(1, 4096, 4096), (100000, 512, 512), (10, 15, 3)])
+@pytest.mark.parametrize("size", [1, 16, 1 << 33])
+def test_kept_state_where_there_is_none(batch, rows, cols, size):
+    """Above 1 GiB with the scratch, and for thin matrices, none is kept, whatever room the caller offers."""
+    assert lib().gsb_orthogonalize_kept_bytes(batch, rows, cols, 5) == 0
+    fwd, bwd, message = both(batch, rows, cols, SOMEWHERE, size)
+    assert fwd == -1 and bwd == -1 and b"no state is kept" in message
+
+
+@pytest.mark.parametrize("batch,rows,cols", [(1, 300, 300), (8, 64, 64)])
+def test_kept_state_too_short(batch, rows, cols):
+    needed = lib().gsb_orthogonalize_kept_bytes(batch, rows, cols, 5)
+    for size in (0, 1, needed - 1):
+        fwd, bwd, message = both(batch, rows, cols, SOMEWHERE, size)
+        assert fwd == -1 and bwd == -1 and b"needs %d" % needed in message

@@ -408,6 +408,9 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
                 }
             }
         if (sh.blocks > 1) {
+            if (*abort) { // a wait of this block ran out: the others' A will be wrong too
+                for (int r = 0; r < sh.blocks; ++r) remote_store_f32(remote(smem_u32(&abort_flag), r), __int_as_float(1));
+            }
             cluster_sync();
             // add up this block's rows, in the order of the blocks, then give them to all
             const int r0 = (int)rank * sh.per, rows = max(0, min(sh.m16, r0 + sh.per) - r0), pieces = rows * (sh.m16 / 8);
@@ -541,9 +544,11 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const bool poisoned = *abort != 0; // a wait ran out
+    for (int i = 0; poisoned && i < 10000; ++i) __nanosleep(1000); // the products in flight end within this time
     if (warp == 0)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(sh.columns) : "memory");
-    const bool poisoned = *abort != 0; // a wait ran out
+    if (keep && poisoned && tid == 0) kept.norms[b] = NAN; // for the backward pass
     auto get = [&](int i, int j) -> float {
         const int w = j & 15;
         const float v = *reinterpret_cast<const float *>((w < 8 ? x_hi : x_lo) + plane_byte(sh.m16, i, (j & ~15) + ((w >> 2) & 1) * 8) + (w & 3) * 4);

@@ -263,6 +263,29 @@ __device__ __forceinline__ void finish32(const OrthoGemm &g, const MuonTable &ta
     else put_out<__half, EPI == kEpiMuon>(to, v, p, stage, lane, lr, decay, poisoned);
 }
 
+// A wait ran out at tile t of the last product: NaN for the warp's part (from row `row` and column `col` of a tile, `width`
+// columns) of this tile and of those that the block had still to do.
+template <int EPI, int BN, int ROWS>
+__device__ void give_up(const OrthoGemm &g, const MuonTable &tab, long long t, long long tiles, long long stride, int per, int tiles_n,
+                        int row, int col, int width) {
+    const int lane = threadIdx.x % 32;
+    for (; t < tiles; t += stride) {
+        const TileAt at = tile_at<kBM>(t, per, tiles_n, false);
+        const int tensor = tab.n > 0 ? muon_tensor_of(tab, at.b) : 0;
+        if (tab.n > 0 && !muon_visible(tab, tensor, at.b)) continue;
+        for (int c = 0; c < width; c += 32) {
+            const OutAt to = out_at<EPI>(g, tab, tensor, at.b, at.i * ROWS + row, at.j * BN + col + c, lane);
+#pragma unroll 1
+            for (int k = 0; k < to.n && k < 32; ++k) {
+                const size_t e = to.at + k * to.step;
+                if (to.dtype == kOrthoF32) static_cast<float *>(to.p)[e] = NAN;
+                else if (to.dtype == kOrthoBF16) static_cast<__nv_bfloat16 *>(to.p)[e] = from_f32<__nv_bfloat16>(NAN);
+                else static_cast<__half *>(to.p)[e] = from_f32<__half>(NAN);
+            }
+        }
+    }
+}
+
 // The operand e of the warp's 32 rows and 32 columns from j, four lanes to a row; nothing past the matrix.
 template <bool SPLIT, int EPI>
 __device__ __forceinline__ void fetch32(const OrthoGemm &g, long long b, int row0, int j, int lane, Eight e[4]) {
@@ -427,7 +450,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         const uint32_t idesc = mma_desc(BN, kQDepthMajor);
         int stage = 0, acc = 0;
         uint32_t phase = 0, acc_phase = 0;
-        bool ok = true;
+        bool ok = true, issued = false;
         for (long long t = first; ok && t < tiles; t += stride) {
             const TileAt at = tile_at<BN>(t, per, tiles_n, kSymmetric);
             if (tab.n > 0 && !muon_visible(tab, muon_tensor_of(tab, at.b), at.b)) continue;
@@ -459,10 +482,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                         phase ^= 1u;
                     }
                 }
-                mma_commit(&sh.acc_full[acc], leader); // also after a wait that ran out: what was issued is waited for
+                if (!ok) __threadfence_block(); // the epilogue finds the abort word set behind this barrier
+                mma_commit(&sh.acc_full[acc], leader);
+                issued = true;
                 acc ^= 1;
                 if (acc == 0) acc_phase ^= 1u;
             }
+        }
+        if (!ok && issued) { // wait, with a limit, for the products in flight, which come to an end in their order
+            const uint32_t last_phase = acc == 0 ? acc_phase ^ 1u : acc_phase;
+            for (unsigned i = 0; i < kWaitLimit && !mbar_try(&sh.acc_full[acc ^ 1], last_phase); ++i) {}
         }
         if (DEEP && shared_tile) {
             __syncwarp();
@@ -477,7 +506,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         int acc = 0;
         uint32_t acc_phase = 0;
         bool ok = true;
-        for (long long t = first; ok && t < tiles; t += stride) {
+        long long t = first;
+        for (; ok && t < tiles; t += stride) {
             const TileAt at = tile_at<BN>(t, per, tiles_n, kSymmetric);
             const int tensor = tab.n > 0 ? muon_tensor_of(tab, at.b) : 0;
             if (tab.n > 0 && !muon_visible(tab, tensor, at.b)) continue;
@@ -492,8 +522,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             }
             fetch32<SPLIT, EPI>(g, at.b, i - lane, j, lane, e);
             float v[W];
-            for (int s0 = begin; s0 < end; s0 += chunk) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[acc], acc_phase, abort));
+            for (int s0 = begin; ok && s0 < end; s0 += chunk) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[acc], acc_phase, abort) && !*abort);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t src = tmem + ((uint32_t)(32 * (warp % 4)) << 16) + acc * BN + half * W;
@@ -545,6 +575,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                 finish32<SPLIT, EPI>(g, tab, tensor, at.b, i, j + 32 * c, lane, v + 32 * c, p, di, dj[c], mirror, poisoned, out_stage);
             }
         }
+        if (!E::to_planes && !ok) give_up<EPI, BN, kBM>(g, tab, t, tiles, stride, per, tiles_n, row, half * W, W);
     }
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");

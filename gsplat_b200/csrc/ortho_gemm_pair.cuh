@@ -48,6 +48,14 @@ __device__ __forceinline__ void commit_pair(unsigned long long *bar, uint32_t le
                  : "memory");
 }
 
+// A wait of this block ran out: the other block's abort word is set too, before what this warp does next can be seen there.
+// Both blocks stay until the last barrier.
+__device__ __forceinline__ void abort_other(volatile int *abort, uint32_t rank) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(const_cast<int *>(abort))), "r"(rank ^ 1u));
+    asm volatile("st.shared::cluster.u32 [%0], %1;\n fence.acq_rel.cluster;" ::"r"(at), "r"(1u) : "memory");
+}
+
 template <bool SPLIT, int EPI>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     ortho_pair_kernel(const __grid_constant__ OrthoGemm g, const __grid_constant__ GemmMaps maps,
@@ -134,6 +142,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                     }
                 }
             }
+            if (!ok) abort_other(abort, rank);
             // a wait ran out: the copies in flight, counted on the leader's barriers, land within this time
             for (int i = 0; !ok && i < 10000; ++i) __nanosleep(1000);
         }
@@ -145,7 +154,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             constexpr uint32_t idesc = 1u << 4 | (kQDepthMajor ? 0u : 1u << 16) | (uint32_t)(kPair / 8) << 17 | (uint32_t)(kPair / 16) << 24;
             int stage = 0, acc = 0;
             uint32_t phase = 0, acc_phase = 0;
-            bool ok = true;
+            bool ok = true, issued = false;
             for (long long t = first; ok && t < tiles; t += pairs) {
                 const TileAt at = tile_at<kBM>(t, per, tiles_n, kSymmetric);
                 if (tab.n > 0 && !muon_visible(tab, muon_tensor_of(tab, at.b), at.b)) continue;
@@ -177,10 +186,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                             phase ^= 1u;
                         }
                     }
+                    if (!ok) abort_other(abort, rank); // found set by both epilogues behind this barrier
                     commit_pair(&sh.acc_full[acc], leader);
+                    issued = true;
                     acc ^= 1;
                     if (acc == 0) acc_phase ^= 1u;
                 }
+            }
+            if (!ok) {
+                abort_other(abort, rank);
+                const uint32_t last_phase = acc == 0 ? acc_phase ^ 1u : acc_phase; // the products in flight, with a limit
+                for (unsigned i = 0; issued && i < kWaitLimit && !mbar_try(&sh.acc_full[acc ^ 1], last_phase); ++i) {}
             }
         }
     }
@@ -194,7 +210,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         int acc = 0;
         uint32_t acc_phase = 0;
         bool ok = true;
-        for (long long t = first; ok && t < tiles; t += pairs) {
+        long long t = first;
+        for (; ok && t < tiles; t += pairs) {
             const TileAt at = tile_at<kBM>(t, per, tiles_n, kSymmetric);
             const int tensor = tab.n > 0 ? muon_tensor_of(tab, at.b) : 0;
             if (tab.n > 0 && !muon_visible(tab, tensor, at.b)) continue;
@@ -221,8 +238,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             };
             if (SPLIT) { // the sum goes on in registers
                 float v[W];
-                for (int s0 = 0; s0 < total; s0 += chunk) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[acc], acc_phase, abort));
+                for (int s0 = 0; ok && s0 < total; s0 += chunk) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[acc], acc_phase, abort) && !*abort);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint32_t src = tmem + ((uint32_t)(32 * (warp % 4)) << 16) + acc * kPair + half * W;
@@ -239,7 +256,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 #pragma unroll
                 for (int c = 0; c < W; c += 32) finish(c, v + c);
             } else {
-                ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[acc], acc_phase, abort));
+                ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[acc], acc_phase, abort) && !*abort);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t src = tmem + ((uint32_t)(32 * (warp % 4)) << 16) + acc * kPair + half * W;
@@ -252,8 +269,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 release();
             }
         }
+        if (!E::to_planes && !ok) give_up<EPI, kPair, kPair>(g, tab, t, tiles, pairs, per, tiles_n, (int)rank * 128 + row, half * W, W);
     }
-    if (threadIdx.x == 0 && sh.abort) atomicExch(g.error, 1);
+    if (warp < kEpilogueWarps && *abort) abort_other(abort, rank);
+    if (threadIdx.x == 0 && *abort) atomicExch(g.error, 1);
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     cluster_barrier(); // neither block leaves while the other may reach its shared memory

@@ -294,7 +294,7 @@ template <typename T>
 __global__ void __launch_bounds__(kNormThreads)
     ortho_grad_out_kernel(OrthoPlanes g, OrthoPlanes x, int rows, int cols, int transposed, const double *partial,
                           int chunks, const double *norms, const double *g_factor, float g_scale, float x_scale, float eps,
-                          T *v_x, int tiles_r, int tiles_c, const int *error) {
+                          T *v_x, int tiles_r, int tiles_c, const int *error, const int *kept_error) {
     __shared__ float tile[kSplitTile][kSplitTile + 1];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const long long per = (long long)tiles_r * tiles_c;
@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(kNormThreads)
     const bool middle = by > 0x1p-100 && by < 0x1p120 && factor >= 0x1p-112 && factor <= 0x1p114;
     const float div = (float)by, f = (float)factor;
     const double all = 1.0 / ((double)g_scale * factor * by);
-    const bool poisoned = *error != 0;
+    const bool poisoned = *error != 0 || (kept_error && *kept_error != 0);
     auto value = [&](float gw, float xw) {
         const float v = fmaf(-xw, along, gw);
         return poisoned ? NAN : middle ? v / g_scale / f / div : (float)((double)v * all);
@@ -486,13 +486,16 @@ struct Carver {
     }
 };
 
-// What a backward pass needs of the steps: each one's X, A and B, and the norms.
+// What a backward pass needs of the steps: each one's X, A and B, and the norms. A wait of the steps that ran out is known by
+// the error word of tiled products, by NaN in the place of its matrix's norm of the clustered kernel, which leaves the word alone.
 struct OrthoBuffers {
+    int *error;
     OrthoPlanes x[kOrthoMaxSteps], a[kOrthoMaxSteps], b[kOrthoMaxSteps];
     float *da[kOrthoMaxSteps], *db[kOrthoMaxSteps];
     double *norms;
 
     OrthoBuffers(Carver &ws, const OrthoPlan &p, long long nb) {
+        error = ws.take<int>(1);
         for (int k = 0; k < p.steps; ++k) {
             x[k] = ws.planes(nb, p.px, p.ldx);
             a[k] = ws.planes(nb, p.pa, p.lda);
@@ -636,7 +639,8 @@ static double backward_scale(const OrthoPlan &p) { return std::fmin(p.s.b, pow2_
 
 // The steps, each one's X, A and B kept; y may be NULL (the last product is then left out).
 static int ortho_tiled_kept(const OrthoPlan &p, const OrthoCoefficients &co, long long nb, const void *src, void *y, int dtype,
-                            const OrthoBuffers &w, float eps, double *partial, int *error, cudaStream_t stream) {
+                            const OrthoBuffers &w, float eps, double *partial, cudaStream_t stream) {
+    int *const error = w.error;
     const double sb = backward_scale(p);
     const MuonTable none = {};
     if (int e = run_split(p, nb, src, dtype, none, (float)p.s.x, eps, w.norms, partial, w.x[0], error, stream)) return e;
@@ -673,12 +677,12 @@ static int ortho_tiled_bwd(const OrthoPlan &p, const OrthoCoefficients &co, long
     double *partial = ws.take<double>((size_t)nb * p.chunks);
     double *factor[2] = {ws.take<double>(nb), ws.take<double>(nb)};
     double *const norms = w.norms;
-    int *error = ws.take<int>(1);
+    int *error = kept ? ws.take<int>(1) : w.error;
     const MuonTable none = {};
     const double shrink = std::exp2(std::ceil(std::log2(p.s.slope)));
     const double sb = backward_scale(p);
     if (!kept)
-        if (int e = ortho_tiled_kept(p, co, nb, src, nullptr, dtype, w, eps, partial, error, stream)) return e;
+        if (int e = ortho_tiled_kept(p, co, nb, src, nullptr, dtype, w, eps, partial, stream)) return e;
     if (int e = run_split(p, nb, v, dtype, none, (float)kPlaneTop, 0.f, factor[0], partial, gr[K & 1], kept ? error : nullptr, stream))
         return e;
     double grown = 1.0; // G's scale has fallen by this
@@ -727,11 +731,12 @@ static int ortho_tiled_bwd(const OrthoPlan &p, const OrthoCoefficients &co, long
     }
     if (int e = run_dot(p, nb, gr[0], w.x[0], partial, stream)) return e;
     const int tr = (p.m + kSplitTile - 1) / kSplitTile, tc = (p.n + kSplitTile - 1) / kSplitTile;
+    const int *kept_error = kept && !ortho_is_clustered(p.rows, p.cols) ? w.error : nullptr;
     return with_source(dtype, none, [&](auto tv, auto, auto) {
         using T = decltype(tv);
         return launch_after(ortho_grad_out_kernel<T>, (unsigned)(nb * tr * tc), kNormThreads, 0, stream, "ortho_grad_out_kernel", gr[0],
                             w.x[0], p.rows, p.cols, p.transposed, (const double *)partial, p.chunks, (const double *)norms,
-                            (const double *)factor[0], (float)grown, (float)p.s.x, eps, static_cast<T *>(v_x), tr, tc, (const int *)error);
+                            (const double *)factor[0], (float)grown, (float)p.s.x, eps, static_cast<T *>(v_x), tr, tc, (const int *)error, kept_error);
     });
 }
 
@@ -832,8 +837,7 @@ extern "C" int gsb_orthogonalize_fwd(long long batch, int rows, int cols, int dt
     if (kept) {
         const OrthoBuffers w(own, p, batch);
         Carver ws{static_cast<char *>(scratch)};
-        double *partial = ws.take<double>((size_t)batch * p.chunks);
-        return ortho_tiled_kept(p, co, batch, x, y, dtype, w, eps, partial, ws.take<int>(1), stream);
+        return ortho_tiled_kept(p, co, batch, x, y, dtype, w, eps, ws.take<double>((size_t)batch * p.chunks), stream);
     }
     const long long chunk = ortho_chunk(p, batch);
     const MuonTable none = {};

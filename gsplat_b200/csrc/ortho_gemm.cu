@@ -54,7 +54,7 @@ int ortho_gemm(const OrthoGemm &g, const MuonTable *table, cudaStream_t stream) 
     const long long t64 = (n64 + sms - 1) / sms * (g.split || n64 * r64 <= sms / 2 ? 79 : 122) / r64;
     const long long t128 = (n128 + sms - 1) / sms * (g.split ? 112 : n128 * r128 <= sms / 2 ? 126 : 162) / r128;
     const long long t256 = (n256 + sms / 2 - 1) / (sms / 2) * (g.split || n256 <= sms / 4 ? 165 : 237);
-    const bool pair = t256 < t128 && t256 < t64;
+    const bool pair = t256 < t128 && t256 < t64 && (g.split || g.K <= kPairHiDepth);
     const int bn = !pair && t64 < t128 ? 64 : 128;
     for (int i = 0; i < g.pairs; ++i) {
         const int qr = g.q_k_major ? g.N : g.K, qc = g.q_k_major ? g.K : g.N, qb = g.q_k_major ? bn : 64;

@@ -5,7 +5,7 @@
 //
 // A tile is 128 x BN of the result, 64 deep a stage. With SPLIT, a stage holds
 // the hi and lo planes of both operands and feeds three products (hi hi, hi lo, lo hi);
-// the sum is taken out of the tensor cores every kChunk stages and continued in
+// the sum is taken out of the tensor cores every kChunk stages (kHiChunk without it) and continued in
 // registers, since their 32-bit adder truncates and the bias of a long sum of
 // squares would be seen in the diagonal of A.
 // A product of a middle-sized matrix takes about 8.5 us: 1.8 from the end of the launch before it, 2.2 until the first copies are
@@ -15,6 +15,7 @@
 
 #include <algorithm>
 #include <cuda.h>
+#include <type_traits>
 
 #include "ortho.cuh"
 #include "tcgen05.cuh"
@@ -24,6 +25,9 @@ namespace gsb {
 constexpr int kBM = 128, kBK = 64;
 constexpr int kChunk = 4; // stages between two readings of the accumulator, split: a result 1.3e-6 off, 2.6e-6 with 8
                           // (FP32 GEMMs 2.5 to 4.8e-6)
+// Products of hi alone are read out every 2048 of depth: the truncation takes 5e-8 of the sum at each of its additions (16
+// deep), 6e-6 in 2048, where the operands' 11 bits take 2e-4. Unread, the square of a row of 8 million was 3e-3 short.
+constexpr int kHiChunk = 32;
 constexpr int kEpilogueWarps = 8;  // four lane quarters x two column halves
 constexpr int kGemmThreads = 32 * (kEpilogueWarps + 2);
 constexpr int kStagePitch = 33;    // floats a row of a warp's 32 x 32 values on their way out
@@ -390,7 +394,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     const int ranks = DEEP ? (int)cluster_size() : 1, rank = DEEP ? (int)block_rank() : 0;
     const int all = kblocks * g.pairs;                                              // stages of a tile
     const int begin = DEEP ? all * rank / ranks : 0, end = DEEP ? all * (rank + 1) / ranks : all; // this block's
-    const int chunk = SPLIT ? kChunk : end - begin;                                 // stages of an accumulation
+    const int chunk = SPLIT ? kChunk : kHiChunk;                                    // stages of an accumulation
     const long long first = DEEP ? blockIdx.x / ranks : blockIdx.x, stride = DEEP ? gridDim.x / ranks : gridDim.x;
     // whether the cluster's one tile is worked on, by all of its blocks' warps
     const bool shared_tile = DEEP && !(tab.n > 0 && !muon_visible(tab, muon_tensor_of(tab, first / per), first / per));
@@ -522,23 +526,34 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             }
             fetch32<SPLIT, EPI>(g, at.b, i - lane, j, lane, e);
             float v[W];
-            for (int s0 = begin; ok && s0 < end; s0 += chunk) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[acc], acc_phase, abort) && !*abort);
-                if (!ok) break;
+            auto take = [&](auto known, bool first_part) { // a part of the sum
+                ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[acc], acc_phase, abort) && (E::to_planes || !*abort));
+                if (!ok) return;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t src = tmem + ((uint32_t)(32 * (warp % 4)) << 16) + acc * BN + half * W;
 #pragma unroll
                 for (int c = 0; c < W; c += 32) {
+                    if (known && first_part) {
+                        tmem_load32(src + c, v + c);
+                        continue;
+                    }
                     float u[32];
                     tmem_load32(src + c, u);
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) v[c + k] = s0 == begin ? u[k] : v[c + k] + u[k];
+                    for (int k = 0; k < 32; ++k) v[c + k] = !known && first_part ? u[k] : v[c + k] + u[k];
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.acc_empty[acc]);
                 acc ^= 1;
                 if (acc == 0) acc_phase ^= 1u;
+            };
+            if (SPLIT) {
+                for (int s0 = begin; ok && s0 < end; s0 += chunk) take(std::false_type(), s0 == begin);
+            } else { // mostly the first part is all
+                take(std::true_type(), true);
+#pragma unroll 1
+                for (int s0 = begin + chunk; ok && s0 < end; s0 += chunk) take(std::true_type(), false);
             }
             if (DEEP) { // rank r's sums at r - 1 of [ranks - 1][warp][W / 4][lane], four columns each
                 const uint32_t sums = stage0 + (uint32_t)(warp * (W / 4) * 32 + lane) * 16;

@@ -14,6 +14,10 @@ namespace gsb {
 
 constexpr int kPair = 256;   // rows and columns of a tile
 constexpr int kPairChunk = 8; // stages between two readings of the accumulator, split (4 cost 8% of a product)
+// Of hi alone sums are not read out, so that they need no registers and a warp finishes 32 columns at a time (with
+// registers for the sum [2048, 8192] took 1047 us instead of 752). The truncation takes 5e-5 of a sum 16384 deep, a quarter of
+// what the operands' 11 bits take; deeper ones are left to the tiles of ortho_gemm.cuh.
+constexpr int kPairHiDepth = 16384;
 
 // Split sums go on in 128 registers of an epilogue thread, more than three warpgroups at 168 leave it: the
 // warpgroup of the copies and products gives 112 of its own. 2 x 224 + 56 = 3 x 168.
@@ -239,7 +243,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             if (SPLIT) { // the sum goes on in registers
                 float v[W];
                 for (int s0 = 0; ok && s0 < total; s0 += chunk) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[acc], acc_phase, abort) && !*abort);
+                    ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[acc], acc_phase, abort) && (E::to_planes || !*abort));
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint32_t src = tmem + ((uint32_t)(32 * (warp % 4)) << 16) + acc * kPair + half * W;
@@ -256,7 +260,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 #pragma unroll
                 for (int c = 0; c < W; c += 32) finish(c, v + c);
             } else {
-                ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[acc], acc_phase, abort) && !*abort);
+                ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[acc], acc_phase, abort) && (E::to_planes || !*abort));
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t src = tmem + ((uint32_t)(32 * (warp % 4)) << 16) + acc * kPair + half * W;

@@ -75,3 +75,14 @@ def test_muon_with_norm_above_the_largest_float(shape):
     want = p.double() - 0.1 * N.newton_schulz(0.19 * g.double())
     allowed = 0.1 * N.tolerance(g, 5, N.QUINTIC) * N.newton_schulz(g).norm() + 4 * 2.0**-24 * want.norm()
     assert (tp.cpu().double() - want).norm() <= allowed
+
+
+@pytest.mark.parametrize("length", [100_000, 8_000_000])
+def test_square_of_a_long_row(length):
+    """A = |x0|^2 = 1, a sum of squares that a truncating adder falls short of. With p = -15 s + 16 s^3 the result is x0, 16 times
+    A's error off in length. bfloat16 operands have 11 bits here: their roundings, of 128 mantissas, leave the mean of
+    squares 2 * 2^-12 / sqrt(128) off, 16 of which are 7e-4; and bfloat16 results scatter by 2^-9, which the mean forgets."""
+    x = data((1, length), torch.bfloat16, 310, 1.0)
+    y = gs().orthogonalize(x.cuda(), steps=1, coefficients=(-15.0, 16.0, 0.0)).cpu().double()
+    x0 = x.double() / x.double().norm()
+    assert abs(float((y * x0).sum()) - 1) < 2e-3

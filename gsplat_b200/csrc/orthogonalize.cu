@@ -938,6 +938,7 @@ static int check_tensors(int n_tensors, const GsbMuonTensor *tensors) {
         const GsbMuonTensor &t = tensors[i];
         if (t.batch < 0 || t.rows < 0 || t.cols < 0 || t.inner < 1)
             return set_error(kErrInvalidArgument, "muon: tensor %d: %lld x [%d, %d], inner %d", i, t.batch, t.rows, t.cols, t.inner);
+        if (!(t.gain == tensors[0].gain)) return set_error(kErrInvalidArgument, "muon: tensor %d: a gain of its own", i);
     }
     return kOk;
 }
@@ -973,8 +974,9 @@ extern "C" int gsb_muon(int n_tensors, const GsbMuonTensor *tensors, int dtype, 
     t.dtype = dtype;
     t.state_dtype = state_dtype;
     t.nesterov = nesterov;
+    const float gain = n_tensors > 0 ? tensors[0].gain : 0.f;
     t.mu = momentum;
-    t.one_minus_mu = (float)(1.0 - (double)momentum);
+    t.one_minus_mu = gain != 0.f ? gain : (float)(1.0 - (double)momentum);
     t.valid = valid;
     int sizes[kOrthoMaxTensors][2]; // rows and columns of the tensors in t
     for (int from = 0; from < n_tensors; from += kMuonSlice) {

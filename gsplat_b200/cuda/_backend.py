@@ -68,6 +68,7 @@ class GsbMuonTensor(ctypes.Structure):
         ("inner", I32),
         ("lr", F32),
         ("decay", F32),
+        ("gain", F32),
     ]
 
 

@@ -326,7 +326,7 @@ def muon(
         batch = numel // (rows * cols)
         inner = batch // shape[0] if len(shape) > 2 else 1
         groups.setdefault((dtype, state_dtype), []).append(
-            (at_p, at_g, at_m, batch, rows, cols, inner, rate * scale, 1.0 - rate * weight_decay))
+            (at_p, at_g, at_m, batch, rows, cols, inner, rate * scale, 1.0 - rate * weight_decay, 1.0 - momentum))
     read_end = write_end = 0
     for start, end, read_only in sorted(spans):
         if start < write_end or (not read_only and start < read_end):

@@ -473,8 +473,10 @@ GSB_API int gsb_adam_multi(int n_groups, const GsbAdamGroup *groups, const bool 
  * wait of the forward call's kernels ran out (shapes above a short side of 128: a first 32-bit word
  * that is not 0): the gradient is then NaN.
  * gsb_muon: for the listed tensors of one type, each a batch of matrices:
- * m <- m + (1 - momentum)(grad - m); u = grad + momentum (m - grad) (nesterov) or m; param <- decay * param - lr * orthogonalized(u). momentum_buffer has
- * the type of param or float32 (state_dtype). valid (optional): a row of a tensor's leading
+ * m <- m + (1 - momentum)(grad - m); u = grad + momentum (m - grad) (nesterov) or m;
+ * param <- decay * param - lr * orthogonalized(u). 1 - momentum is taken from the tensors' gain where that is not 0
+ * (the same for all), since a float near 1 leaves few bits of it.
+ * momentum_buffer has the type of param or float32 (state_dtype). valid (optional): a row of a tensor's leading
  * dimension (`inner` matrices) whose entry is false keeps its values. Tensors must not overlap.
  * Scratch: gsb_orthogonalize_scratch_bytes of the whole batch (kept = 1: for a call with a
  * kept state), gsb_muon_scratch_bytes of the list; 0 where none is needed. Calls that
@@ -500,6 +502,7 @@ typedef struct GsbMuonTensor {
     int inner;       /* matrices of one row of the leading dimension */
     float lr;        /* of the update, with the factor of the matrix's shape where there is one */
     float decay;     /* 1 - (learning rate) * weight_decay; without that factor */
+    float gain;      /* 1 - momentum, or 0: from the float */
 } GsbMuonTensor;
 GSB_API size_t gsb_muon_scratch_bytes(int n_tensors, const GsbMuonTensor *tensors, int dtype, int steps);
 GSB_API int gsb_muon(int n_tensors, const GsbMuonTensor *tensors, int dtype, int state_dtype,

@@ -68,3 +68,13 @@ def test_visibility_and_checkpoint():
     opt.step(vis)
     other.step(vis)
     assert torch.equal(q.detach(), sh.detach()) and torch.equal(other.state[q]["momentum_buffer"], buffer)
+
+
+@pytest.mark.parametrize("shape", [(300, 15, 3), (2, 4, 60), (40, 30), (200, 140)])
+def test_momentum_near_one(shape):
+    """1 - 0.9999 to 32 bits: from a buffer of zeros m = (1 - momentum) g, in three roundings."""
+    p, g = data(shape, torch.float32, 230, 0.1).cuda(), data(shape, torch.float32, 231, 1.0).cuda()
+    m = torch.zeros_like(p)
+    gs().muon(p, g, m, None, 0.1, 0.9999)
+    want = (1 - 0.9999) * g.double()
+    assert ((m.double() - want).abs() <= 3 * 2.0**-24 * want.abs()).all()

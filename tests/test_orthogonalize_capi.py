@@ -1,4 +1,5 @@
-"""CPU checks of the C entry points' kept state: it is refused before any launch where there is none or it is too short."""
+"""CPU checks of what the C entry points refuse before any launch: a kept state where there is none or that is too short, and lists
+that do not agree."""
 
 import ctypes
 
@@ -44,3 +45,12 @@ def test_kept_state_too_short(batch, rows, cols):
     for size in (0, 1, needed - 1):
         fwd, bwd, message = both(batch, rows, cols, SOMEWHERE, size)
         assert fwd == -1 and bwd == -1 and b"needs %d" % needed in message
+
+
+def test_gains_of_a_muon_list_must_agree():
+    from gsplat_b200.cuda._backend import GsbMuonTensor
+
+    L, c = lib(), (ctypes.c_float * 15)(*(list(N.QUINTIC) * 5))
+    for other in (0.0, 0.2, float("nan")):
+        two = (GsbMuonTensor * 2)((None, None, None, 0, 4, 4, 1, 0.1, 1.0, 0.1), (None, None, None, 0, 4, 4, 1, 0.1, 1.0, other))
+        assert L.gsb_muon(2, two, 0, 0, None, 0.9, 1, 5, c, 1e-7, None, 0, None) == -1 and b"gain" in L.gsb_last_error()

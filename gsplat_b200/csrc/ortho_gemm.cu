@@ -72,7 +72,10 @@ int ortho_gemm(const OrthoGemm &g, const MuonTable *table, cudaStream_t stream) 
     }
     static const MuonTable none = {};
     const MuonTable &tab = table ? *table : none;
-    if (pair) return g.split ? ortho_pair_launch<true>(g, maps, tab, sms, stream) : ortho_pair_launch<false>(g, maps, tab, sms, stream);
+    if (pair) {
+        const int e = g.split ? ortho_pair_launch<true>(g, maps, tab, sms, stream) : ortho_pair_launch<false>(g, maps, tab, sms, stream);
+        if (e != kPairUnfit) return e; // else 128 x 128 tiles, whose tensor maps are the same
+    }
     if (bn == 64)
         return g.split ? ortho_gemm_launch<true, 64>(g, maps, tab, sms, stream) : ortho_gemm_launch<false, 64>(g, maps, tab, sms, stream);
     return g.split ? ortho_gemm_launch<true, 128>(g, maps, tab, sms, stream) : ortho_gemm_launch<false, 128>(g, maps, tab, sms, stream);

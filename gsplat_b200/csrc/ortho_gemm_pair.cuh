@@ -8,6 +8,8 @@
 // counted on the leader's barriers, and its commits free the stages and hand over the accumulators of both.
 #pragma once
 
+#include <atomic>
+
 #include "ortho_gemm.cuh"
 
 namespace gsb {
@@ -22,6 +24,8 @@ constexpr int kPairHiDepth = 16384;
 // Split sums go on in 128 registers of an epilogue thread, more than three warpgroups at 168 leave it: the
 // warpgroup of the copies and products gives 112 of its own. 2 x 224 + 56 = 3 x 168.
 constexpr int kPairThreads = 384, kPairRegisters = 168, kEpilogueRegisters = 224, kIssueRegisters = 56;
+
+constexpr int kPairUnfit = 1; // of a launch: the kernel was built with other registers. Tiles of one SM serve
 
 template <bool SPLIT> struct PairStages {
     static constexpr int plane = 128 * kBK * 2, bytes = (SPLIT ? 4 : 2) * plane;
@@ -293,12 +297,13 @@ static int pair_one(const OrthoGemm &g, const GemmMaps &maps, const MuonTable &t
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
         return check_launch("ortho_pair_kernel attributes");
     if (SPLIT) { // the warpgroups' shares must be what the block is launched with, or they would be waited for
-        static const int registers = [kernel] {
+        static std::atomic<int> registers{0}; // 0: not known
+        if (registers == 0) {
             cudaFuncAttributes a;
-            return cudaFuncGetAttributes(&a, kernel) == cudaSuccess ? a.numRegs : 0;
-        }();
-        if (registers != kPairRegisters)
-            return set_error(kErrUnsupported, "ortho_pair_kernel: built with %d registers, not %d", registers, kPairRegisters);
+            if (cudaFuncGetAttributes(&a, kernel) != cudaSuccess) return check_launch("ortho_pair_kernel registers");
+            registers = a.numRegs;
+        }
+        if (registers != kPairRegisters) return kPairUnfit;
     }
     const long long pairs = tiles < sms / 2 ? tiles : sms / 2;
     return launch_after(kernel, (unsigned)(2 * pairs), kPairThreads, smem, stream, "ortho_pair_kernel", g, maps, tab, per, tn, tiles);

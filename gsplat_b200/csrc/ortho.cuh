@@ -223,4 +223,10 @@ struct OrthoGemm {
 
 int ortho_gemm(const OrthoGemm &g, const MuonTable *table, cudaStream_t stream);
 
+// The tile that a product takes on a GPU of `sms` SMs: its columns (256: of a pair of SMs) and the blocks that share its depth.
+struct OrthoTile {
+    int columns, ranks;
+};
+OrthoTile ortho_tile(const OrthoGemm &g, int sms);
+
 } // namespace gsb

@@ -37,14 +37,12 @@ static int sm_count() {
     return sms;
 }
 
-int ortho_gemm(const OrthoGemm &g, const MuonTable *table, cudaStream_t stream) {
-    if (encode_fn() == nullptr) return set_error(kErrUnsupported, "orthogonalize: the driver offers no tensor maps");
-    GemmMaps maps;
+OrthoTile ortho_tile(const OrthoGemm &g, int sms) {
     // The tile with the least time: rounds over the SMs x cycles of a product 16 deep / blocks that share the depth. The
     // cycles are measured: the operand bytes that an SM's shared memory delivers bound them where few SMs work, those
     // that the L2 delivers (7 KB a cycle) where all do. A 128 x 64 tile 79, or 122 for hi planes alone on all SMs;
     // 128 x 128 112 split, 126 or 162; a pair's 256 x 256 165 split (also where few work, for its longer end), 237.
-    const int sms = sm_count(), tm = (g.M + kBM - 1) / kBM, tn = (g.N + 127) / 128, tn64 = (g.N + 63) / 64;
+    const int tm = (g.M + kBM - 1) / kBM, tn = (g.N + 127) / 128, tn64 = (g.N + 63) / 64;
     const int pm = (g.M + kPair - 1) / kPair, pn = (g.N + kPair - 1) / kPair;
     const long long n64 = g.batch * (g.symmetric ? tm * (tm + 1) - (2 * tm - tn64) : tm * tn64);
     const long long n128 = g.batch * (g.symmetric ? tm * (tm + 1) / 2 : tm * tn);
@@ -54,8 +52,14 @@ int ortho_gemm(const OrthoGemm &g, const MuonTable *table, cudaStream_t stream) 
     const long long t64 = (n64 + sms - 1) / sms * (g.split || n64 * r64 <= sms / 2 ? 79 : 122) / r64;
     const long long t128 = (n128 + sms - 1) / sms * (g.split ? 112 : n128 * r128 <= sms / 2 ? 126 : 162) / r128;
     const long long t256 = (n256 + sms / 2 - 1) / (sms / 2) * (g.split || n256 <= sms / 4 ? 165 : 237);
-    const bool pair = t256 < t128 && t256 < t64 && (g.split || g.K <= kPairHiDepth);
-    const int bn = !pair && t64 < t128 ? 64 : 128;
+    if (t256 < t128 && t256 < t64 && (g.split || g.K <= kPairHiDepth)) return {256, 1};
+    return t64 < t128 ? OrthoTile{64, r64} : OrthoTile{128, r128};
+}
+
+int ortho_gemm(const OrthoGemm &g, const MuonTable *table, cudaStream_t stream) {
+    if (encode_fn() == nullptr) return set_error(kErrUnsupported, "orthogonalize: the driver offers no tensor maps");
+    GemmMaps maps;
+    const int sms = sm_count(), columns = ortho_tile(g, sms).columns, bn = std::min(columns, 128);
     for (int i = 0; i < g.pairs; ++i) {
         const int qr = g.q_k_major ? g.N : g.K, qc = g.q_k_major ? g.K : g.N, qb = g.q_k_major ? bn : 64;
         if (!encode(&maps.p_hi[i], g.p[i].hi, g.p[i], g.M, g.K, g.batch, kBM) ||
@@ -72,7 +76,7 @@ int ortho_gemm(const OrthoGemm &g, const MuonTable *table, cudaStream_t stream) 
     }
     static const MuonTable none = {};
     const MuonTable &tab = table ? *table : none;
-    if (pair) {
+    if (columns == 256) {
         const int e = g.split ? ortho_pair_launch<true>(g, maps, tab, sms, stream) : ortho_pair_launch<false>(g, maps, tab, sms, stream);
         if (e != kPairUnfit) return e; // else 128 x 128 tiles, whose tensor maps are the same
     }

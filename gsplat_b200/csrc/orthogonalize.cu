@@ -808,6 +808,25 @@ static int check_kept(long long batch, int rows, int cols, int steps, const void
     return kOk;
 }
 
+extern "C" int gsb_orthogonalize_tile(long long batch, int rows, int cols, int dtype, int kept, int product, int sms) {
+    if (batch <= 0 || rows <= 0 || cols <= 0 || product < 0 || product > 5 || sms < 2 || ortho_is_thin(rows, cols) ||
+        (product < 3 && ortho_is_clustered(rows, cols)))
+        return 0;
+    OrthoCoefficients co = {};
+    co.steps = 1;
+    const OrthoPlan p = ortho_plan(rows, cols, dtype, co, product >= 3, kept != 0);
+    static const int epilogues[6] = {kEpiGram, kEpiSquare, kEpiApply, kEpiSym, kEpiAnti, kEpiApply};
+    OrthoGemm g = gemm_base(p, batch, nullptr);
+    g.M = p.m;
+    g.N = product % 3 == 2 ? p.n : p.m;
+    g.K = product % 3 == 0 ? p.n : p.m;
+    g.pairs = product < 3 ? 1 : 2;
+    g.epilogue = epilogues[product];
+    g.symmetric = product % 3 != 2;
+    const OrthoTile t = ortho_tile(g, sms);
+    return 1000 * t.ranks + t.columns;
+}
+
 static const char *at_matrix(const void *p, long long b, int rows, int cols, int dtype) {
     return static_cast<const char *>(p) + (size_t)b * rows * cols * (dtype == kOrthoF32 ? 4 : 2);
 }

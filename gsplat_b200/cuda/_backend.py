@@ -174,6 +174,7 @@ SIGNATURES = {
     "gsb_adam_multi": (I32, [I32, ctypes.POINTER(GsbAdamGroup), P, F32, F32, P]),
     "gsb_orthogonalize_kept_bytes": (SZ, [I64, I32, I32, I32]),
     "gsb_orthogonalize_scratch_bytes": (SZ, [I64, I32, I32, I32, I32, I32, I32]),
+    "gsb_orthogonalize_tile": (I32, [I64, I32, I32, I32, I32, I32, I32]),
     "gsb_orthogonalize_fwd": (I32, [I64, I32, I32, I32, P, P, I32, P, F32, P, SZ, P, SZ, P]),
     "gsb_orthogonalize_bwd": (I32, [I64, I32, I32, I32, P, P, P, I32, P, F32, P, SZ, P, SZ, P]),
     "gsb_muon_scratch_bytes": (SZ, [I32, ctypes.POINTER(GsbMuonTensor), I32, I32]),

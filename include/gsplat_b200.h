@@ -484,6 +484,9 @@ GSB_API int gsb_adam_multi(int n_groups, const GsbAdamGroup *groups, const bool 
 GSB_API size_t gsb_orthogonalize_kept_bytes(long long batch, int rows, int cols, int steps);
 GSB_API size_t gsb_orthogonalize_scratch_bytes(long long batch, int rows, int cols, int dtype,
                                        int steps, int backward, int kept);
+/* Which tile a product takes on a GPU of `sms` SMs, 1000 x (blocks that share its depth) + its columns (256: a pair of
+ * SMs'), or 0 where there are no tiles. product: a step's A, B, X (0 to 2), the backward pass's S, T, G (3 to 5). For tests. */
+GSB_API int gsb_orthogonalize_tile(long long batch, int rows, int cols, int dtype, int kept, int product, int sms);
 GSB_API int gsb_orthogonalize_fwd(long long batch, int rows, int cols, int dtype, const void *x,
                           void *y, int steps, const float *coefficients, float eps, void *kept,
                           size_t kept_bytes, void *scratch, size_t scratch_bytes,

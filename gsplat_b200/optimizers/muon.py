@@ -52,7 +52,17 @@ class Muon(torch.optim.Optimizer):
                     self.state[p]["momentum_buffer"] = buffer.to(p.device, group["momentum_dtype"] or p.dtype).contiguous()
 
     @torch.no_grad()
-    def step(self, visibility=None):
+    def step(self, visibility=None, closure=None):
+        """One step. ``visibility`` [B]: the rows that are stepped, of parameters [B, ..., M, N]. A ``closure`` (also as the only
+        argument, as of torch's optimizers) is called first, with gradients on, and its value returned."""
+        if callable(visibility):
+            if closure is not None:
+                raise TypeError("step() takes one closure")
+            visibility, closure = None, visibility
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
         if visibility is not None:
             visibility = visibility.contiguous()
         for group in self.param_groups:
@@ -73,6 +83,7 @@ class Muon(torch.optim.Optimizer):
                 scales.append(_shape_factor(group["adjust_lr_fn"], *p.shape[-2:]))
             muon(params, grads, buffers, visibility, group["lr"], group["momentum"], group["weight_decay"], group["nesterov"],
                  group["ns_steps"], group["ns_coefficients"], group["eps"], scales)
+        return loss
 
 
 def _shape_factor(rule, rows: int, cols: int) -> float:

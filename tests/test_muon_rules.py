@@ -95,3 +95,27 @@ def test_state_of_torch_muon_is_taken(plain):
     b.grad = torch.ones(4, 6, dtype=torch.bfloat16)
     opt.step()
     assert opt.state[b]["momentum_buffer"].dtype == torch.float32
+
+
+def test_step_takes_a_closure(plain):
+    """As torch's optimizers do: called with gradients on, before the step, its value returned."""
+    gen = torch.Generator().manual_seed(3)
+    w = torch.randn(6, 5, generator=gen)
+    ours, theirs = (torch.nn.Parameter(w.clone()) for _ in range(2))
+    opt = gsplat_b200.Muon([ours], lr=0.1)
+    other = gsplat_b200.Muon([theirs], lr=0.1)
+
+    def closure():
+        opt.zero_grad()
+        loss = (ours * ours).sum()
+        loss.backward()
+        return loss
+
+    (theirs * theirs).sum().backward()
+    other.step()
+    assert float(opt.step(closure)) == pytest.approx(float((w * w).sum()), rel=1e-6)
+    assert torch.equal(ours, theirs) and not torch.equal(ours, w)
+    assert float(opt.step(closure=closure)) < float((w * w).sum())
+    assert opt.step() is None
+    with pytest.raises(TypeError):
+        opt.step(closure, closure)

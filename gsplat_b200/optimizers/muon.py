@@ -30,10 +30,14 @@ class Muon(torch.optim.Optimizer):
                         ns_coefficients=ns_coefficients, eps=eps, ns_steps=ns_steps, adjust_lr_fn=adjust_lr_fn,
                         momentum_dtype=momentum_dtype)
         super().__init__(params, defaults)
-        for group in self.param_groups:
-            for p in group["params"]:
-                if p.dim() < 2:
-                    raise ValueError(f"Muon takes matrices [..., M, N], got a parameter {tuple(p.shape)}")
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        try:
+            _check_group(self.param_groups[-1])
+        except (TypeError, ValueError):
+            self.param_groups.pop()
+            raise
 
     def load_state_dict(self, state_dict):
         """As torch's, which casts all state to the parameter's type; the momentum buffers are taken from the saved state
@@ -84,6 +88,15 @@ class Muon(torch.optim.Optimizer):
             muon(params, grads, buffers, visibility, group["lr"], group["momentum"], group["weight_decay"], group["nesterov"],
                  group["ns_steps"], group["ns_coefficients"], group["eps"], scales)
         return loss
+
+
+def _check_group(group) -> None:
+    for p in group["params"]:
+        if p.dim() < 2:
+            raise ValueError(f"Muon takes matrices [..., M, N], got a parameter {tuple(p.shape)}")
+        if group["momentum_dtype"] not in (None, p.dtype, torch.float32):
+            raise TypeError(f"momentum_dtype must be None, the parameter's type or float32, got {group['momentum_dtype']} "
+                            f"for {p.dtype}")
 
 
 def _shape_factor(rule, rows: int, cols: int) -> float:

@@ -119,3 +119,18 @@ def test_step_takes_a_closure(plain):
     assert opt.step() is None
     with pytest.raises(TypeError):
         opt.step(closure, closure)
+
+
+def test_unsuitable_parameters_are_refused_before_the_first_step():
+    half, full = torch.nn.Parameter(torch.ones(4, 4, dtype=torch.bfloat16)), torch.nn.Parameter(torch.ones(4, 4))
+    for p, dtype in ((half, torch.float16), (full, torch.bfloat16), (full, torch.float64)):
+        with pytest.raises(TypeError, match="momentum_dtype"):
+            gsplat_b200.Muon([p], momentum_dtype=dtype)
+    for p, dtype in ((half, torch.bfloat16), (half, torch.float32), (half, None), (full, torch.float32)):
+        gsplat_b200.Muon([p], momentum_dtype=dtype)
+    opt = gsplat_b200.Muon([full])
+    for bad in (dict(params=[torch.nn.Parameter(torch.ones(4))]), dict(params=[half], momentum_dtype=torch.float16)):
+        with pytest.raises((TypeError, ValueError)):
+            opt.add_param_group(bad)
+    assert len(opt.param_groups) == 1
+    opt.add_param_group(dict(params=[half], momentum_dtype=torch.float32))

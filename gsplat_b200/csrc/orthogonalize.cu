@@ -447,7 +447,7 @@ static OrthoPlan ortho_plan(int rows, int cols, int dtype, const OrthoCoefficien
     size_t bytes = sizeof(double) * (size_t)(p.chunks + 2); // sums, and norms or two factors
     if (backward)
         bytes += 2 * halves * (p.px + p.pa); // G twice, S, T
-    else
+    else if (!kept) // else all but the sums lies in the state
         bytes += 2 * halves * (p.px + p.pa) + 2 * sizeof(float) * p.m; // X twice, A, B, diagonals
     p.per_matrix = bytes;
     p.fixed = 256 * 24;

@@ -54,3 +54,11 @@ def test_gains_of_a_muon_list_must_agree():
     for other in (0.0, 0.2, float("nan")):
         two = (GsbMuonTensor * 2)((None, None, None, 0, 4, 4, 1, 0.1, 1.0, 0.1), (None, None, None, 0, 4, 4, 1, 0.1, 1.0, other))
         assert L.gsb_muon(2, two, 0, 0, None, 0.9, 1, 5, c, 1e-7, None, 0, None) == -1 and b"gain" in L.gsb_last_error()
+
+
+def test_scratch_of_a_forward_that_keeps_its_state():
+    """X, A and B lie in the state: beside it only the norm's sums are needed."""
+    size = lib().gsb_orthogonalize_scratch_bytes
+    assert size(1, 3000, 2900, 0, 5, 0, 0) > 100 * 2**20
+    assert size(1, 3000, 2900, 0, 5, 0, 1) < 2**16
+    assert size(1, 300, 200, 0, 5, 1, 1) > 2**20 // 4  # backwards G, S and T are

@@ -32,7 +32,6 @@ struct ClusterShape {
     int m, n, transposed;   // short, long; the tensor is [n, m]
     int m16, mk, ns, ns64;  // rounded up: m to 16 and 64, a block's columns to 16 and 64
     int blocks, columns;    // of a cluster; of TMEM
-    int slack;              // bytes behind the planes that a 128-row operand may touch
     int per;                // rows of A that a block of a cluster adds up
     float x_scale, to_a, to_d, unscale_b, unscale_x;
     size_t smem;

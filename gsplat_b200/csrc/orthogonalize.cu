@@ -411,7 +411,7 @@ constexpr double kOrthoMaxTop = 16.0; // larger singular values would leave the 
 
 struct OrthoPlan {
     int rows, cols, m, n, transposed, steps;
-    bool split, backward;
+    bool split;
     int chunks;        // of the norm's sum
     size_t chunk_size; // values
     OrthoScales s;
@@ -431,7 +431,6 @@ static OrthoPlan ortho_plan(int rows, int cols, int dtype, const OrthoCoefficien
     p.m = p.transposed ? cols : rows;
     p.n = p.transposed ? rows : cols;
     p.steps = co.steps;
-    p.backward = backward;
     p.split = dtype != kOrthoBF16 || backward || kept || p.n <= 128;
     const size_t numel = (size_t)rows * cols;
     p.chunk_size = std::max<size_t>(8192, (numel / 512 + 3) / 4 * 4); // about 512 blocks for a large matrix

@@ -21,6 +21,7 @@ enum OrthoDtype : int { kOrthoF32 = 0, kOrthoBF16 = 1, kOrthoF16 = 2 };
 
 constexpr int kOrthoMaxSteps = 32;
 constexpr int kOrthoMaxTensors = 32; // tensors of one launch
+constexpr int kOrthoMaxSide = 2000000000; // rows or columns: sides rounded up to a tile are held in 32 bits
 
 struct OrthoCoefficients {
     int steps;

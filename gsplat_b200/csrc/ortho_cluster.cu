@@ -621,7 +621,7 @@ static bool cluster_fits(const ClusterShape &s) { return s.columns <= 512 && s.s
 
 // The blocks of a cluster for a matrix, or 0 where it does not fit.
 static int cluster_blocks(int rows, int cols) {
-    if (std::min(rows, cols) > kClusterMaxShort) return 0;
+    if (std::min(rows, cols) > kClusterMaxShort || std::max(rows, cols) > 512 * kClusterMax) return 0; // 512 columns of TMEM a block
     for (int c = 1; c <= kClusterMax; c *= 2)
         if (cluster_fits(cluster_shape(rows, cols, c))) return c;
     return 0;

@@ -742,6 +742,8 @@ static int ortho_tiled_bwd(const OrthoPlan &p, const OrthoCoefficients &co, long
 static int check_common(const char *what, long long batch, int rows, int cols, int dtype, int steps,
                         const float *coefficients, float eps, OrthoCoefficients *co) {
     if (batch < 0 || rows < 0 || cols < 0) return set_error(kErrInvalidArgument, "%s: negative size", what);
+    if (std::max(rows, cols) > kOrthoMaxSide)
+        return set_error(kErrInvalidArgument, "%s: [%d, %d]: a side may have %d values", what, rows, cols, kOrthoMaxSide);
     if (dtype < kOrthoF32 || dtype > kOrthoF16) return set_error(kErrUnsupported, "%s: dtype %d", what, dtype);
     if (steps < 1 || steps > kOrthoMaxSteps)
         return set_error(kErrInvalidArgument, "%s: steps must be 1 to %d, got %d", what, kOrthoMaxSteps, steps);
@@ -782,7 +784,9 @@ static size_t plan_bytes(const OrthoPlan &p, long long batch) {
 using namespace gsb;
 
 extern "C" size_t gsb_orthogonalize_kept_bytes(long long batch, int rows, int cols, int steps) {
-    if (batch <= 0 || rows <= 0 || cols <= 0 || steps < 1 || steps > kOrthoMaxSteps || ortho_is_thin(rows, cols)) return 0;
+    if (batch <= 0 || rows <= 0 || cols <= 0 || std::max(rows, cols) > kOrthoMaxSide || steps < 1 || steps > kOrthoMaxSteps ||
+        ortho_is_thin(rows, cols))
+        return 0;
     OrthoCoefficients co = {};
     co.steps = steps;
     const OrthoPlan p = ortho_plan(rows, cols, kOrthoF32, co, true, true);
@@ -792,7 +796,9 @@ extern "C" size_t gsb_orthogonalize_kept_bytes(long long batch, int rows, int co
 }
 
 extern "C" size_t gsb_orthogonalize_scratch_bytes(long long batch, int rows, int cols, int dtype, int steps, int backward, int kept) {
-    if (batch <= 0 || rows <= 0 || cols <= 0 || steps < 1 || steps > kOrthoMaxSteps || ortho_is_thin(rows, cols)) return 0;
+    if (batch <= 0 || rows <= 0 || cols <= 0 || std::max(rows, cols) > kOrthoMaxSide || steps < 1 || steps > kOrthoMaxSteps ||
+        ortho_is_thin(rows, cols))
+        return 0;
     if (!backward && ortho_is_clustered(rows, cols)) return 0;
     OrthoCoefficients co = {};
     co.steps = steps;
@@ -808,7 +814,7 @@ static int check_kept(long long batch, int rows, int cols, int steps, const void
 }
 
 extern "C" int gsb_orthogonalize_tile(long long batch, int rows, int cols, int dtype, int kept, int product, int sms) {
-    if (batch <= 0 || rows <= 0 || cols <= 0 || product < 0 || product > 5 || sms < 2 || ortho_is_thin(rows, cols) ||
+    if (batch <= 0 || rows <= 0 || cols <= 0 || std::max(rows, cols) > kOrthoMaxSide || product < 0 || product > 5 || sms < 2 || ortho_is_thin(rows, cols) ||
         (product < 3 && ortho_is_clustered(rows, cols)))
         return 0;
     OrthoCoefficients co = {};
@@ -954,7 +960,7 @@ static int check_tensors(int n_tensors, const GsbMuonTensor *tensors) {
     if (n_tensors > 0 && tensors == nullptr) return set_error(kErrInvalidArgument, "muon: no tensor list");
     for (int i = 0; i < n_tensors; ++i) {
         const GsbMuonTensor &t = tensors[i];
-        if (t.batch < 0 || t.rows < 0 || t.cols < 0 || t.inner < 1)
+        if (t.batch < 0 || t.rows < 0 || t.cols < 0 || std::max(t.rows, t.cols) > kOrthoMaxSide || t.inner < 1)
             return set_error(kErrInvalidArgument, "muon: tensor %d: %lld x [%d, %d], inner %d", i, t.batch, t.rows, t.cols, t.inner);
         if (!(t.gain == tensors[0].gain)) return set_error(kErrInvalidArgument, "muon: tensor %d: a gain of its own", i);
     }

@@ -113,6 +113,8 @@ def adam_multi(groups, valid: Optional[Tensor], b1: float, b2: float) -> None:
 #: singular values down to about 0.003 into [0.7, 1.2].
 MUON_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
+_ORTHO_MAX_SIDE = 2_000_000_000
+
 _ORTHO_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -185,6 +187,8 @@ def orthogonalize(
     """
     if x.dim() < 2:
         raise ValueError(f"x must be [..., M, N], got {tuple(x.shape)}")
+    if max(x.shape[-2:]) > _ORTHO_MAX_SIDE:
+        raise ValueError(f"x {tuple(x.shape)}: a side may have {_ORTHO_MAX_SIDE} values")
     _ortho_dtype("x", x)
     if not eps > 0:
         raise ValueError(f"eps must be positive, got {eps}")
@@ -318,13 +322,15 @@ def muon(
         numel = p.numel()
         if numel == 0:
             continue
+        rows, cols = shape[-2:]
+        if rows > _ORTHO_MAX_SIDE or cols > _ORTHO_MAX_SIDE:
+            raise ValueError(f"param {tuple(shape)}: a side may have {_ORTHO_MAX_SIDE} values")
         at_p, at_g, at_m = p.data_ptr(), g.data_ptr(), m.data_ptr()
         size, state_dtype = numel * (2 if dtype else 4), _ORTHO_DTYPES[m.dtype]
         spans += ((at_p, at_p + size, False), (at_g, at_g + size, True),
                   (at_m, at_m + numel * (2 if state_dtype else 4), False))
-        rows, cols = shape[-2:]
         batch = numel // (rows * cols)
-        inner = batch // shape[0] if len(shape) > 2 else 1
+        inner = batch // shape[0] if valid is not None else 1
         groups.setdefault((dtype, state_dtype), []).append(
             (at_p, at_g, at_m, batch, rows, cols, inner, rate * scale, 1.0 - rate * weight_decay, 1.0 - momentum))
     read_end = write_end = 0

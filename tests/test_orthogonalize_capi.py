@@ -62,3 +62,30 @@ def test_scratch_of_a_forward_that_keeps_its_state():
     assert size(1, 3000, 2900, 0, 5, 0, 0) > 100 * 2**20
     assert size(1, 3000, 2900, 0, 5, 0, 1) < 2**16
     assert size(1, 300, 200, 0, 5, 1, 1) > 2**20 // 4  # backwards G, S and T are
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 1_100_000_000), (1_999_999_999, 1), (5000, 128), (128, 4097)])
+def test_sizes_of_long_matrices(rows, cols):
+    """Far beyond what a cluster holds, where its size was searched for without end; the scratch holds two X as pairs of halves."""
+    x = -(-max(rows, cols) // 8) * 8 * min(rows, cols)
+    assert 8 * x < lib().gsb_orthogonalize_scratch_bytes(1, rows, cols, 1, 5, 0, 0) < 8 * x + 2**20
+    assert lib().gsb_orthogonalize_tile(1, rows, cols, 1, 0, 0, 148) > 0
+
+
+def test_sides_that_do_not_fit_are_refused():
+    from gsplat_b200.cuda._backend import GsbMuonTensor
+
+    L, c, side = lib(), (ctypes.c_float * 15)(*(list(N.QUINTIC) * 5)), 2_000_000_001
+    for rows, cols in ((1, side), (side, 1), (1, 2**31 - 1)):
+        assert L.gsb_orthogonalize_scratch_bytes(1, rows, cols, 0, 5, 0, 0) == 0 and L.gsb_orthogonalize_kept_bytes(1, rows, cols, 5) == 0
+        for f, pointers in ((L.gsb_orthogonalize_fwd, 2), (L.gsb_orthogonalize_bwd, 3)):
+            rc = f(1, rows, cols, 0, *[None] * pointers, 5, c, 1e-7, None, 0, SOMEWHERE, 1 << 40, None)
+            assert rc == -1 and b"a side may" in L.gsb_last_error()
+        one = (GsbMuonTensor * 1)((None, None, None, 1, rows, cols, 1, 0.1, 1.0))
+        assert L.gsb_muon(1, one, 0, 0, None, 0.9, 1, 5, c, 1e-7, SOMEWHERE, 1 << 40, None) == -1
+    import gsplat_b200
+
+    # a size of 2^32 + 3 would otherwise pass for 3
+    for shape in ((1, 2**32 + 3), (2**32 + 3, 1), (2, 1, side)):
+        with pytest.raises(ValueError, match="a side may"):
+            gsplat_b200.orthogonalize(torch.zeros(1).expand(shape))

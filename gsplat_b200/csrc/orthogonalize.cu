@@ -832,6 +832,18 @@ extern "C" int gsb_orthogonalize_tile(long long batch, int rows, int cols, int d
     return 1000 * t.ranks + t.columns;
 }
 
+// What a kernel would follow: the caller's tensors, on a value's boundary, and memory that is read 16 bytes at a time.
+static int check_tensor(const char *what, const void *p, int dtype) {
+    if (p == nullptr) return set_error(kErrInvalidArgument, "%s: a tensor is missing", what);
+    if (reinterpret_cast<uintptr_t>(p) % (dtype == kOrthoF32 ? 4 : 2))
+        return set_error(kErrInvalidArgument, "%s: a tensor between two of its type's values", what);
+    return kOk;
+}
+static int check_room(const char *what, const void *p) {
+    if (reinterpret_cast<uintptr_t>(p) % 16) return set_error(kErrInvalidArgument, "%s: scratch and kept state are aligned to 16 bytes", what);
+    return kOk;
+}
+
 static const char *at_matrix(const void *p, long long b, int rows, int cols, int dtype) {
     return static_cast<const char *>(p) + (size_t)b * rows * cols * (dtype == kOrthoF32 ? 4 : 2);
 }
@@ -843,6 +855,13 @@ extern "C" int gsb_orthogonalize_fwd(long long batch, int rows, int cols, int dt
     if (int e = check_common("orthogonalize", batch, rows, cols, dtype, steps, coefficients, eps, &co)) return e;
     if (batch == 0 || rows == 0 || cols == 0) return kOk;
     if (int e = check_kept(batch, rows, cols, steps, kept, kept_bytes)) return e;
+    const size_t needed = gsb_orthogonalize_scratch_bytes(batch, rows, cols, dtype, steps, 0, kept != nullptr);
+    if (needed > 0 && (scratch == nullptr || scratch_bytes < needed))
+        return set_error(kErrInvalidArgument, "orthogonalize: %zu scratch bytes are needed", needed);
+    if (int e = check_room("orthogonalize", needed > 0 ? scratch : nullptr)) return e;
+    if (int e = check_room("orthogonalize", kept)) return e;
+    for (const void *t : {x, (const void *)y})
+        if (int e = check_tensor("orthogonalize", t, dtype)) return e;
     if (ortho_is_thin(rows, cols)) return ortho_thin_fwd(batch, rows, cols, dtype, x, y, co, eps, stream);
     const OrthoPlan p = make_plan(rows, cols, dtype, co, false, kept != nullptr);
     Carver own{static_cast<char *>(kept)};
@@ -856,8 +875,6 @@ extern "C" int gsb_orthogonalize_fwd(long long batch, int rows, int cols, int dt
         k.step = steps > 1 ? w.x[1].hi - w.x[0].hi : 0;
         return ortho_cluster_fwd(batch, rows, cols, dtype, x, y, co, (float)p.s.x, (float)p.s.a, (float)backward_scale(p), eps, k, stream);
     }
-    if (scratch == nullptr || scratch_bytes < plan_bytes(p, batch))
-        return set_error(kErrInvalidArgument, "orthogonalize: %zu scratch bytes are needed", plan_bytes(p, batch));
     if (kept) {
         const OrthoBuffers w(own, p, batch);
         Carver ws{static_cast<char *>(scratch)};
@@ -881,10 +898,15 @@ extern "C" int gsb_orthogonalize_bwd(long long batch, int rows, int cols, int dt
     if (int e = check_common("orthogonalize", batch, rows, cols, dtype, steps, coefficients, eps, &co)) return e;
     if (batch == 0 || rows == 0 || cols == 0) return kOk;
     if (int e = check_kept(batch, rows, cols, steps, kept, kept_bytes)) return e;
+    const size_t needed = gsb_orthogonalize_scratch_bytes(batch, rows, cols, dtype, steps, 1, kept != nullptr);
+    if (needed > 0 && (scratch == nullptr || scratch_bytes < needed))
+        return set_error(kErrInvalidArgument, "orthogonalize: %zu scratch bytes are needed", needed);
+    if (int e = check_room("orthogonalize", needed > 0 ? scratch : nullptr)) return e;
+    if (int e = check_room("orthogonalize", kept)) return e;
+    for (const void *t : {x, v_y, (const void *)v_x})
+        if (int e = check_tensor("orthogonalize", t, dtype)) return e;
     if (ortho_is_thin(rows, cols)) return ortho_thin_bwd(batch, rows, cols, dtype, x, v_y, v_x, co, eps, stream);
     const OrthoPlan p = make_plan(rows, cols, dtype, co, true, kept != nullptr);
-    if (scratch == nullptr || scratch_bytes < plan_bytes(p, batch))
-        return set_error(kErrInvalidArgument, "orthogonalize: %zu scratch bytes are needed", plan_bytes(p, batch));
     const long long chunk = kept ? batch : ortho_chunk(p, batch);
     for (long long b = 0; b < batch; b += chunk) {
         if (int e = ortho_tiled_bwd(p, co, std::min(chunk, batch - b), at_matrix(x, b, rows, cols, dtype),
@@ -994,6 +1016,14 @@ extern "C" int gsb_muon(int n_tensors, const GsbMuonTensor *tensors, int dtype, 
     const size_t needed = gsb_muon_scratch_bytes(n_tensors, tensors, dtype, steps);
     if (needed > 0 && (scratch == nullptr || scratch_bytes < needed))
         return set_error(kErrInvalidArgument, "muon: %zu scratch bytes are needed", needed);
+    if (int e = check_room("muon", needed > 0 ? scratch : nullptr)) return e;
+    for (int i = 0; i < n_tensors; ++i) {
+        const GsbMuonTensor &u = tensors[i];
+        if (muon_empty(u)) continue;
+        if (int e = check_tensor("muon", u.param, dtype)) return e;
+        if (int e = check_tensor("muon", u.grad, dtype)) return e;
+        if (int e = check_tensor("muon", u.momentum_buffer, state_dtype)) return e;
+    }
     MuonTable t = {};
     t.dtype = dtype;
     t.state_dtype = state_dtype;

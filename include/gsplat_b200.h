@@ -478,7 +478,7 @@ GSB_API int gsb_adam_multi(int n_groups, const GsbAdamGroup *groups, const bool 
  * (the same for all), since a float near 1 leaves few bits of it.
  * momentum_buffer has the type of param or float32 (state_dtype). valid (optional): a row of a tensor's leading
  * dimension (`inner` matrices) whose entry is false keeps its values. Tensors must not overlap.
- * Scratch: gsb_orthogonalize_scratch_bytes of the whole batch (kept = 1: for a call with a
+ * Scratch and kept state are aligned to 16 bytes. Scratch: gsb_orthogonalize_scratch_bytes of the whole batch (kept = 1: for a call with a
  * kept state), gsb_muon_scratch_bytes of the list; 0 where none is needed. Calls that
  * may run at the same time need scratch of their own. */
 GSB_API size_t gsb_orthogonalize_kept_bytes(long long batch, int rows, int cols, int steps);

@@ -89,3 +89,37 @@ def test_sides_that_do_not_fit_are_refused():
     for shape in ((1, 2**32 + 3), (2**32 + 3, 1), (2, 1, side)):
         with pytest.raises(ValueError, match="a side may"):
             gsplat_b200.orthogonalize(torch.zeros(1).expand(shape))
+
+
+def test_missing_and_misplaced_pointers_are_refused():
+    from gsplat_b200.cuda._backend import GsbMuonTensor
+
+    L, c = lib(), (ctypes.c_float * 15)(*(list(N.QUINTIC) * 5))
+
+    def fwd(rows, cols, dtype, x, y, scratch=SOMEWHERE, kept=None):
+        size = L.gsb_orthogonalize_kept_bytes(1, rows, cols, 5) if kept else 0
+        return L.gsb_orthogonalize_fwd(1, rows, cols, dtype, x, y, 5, c, 1e-7, kept, size, scratch, 1 << 40, None)
+
+    def bwd(rows, cols, dtype, x, v, out, scratch=SOMEWHERE):
+        return L.gsb_orthogonalize_bwd(1, rows, cols, dtype, x, v, out, 5, c, 1e-7, None, 0, scratch, 1 << 40, None)
+
+    for rows, cols in ((15, 3), (3, 60), (40, 50), (300, 200)):
+        for bad in (None, SOMEWHERE + 1, SOMEWHERE + 2):
+            want = b"missing" if bad is None else b"between"
+            assert fwd(rows, cols, 0, bad, SOMEWHERE) == -1 and want in L.gsb_last_error()
+            assert fwd(rows, cols, 0, SOMEWHERE, bad) == -1 and want in L.gsb_last_error()
+            for i in range(3):
+                p = [SOMEWHERE] * 3
+                p[i] = bad
+                assert bwd(rows, cols, 0, *p) == -1 and want in L.gsb_last_error()
+        assert fwd(rows, cols, 1, SOMEWHERE + 1, SOMEWHERE) == -1 and b"between" in L.gsb_last_error()
+    assert fwd(300, 200, 0, SOMEWHERE, SOMEWHERE, scratch=SOMEWHERE + 8) == -1 and b"16 bytes" in L.gsb_last_error()
+    assert fwd(300, 200, 0, SOMEWHERE, SOMEWHERE, kept=SOMEWHERE + 8) == -1 and b"16 bytes" in L.gsb_last_error()
+    assert bwd(40, 50, 0, SOMEWHERE, SOMEWHERE, SOMEWHERE, scratch=SOMEWHERE + 4) == -1 and b"16 bytes" in L.gsb_last_error()
+    for i in range(3):
+        for bad, state in ((None, 0), (SOMEWHERE + 2, 0), (SOMEWHERE + 1, 1)):
+            p = [SOMEWHERE] * 3
+            p[i] = bad
+            one = (GsbMuonTensor * 1)((*p, 1, 4, 4, 1, 0.1, 1.0))
+            assert L.gsb_muon(1, one, state, state, None, 0.9, 1, 5, c, 1e-7, None, 0, None) == -1
+            assert (b"missing" if bad is None else b"between") in L.gsb_last_error()

@@ -69,6 +69,10 @@ class Muon(torch.optim.Optimizer):
                 loss = closure()
         if visibility is not None:
             visibility = visibility.contiguous()
+            for group in self.param_groups:  # all or nothing
+                for p in group["params"]:
+                    if p.grad is not None and (p.dim() < 3 or p.shape[0] != len(visibility)):
+                        raise ValueError(f"visibility [{len(visibility)}] does not mask the leading dimension of {tuple(p.shape)}")
         for group in self.param_groups:
             params, grads, buffers, scales = [], [], [], []
             for p in group["params"]:

@@ -134,3 +134,16 @@ def test_unsuitable_parameters_are_refused_before_the_first_step():
             opt.add_param_group(bad)
     assert len(opt.param_groups) == 1
     opt.add_param_group(dict(params=[half], momentum_dtype=torch.float32))
+
+
+def test_unsuitable_mask_leaves_all_groups_as_they_were(plain):
+    rows, plain_matrix = torch.nn.Parameter(torch.ones(5, 4, 3)), torch.nn.Parameter(torch.ones(5, 4))
+    for other in (plain_matrix, torch.nn.Parameter(torch.ones(6, 4, 3))):
+        opt = gsplat_b200.Muon([dict(params=[rows]), dict(params=[other])])
+        rows.grad, other.grad = torch.ones(5, 4, 3), torch.ones_like(other)
+        with pytest.raises(ValueError, match="does not mask"):
+            opt.step(torch.ones(5, dtype=torch.bool))
+        assert (rows == 1).all() and not opt.state
+    other.grad = None  # nothing to step there
+    opt.step(torch.ones(5, dtype=torch.bool))
+    assert (rows != 1).any()

@@ -219,7 +219,7 @@ struct OrthoGemm {
     void *y;                 // kEpiOut: [batch, rows, cols] of `dtype`
     int dtype, transposed;   // transposed: y is [N, M] in memory (kEpiMuon: the table says it)
     int *error;              // set when a kernel's wait ran out; the last product then writes NaN. Where that is the product
-                             // whose wait ran out, its block does for this tile and those it had still to do
+                             // whose wait ran out, its block does for all of its tiles
 };
 
 int ortho_gemm(const OrthoGemm &g, const MuonTable *table, cudaStream_t stream);

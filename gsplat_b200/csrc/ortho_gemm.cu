@@ -40,7 +40,7 @@ static int sm_count() {
 OrthoTile ortho_tile(const OrthoGemm &g, int sms) {
     // The tile with the least time: rounds over the SMs x cycles of a product 16 deep / blocks that share the depth. The
     // cycles are measured: the operand bytes that an SM's shared memory delivers bound them where few SMs work, those
-    // that the L2 delivers (7 KB a cycle) where all do. A 128 x 64 tile 79, or 122 for hi planes alone on all SMs;
+    // that the L2 delivers (5 to 6.3 KB a cycle with all of them) where all do. A 128 x 64 tile 79, or 122 for hi planes alone on all SMs;
     // 128 x 128 112 split, 126 or 162; a pair's 256 x 256 165 split (also where few work, for its longer end), 237.
     const int tm = (g.M + kBM - 1) / kBM, tn = (g.N + 127) / 128, tn64 = (g.N + 63) / 64;
     const int pm = (g.M + kPair - 1) / kPair, pn = (g.N + kPair - 1) / kPair;
@@ -52,7 +52,7 @@ OrthoTile ortho_tile(const OrthoGemm &g, int sms) {
     const long long t64 = (n64 + sms - 1) / sms * (g.split || n64 * r64 <= sms / 2 ? 79 : 122) / r64;
     const long long t128 = (n128 + sms - 1) / sms * (g.split ? 112 : n128 * r128 <= sms / 2 ? 126 : 162) / r128;
     const long long t256 = (n256 + sms / 2 - 1) / (sms / 2) * (g.split || n256 <= sms / 4 ? 165 : 237);
-    if (t256 < t128 && t256 < t64 && (g.split || g.K <= kPairHiDepth)) return {256, 1};
+    if (t256 < t128 && t256 < t64 && (g.split || g.K <= kHiDepth)) return {256, 1};
     return t64 < t128 ? OrthoTile{64, r64} : OrthoTile{128, r128};
 }
 

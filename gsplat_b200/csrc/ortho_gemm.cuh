@@ -5,7 +5,7 @@
 //
 // A tile is 128 x BN of the result, 64 deep a stage. With SPLIT, a stage holds
 // the hi and lo planes of both operands and feeds three products (hi hi, hi lo, lo hi);
-// the sum is taken out of the tensor cores every kChunk stages (kHiChunk without it) and continued in
+// the sum is taken out of the tensor cores every kChunk stages and continued in
 // registers, since their 32-bit adder truncates and the bias of a long sum of
 // squares would be seen in the diagonal of A.
 // A product of a middle-sized matrix takes about 8.5 us: 1.8 from the end of the launch before it, 2.2 until the first copies are
@@ -15,7 +15,6 @@
 
 #include <algorithm>
 #include <cuda.h>
-#include <type_traits>
 
 #include "ortho.cuh"
 #include "tcgen05.cuh"
@@ -25,9 +24,10 @@ namespace gsb {
 constexpr int kBM = 128, kBK = 64;
 constexpr int kChunk = 4; // stages between two readings of the accumulator, split: a result 1.3e-6 off, 2.6e-6 with 8
                           // (FP32 GEMMs 2.5 to 4.8e-6)
-// Products of hi alone are read out every 2048 of depth: the truncation takes 5e-8 of the sum at each of its additions (16
-// deep), 6e-6 in 2048, where the operands' 11 bits take 2e-4. Unread, the square of a row of 8 million was 3e-3 short.
-constexpr int kHiChunk = 32;
+// Products of hi alone deeper than kHiDepth (LONG) are read out every kHiChunk stages: the truncation takes 5e-8 of the sum at each
+// of its additions (16 deep), 5e-5 in 16384, where the operands' 11 bits take 2e-4. Unread, the square of a row of 8 million
+// was 0.7% short. The others are not read out, which is 1 to 2% faster.
+constexpr int kHiDepth = 16384, kHiChunk = 32;
 constexpr int kEpilogueWarps = 8;  // four lane quarters x two column halves
 constexpr int kGemmThreads = 32 * (kEpilogueWarps + 2);
 constexpr int kStagePitch = 33;    // floats a row of a warp's 32 x 32 values on their way out
@@ -267,17 +267,18 @@ __device__ __forceinline__ void finish32(const OrthoGemm &g, const MuonTable &ta
     else put_out<__half, EPI == kEpiMuon>(to, v, p, stage, lane, lr, decay, poisoned);
 }
 
-// A wait ran out at tile t of the last product: NaN for the warp's part (from row `row` and column `col` of a tile, `width`
-// columns) of this tile and of those that the block had still to do.
+// A wait of the last product ran out in this block: its epilogue warps write NaN to its 128 rows, from row0, of each of its
+// tiles, of which one may have been finished from a sum that was not whole.
 template <int EPI, int BN, int ROWS>
 __device__ void give_up(const OrthoGemm &g, const MuonTable &tab, long long t, long long tiles, long long stride, int per, int tiles_n,
-                        int row, int col, int width) {
-    const int lane = threadIdx.x % 32;
-    for (; t < tiles; t += stride) {
+                        int row0) {
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, row = row0 + 32 * (warp % 4) + lane, col = warp / 4 * (BN / 2);
+    for (; warp < kEpilogueWarps && t < tiles; t += stride) {
         const TileAt at = tile_at<kBM>(t, per, tiles_n, false);
         const int tensor = tab.n > 0 ? muon_tensor_of(tab, at.b) : 0;
         if (tab.n > 0 && !muon_visible(tab, tensor, at.b)) continue;
-        for (int c = 0; c < width; c += 32) {
+#pragma unroll 1
+        for (int c = 0; c < BN / 2; c += 32) {
             const OutAt to = out_at<EPI>(g, tab, tensor, at.b, at.i * ROWS + row, at.j * BN + col + c, lane);
 #pragma unroll 1
             for (int k = 0; k < to.n && k < 32; ++k) {
@@ -346,7 +347,7 @@ __device__ __forceinline__ void store_at(uint32_t addr, float4 v) {
 // sums in its shared memory (where its stages were), and it adds them in the order of the blocks and finishes
 // the tile; a launch then has one tile a cluster. For long contractions with few tiles (A of a
 // short matrix), whose blocks would otherwise work through the depth alone.
-template <bool SPLIT, int BN, int EPI, bool DEEP>
+template <bool SPLIT, int BN, int EPI, bool DEEP, bool LONG>
 __global__ void __launch_bounds__(kGemmThreads, 1)
     ortho_gemm_kernel(const __grid_constant__ OrthoGemm g, const __grid_constant__ GemmMaps maps,
                       const __grid_constant__ MuonTable tab, int per, int tiles_n, long long tiles) {
@@ -394,7 +395,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     const int ranks = DEEP ? (int)cluster_size() : 1, rank = DEEP ? (int)block_rank() : 0;
     const int all = kblocks * g.pairs;                                              // stages of a tile
     const int begin = DEEP ? all * rank / ranks : 0, end = DEEP ? all * (rank + 1) / ranks : all; // this block's
-    const int chunk = SPLIT ? kChunk : kHiChunk;                                    // stages of an accumulation
+    const int chunk = SPLIT ? kChunk : LONG ? kHiChunk : end - begin;                                // stages of an accumulation
     const long long first = DEEP ? blockIdx.x / ranks : blockIdx.x, stride = DEEP ? gridDim.x / ranks : gridDim.x;
     // whether the cluster's one tile is worked on, by all of its blocks' warps
     const bool shared_tile = DEEP && !(tab.n > 0 && !muon_visible(tab, muon_tensor_of(tab, first / per), first / per));
@@ -510,8 +511,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         int acc = 0;
         uint32_t acc_phase = 0;
         bool ok = true;
-        long long t = first;
-        for (; ok && t < tiles; t += stride) {
+        for (long long t = first; ok && t < tiles; t += stride) {
             const TileAt at = tile_at<BN>(t, per, tiles_n, kSymmetric);
             const int tensor = tab.n > 0 ? muon_tensor_of(tab, at.b) : 0;
             if (tab.n > 0 && !muon_visible(tab, tensor, at.b)) continue;
@@ -526,34 +526,23 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             }
             fetch32<SPLIT, EPI>(g, at.b, i - lane, j, lane, e);
             float v[W];
-            auto take = [&](auto known, bool first_part) { // a part of the sum
-                ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[acc], acc_phase, abort) && (E::to_planes || !*abort));
-                if (!ok) return;
+            for (int s0 = begin; s0 < end; s0 += chunk) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[acc], acc_phase, abort));
+                if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t src = tmem + ((uint32_t)(32 * (warp % 4)) << 16) + acc * BN + half * W;
 #pragma unroll
                 for (int c = 0; c < W; c += 32) {
-                    if (known && first_part) {
-                        tmem_load32(src + c, v + c);
-                        continue;
-                    }
                     float u[32];
                     tmem_load32(src + c, u);
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) v[c + k] = !known && first_part ? u[k] : v[c + k] + u[k];
+                    for (int k = 0; k < 32; ++k) v[c + k] = s0 == begin ? u[k] : v[c + k] + u[k];
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.acc_empty[acc]);
                 acc ^= 1;
                 if (acc == 0) acc_phase ^= 1u;
-            };
-            if (SPLIT) {
-                for (int s0 = begin; ok && s0 < end; s0 += chunk) take(std::false_type(), s0 == begin);
-            } else { // mostly the first part is all
-                take(std::true_type(), true);
-#pragma unroll 1
-                for (int s0 = begin + chunk; ok && s0 < end; s0 += chunk) take(std::true_type(), false);
             }
             if (DEEP) { // rank r's sums at r - 1 of [ranks - 1][warp][W / 4][lane], four columns each
                 const uint32_t sums = stage0 + (uint32_t)(warp * (W / 4) * 32 + lane) * 16;
@@ -590,12 +579,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                 finish32<SPLIT, EPI>(g, tab, tensor, at.b, i, j + 32 * c, lane, v + 32 * c, p, di, dj[c], mirror, poisoned, out_stage);
             }
         }
-        if (!E::to_planes && !ok) give_up<EPI, BN, kBM>(g, tab, t, tiles, stride, per, tiles_n, row, half * W, W);
     }
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (!E::to_planes && *abort) give_up<EPI, BN, kBM>(g, tab, blockIdx.x, tiles, gridDim.x, per, tiles_n, 0);
     if (warp == kEpilogueWarps + 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BN) : "memory");
     if (threadIdx.x == 0 && sh.abort) atomicExch(g.error, 1);
@@ -613,26 +602,35 @@ template <bool SPLIT, int BN> static int tile_ranks(const OrthoGemm &g, long lon
     return ranks < 2 ? 1 : tiles <= 8 ? ranks : ranks >= 4 && 4 * tiles <= sms * 7 / 8 ? 4 : 2;
 }
 
-template <bool SPLIT, int BN, int EPI>
-static int launch_one(const OrthoGemm &g, const GemmMaps &maps, const MuonTable &tab, int per, int tn, long long tiles,
+template <bool SPLIT, int BN, int EPI, bool LONG>
+static int launch_depth(const OrthoGemm &g, const GemmMaps &maps, const MuonTable &tab, int per, int tn, long long tiles,
                       int sms, cudaStream_t stream) {
     constexpr int smem = Stages<SPLIT, BN>::smem;
     const int ranks = tile_ranks<SPLIT, BN>(g, tiles, sms);
     constexpr bool kDeep = EPI == kEpiGram || EPI == kEpiSym;
     if constexpr (kDeep) {
         if (ranks > 1) {
-            auto *kernel = ortho_gemm_kernel<SPLIT, BN, EPI, true>;
+            auto *kernel = ortho_gemm_kernel<SPLIT, BN, EPI, true, LONG>;
             if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
                 return check_launch("ortho_gemm_kernel attributes");
             return launch_clusters_after(kernel, ranks, (unsigned)(tiles * ranks), kGemmThreads, smem, stream, "ortho_gemm_kernel", g, maps,
                                          tab, per, tn, tiles);
         }
     }
-    auto *kernel = ortho_gemm_kernel<SPLIT, BN, EPI, false>;
+    auto *kernel = ortho_gemm_kernel<SPLIT, BN, EPI, false, LONG>;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
         return check_launch("ortho_gemm_kernel attributes");
     return launch_after(kernel, (unsigned)(tiles < sms ? tiles : sms), kGemmThreads, smem, stream, "ortho_gemm_kernel", g, maps, tab,
                         per, tn, tiles);
+}
+
+template <bool SPLIT, int BN, int EPI>
+static int launch_one(const OrthoGemm &g, const GemmMaps &maps, const MuonTable &tab, int per, int tn, long long tiles,
+                      int sms, cudaStream_t stream) {
+    // (B and X are as wide as they are deep, at least, and then never take 64 columns)
+    constexpr bool kLong = !SPLIT && (BN == 128 || EPI == kEpiGram);
+    if (kLong && g.K > kHiDepth) return launch_depth<SPLIT, BN, EPI, kLong>(g, maps, tab, per, tn, tiles, sms, stream);
+    return launch_depth<SPLIT, BN, EPI, false>(g, maps, tab, per, tn, tiles, sms, stream);
 }
 
 template <bool SPLIT, int BN>

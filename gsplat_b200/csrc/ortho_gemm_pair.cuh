@@ -15,12 +15,10 @@
 namespace gsb {
 
 constexpr int kPair = 256;   // rows and columns of a tile
-constexpr int kPairChunk = 8; // stages between two readings of the accumulator, split (4 cost 8% of a product)
-// Of hi alone sums are not read out, so that they need no registers and a warp finishes 32 columns at a time (with
-// registers for the sum [2048, 8192] took 1047 us instead of 752). The truncation takes 5e-5 of a sum 16384 deep, a quarter of
-// what the operands' 11 bits take; deeper ones are left to the tiles of ortho_gemm.cuh.
-constexpr int kPairHiDepth = 16384;
-
+// Stages between two readings of the accumulator, split (4 cost 8% of a product). Of hi alone sums are not read out, so that they
+// need no registers and a warp finishes 32 columns at a time (with registers for the sum [2048, 8192] took 1047 us instead of
+// 752); those deeper than kHiDepth are left to the tiles of one SM.
+constexpr int kPairChunk = 8;
 // Split sums go on in 128 registers of an epilogue thread, more than three warpgroups at 168 leave it: the
 // warpgroup of the copies and products gives 112 of its own. 2 x 224 + 56 = 3 x 168.
 constexpr int kPairThreads = 384, kPairRegisters = 168, kEpilogueRegisters = 224, kIssueRegisters = 56;
@@ -218,8 +216,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         int acc = 0;
         uint32_t acc_phase = 0;
         bool ok = true;
-        long long t = first;
-        for (; ok && t < tiles; t += pairs) {
+        for (long long t = first; ok && t < tiles; t += pairs) {
             const TileAt at = tile_at<kBM>(t, per, tiles_n, kSymmetric);
             const int tensor = tab.n > 0 ? muon_tensor_of(tab, at.b) : 0;
             if (tab.n > 0 && !muon_visible(tab, tensor, at.b)) continue;
@@ -247,7 +244,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             if (SPLIT) { // the sum goes on in registers
                 float v[W];
                 for (int s0 = 0; ok && s0 < total; s0 += chunk) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[acc], acc_phase, abort) && (E::to_planes || !*abort));
+                    ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[acc], acc_phase, abort));
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint32_t src = tmem + ((uint32_t)(32 * (warp % 4)) << 16) + acc * kPair + half * W;
@@ -264,7 +261,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 #pragma unroll
                 for (int c = 0; c < W; c += 32) finish(c, v + c);
             } else {
-                ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[acc], acc_phase, abort) && (E::to_planes || !*abort));
+                ok = __all_sync(0xffffffffu, mbar_wait(&sh.acc_full[acc], acc_phase, abort));
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t src = tmem + ((uint32_t)(32 * (warp % 4)) << 16) + acc * kPair + half * W;
@@ -277,7 +274,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 release();
             }
         }
-        if (!E::to_planes && !ok) give_up<EPI, kPair, kPair>(g, tab, t, tiles, pairs, per, tiles_n, (int)rank * 128 + row, half * W, W);
     }
     if (warp < kEpilogueWarps && *abort) abort_other(abort, rank);
     if (threadIdx.x == 0 && *abort) atomicExch(g.error, 1);
@@ -285,6 +281,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     cluster_barrier(); // neither block leaves while the other may reach its shared memory
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (!E::to_planes && *abort) give_up<EPI, kPair, kPair>(g, tab, first, tiles, pairs, per, tiles_n, (int)rank * 128);
     if (warp == kEpilogueWarps + 1)
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * kPair) : "memory");
 }

@@ -140,3 +140,16 @@ def test_muon_step_taken_in_pieces():
         # the update has a norm of about 11, lr 0.1 of it; the parameter's is about 3.5 and its rounding beside that
         tol = 2 * N.tolerance(g[:50].cpu(), 5, N.QUINTIC)
         assert per_matrix(got_p[valid], q) <= tol + 5 * 2.0**-24
+
+
+def test_deep_products_of_bfloat16():
+    """Short sides above 16384: every product of hi alone is read out on its way. The model's distance is taken of a smaller
+    matrix of the same make; it does not grow with the side, whose roundings are independent."""
+    shape, steps = (1, 16400, 16500), 2
+    x = made(shape, torch.bfloat16, 560)
+    want = N.newton_schulz(x, steps)
+    tol = N.tolerance(made((1, 2000, 2100), torch.bfloat16, 561).cpu(), steps, N.QUINTIC)
+    assert per_matrix(gs().orthogonalize(x, steps), want) <= 2 * tol
+    p, m = torch.zeros_like(x), torch.zeros_like(x)
+    gs().muon(p, x, m, None, 1.0, 0.0, nesterov=False, steps=steps)
+    assert per_matrix(-p, want) <= 2 * tol

@@ -39,3 +39,8 @@ def test_no_tiles_where_there_are_none():
     assert tiles((5, 15, 3), 0, range(6)) == [0] * 6  # thin
     assert tiles((5, 64, 64), 0, range(3)) == [0] * 3 and tiles((5, 64, 64), 0, [3]) == [1064]  # clustered, but not backwards
     assert tiles((5, 200, 200), 0, [-1, 6]) == [0, 0]
+
+
+def test_deep_products_of_bfloat16_leave_the_pair():
+    assert tiles((1, 16300, 16300), 1, range(3)) == [1256] * 3 and tiles((1, 16400, 16500), 1, range(3)) == [1128] * 3
+    assert tiles((1, 16400, 16500), 0, range(3)) == [1256] * 3

@@ -273,7 +273,7 @@ template <int EPI, int BN, int ROWS>
 __device__ void give_up(const OrthoGemm &g, const MuonTable &tab, long long t, long long tiles, long long stride, int per, int tiles_n,
                         int row0) {
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, row = row0 + 32 * (warp % 4) + lane, col = warp / 4 * (BN / 2);
-    for (; warp < kEpilogueWarps && t < tiles; t += stride) {
+    for (; t < tiles; t += stride) {
         const TileAt at = tile_at<kBM>(t, per, tiles_n, false);
         const int tensor = tab.n > 0 ? muon_tensor_of(tab, at.b) : 0;
         if (tab.n > 0 && !muon_visible(tab, tensor, at.b)) continue;
@@ -584,7 +584,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    if (!E::to_planes && *abort) give_up<EPI, BN, kBM>(g, tab, blockIdx.x, tiles, gridDim.x, per, tiles_n, 0);
+    if (!E::to_planes && warp < kEpilogueWarps && *abort) give_up<EPI, BN, kBM>(g, tab, blockIdx.x, tiles, gridDim.x, per, tiles_n, 0);
     if (warp == kEpilogueWarps + 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BN) : "memory");
     if (threadIdx.x == 0 && sh.abort) atomicExch(g.error, 1);

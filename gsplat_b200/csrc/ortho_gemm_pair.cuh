@@ -281,7 +281,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     cluster_barrier(); // neither block leaves while the other may reach its shared memory
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    if (!E::to_planes && *abort) give_up<EPI, kPair, kPair>(g, tab, first, tiles, pairs, per, tiles_n, (int)rank * 128);
+    if (!E::to_planes && warp < kEpilogueWarps && *abort) give_up<EPI, kPair, kPair>(g, tab, first, tiles, pairs, per, tiles_n, (int)rank * 128);
     if (warp == kEpilogueWarps + 1)
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * kPair) : "memory");
 }

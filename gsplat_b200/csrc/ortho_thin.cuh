@@ -8,8 +8,9 @@
 //    paired 32-bit instruction, and its block moves the matrices between global and shared memory
 //    in their own order. Nothing is repeated or shuffled, which matters since the
 //    instruction issue, not memory, bounded the other layout (83% of issue slots
-//    and 11% of DRAM at 1M x [15, 3]). 1M x [15, 3] fp32: forward 80 us (4.5 TB/s), Muon step 146 (6.2 TB/s), with 45% of the
-//    matrices visible 136, backward 327.
+//    and 11% of DRAM at 1M x [15, 3]). 1M x [15, 3] fp32: forward 80 us (4.5 TB/s; 70% of issue slots, 19 warps an SM), Muon
+//    step 147 (6.1 TB/s), with 45% of the matrices visible 136 (39% of issue slots, 15 warps), backward 330: every step's X lies in shared
+//    memory, which leaves room for 6 warps an SM (44% of issue slots).
 //  - "grouped", for few matrices or long ones: 2^g lanes hold one matrix, four rows a
 //    lane, and A is summed over them with shuffles.
 #pragma once

@@ -14,7 +14,8 @@
 // Products are of hi + lo, in three matrix products (lo lo is below 2^-22). Those of
 // bfloat16 matrices (8 bits) are of hi alone, with its 11 bits, while X itself goes from
 // step to step with hi and lo: a X + B X is where small singular values would lose theirs.
-// The result is then 0.0005 to 0.001 off (2-norm), against the type's own rounding of 0.0017.
+// The result is then 0.0005 to 0.001 off (2-norm), against the type's own rounding of 0.0017; sums are read out of the tensor
+// cores before their truncation counts beside that (ortho_gemm.cuh), so that it holds for long sides too.
 // float16 results would be off by three times their rounding that way, and backward passes by the
 // sum of theirs, so they take hi + lo as float32 does; so do matrices of at most 128 x 128, whose
 // calls are bound by latency.

@@ -178,8 +178,10 @@ def orthogonalize(
     coefficients bring all but the smallest near 1 in five steps; (1.5, -0.5, 0) converges to the orthogonal
     factor itself. ``coefficients`` may also be a list with a triple for each step. Polynomials that
     take a singular value in [0, 1] above 16 are refused. Matrices are multiplied with 22 significand
-    bits, bfloat16 ones with a side above 128 with 11 where no gradient is wanted; the result has x's
-    shape and type. A matrix with a NaN or an infinity becomes NaN, and no other of the batch.
+    bits, bfloat16 ones with a side above 128 with 11 where no gradient is wanted (the result is then off by up to 0.001 of
+    its norm, and its type's own rounding by 0.0017; ``x.float()`` is multiplied with 22). The result has x's
+    shape and type. X is carried with 22 bits too, but no finer than 2^-37 of a norm of 1: a list of triples that shrinks it on
+    the way, or an ``eps`` far above the norm, costs bits. A matrix with a NaN or an infinity becomes NaN, and no other of the batch.
 
     Differentiable once, in reverse mode. The steps' state is kept for the backward pass, about
     4 steps (x.numel() + 2 B M M) bytes for B matrices of shorter side M (none where it is at most 4 and the
@@ -277,7 +279,9 @@ def muon(
     their parameter's type (float32, bfloat16 or float16), buffers that type or float32. As in :func:`adam`,
     ``valid`` masks the leading dimension, which all params then share (three dimensions or more): masked
     matrices keep their parameter and momentum. Tensors of one shape (or its transpose), and small
-    matrices of any, go through the kernels together. A tensor must not be listed twice or overlap another.
+    matrices of any, go through the kernels together. A tensor must not be listed twice or overlap another, and
+    all must be on one device. bfloat16 updates with a side above 128 are orthogonalised with 11 significand bits in the
+    products, as :func:`orthogonalize` says, whatever the buffer's type; all others with 22.
     """
     if isinstance(params, Tensor):
         params, param_grads, momentum_buffers = [params], [param_grads], [momentum_buffers]

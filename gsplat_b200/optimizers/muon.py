@@ -3,8 +3,8 @@
 No counterpart in the reference; constructor arguments, state (``momentum_buffer``) and
 learning-rate rules are those of ``torch.optim.Muon``. Parameters may also be batches of matrices
 [B, ..., M, N] (the SH bands of N splats, [N, 15, 3], are N matrices), and ``step`` takes
-the visibility mask of ``SelectiveAdam`` for them. All parameters of one shape and type go through the
-kernels together (``gsb_muon``).
+the visibility mask of ``SelectiveAdam`` for them. Each parameter group is one call of ``gsb_muon``, in which the parameters
+of one shape and type go through the kernels together; those of a group are on one device.
 """
 
 import math
@@ -18,7 +18,10 @@ class Muon(torch.optim.Optimizer):
     """``adjust_lr_fn`` scales the update by the matrix's shape: None or ``"original"``:
     sqrt(max(1, M / N)); ``"match_rms_adamw"``: 0.2 sqrt(max(M, N)), the root mean square of an Adam step. The weight
     decay goes by the learning rate alone: param (1 - lr weight_decay).
-    ``momentum_dtype``: the type of the momentum buffers (None: the parameter's; or torch.float32)."""
+    ``momentum_dtype``: the type of the momentum buffers (None: the parameter's; or torch.float32).
+
+    bfloat16 parameters with a side above 128 have their updates orthogonalised with 11 significand bits in the products (off
+    by up to 0.001 of the update's norm), all others with 22."""
 
     def __init__(self, params, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True,
                  ns_coefficients=MUON_COEFFICIENTS, eps=1e-7, ns_steps=5, adjust_lr_fn=None, momentum_dtype=None):

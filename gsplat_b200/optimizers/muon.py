@@ -56,7 +56,7 @@ class Muon(torch.optim.Optimizer):
             for p, key in zip(group["params"], saved["params"]):
                 buffer = loaded[-1]["state"].get(key, {}).get("momentum_buffer")
                 if buffer is not None:
-                    self.state[p]["momentum_buffer"] = buffer.to(p.device, group["momentum_dtype"] or p.dtype).contiguous()
+                    self.state[p]["momentum_buffer"] = buffer.to(p.device, _momentum_type(group, p)).contiguous()
 
     @torch.no_grad()
     def step(self, visibility=None, closure=None):
@@ -83,7 +83,7 @@ class Muon(torch.optim.Optimizer):
                     continue
                 state = self.state[p]
                 if "momentum_buffer" not in state:
-                    state["momentum_buffer"] = torch.zeros_like(p, dtype=group["momentum_dtype"],
+                    state["momentum_buffer"] = torch.zeros_like(p, dtype=_momentum_type(group, p),
                                                                 memory_format=torch.contiguous_format)
                 grad = p.grad
                 if grad.is_sparse:
@@ -104,6 +104,11 @@ def _check_group(group) -> None:
         if group["momentum_dtype"] not in (None, p.dtype, torch.float32):
             raise TypeError(f"momentum_dtype must be None, the parameter's type or float32, got {group['momentum_dtype']} "
                             f"for {p.dtype}")
+
+
+def _momentum_type(group, p):
+    """The group's, or the parameter's where that does not suit it (a loaded group of parameters of another type)."""
+    return group["momentum_dtype"] if group["momentum_dtype"] in (p.dtype, torch.float32) else p.dtype
 
 
 def _shape_factor(rule, rows: int, cols: int) -> float:

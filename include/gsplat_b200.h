@@ -470,7 +470,7 @@ GSB_API int gsb_adam_multi(int n_groups, const GsbAdamGroup *groups, const bool 
  * `kept` state of gsb_orthogonalize_kept_bytes (0: there is none for this shape, or it would be
  * above 1 GiB with the scratch) that the forward call wrote, the backward call, of the
  * same arguments, need not take the steps again; both may have NULL instead. The state says where a
- * wait of the forward call's kernels ran out (shapes above a short side of 128: a first 32-bit word
+ * wait of the forward call's kernels ran out (where that call needs scratch, by a first 32-bit word
  * that is not 0): the gradient is then NaN.
  * gsb_muon: for the listed tensors of one type, each a batch of matrices:
  * m <- m + (1 - momentum)(grad - m); u = grad + momentum (m - grad) (nesterov) or m;

@@ -147,3 +147,20 @@ def test_unsuitable_mask_leaves_all_groups_as_they_were(plain):
     other.grad = None  # nothing to step there
     opt.step(torch.ones(5, dtype=torch.bool))
     assert (rows != 1).any()
+
+
+def test_checkpoint_of_other_parameter_types(plain):
+    """Buffers go to the new parameter's type where the saved momentum_dtype does not suit it, as torch casts them."""
+    half = torch.nn.Parameter(torch.ones(4, 6, dtype=torch.bfloat16))
+    opt = gsplat_b200.Muon([half], momentum_dtype=torch.bfloat16)
+    half.grad = torch.ones(4, 6, dtype=torch.bfloat16)
+    opt.step()
+    full, fresh = torch.nn.Parameter(torch.ones(4, 6)), torch.nn.Parameter(torch.ones(4, 6))
+    other = gsplat_b200.Muon([full])
+    other.load_state_dict(opt.state_dict())
+    assert other.state[full]["momentum_buffer"].dtype == torch.float32
+    assert torch.equal(other.state[full]["momentum_buffer"], opt.state[half]["momentum_buffer"].float())
+    other.param_groups[0]["params"].append(fresh)
+    full.grad, fresh.grad = torch.ones(4, 6), torch.ones(4, 6)
+    other.step()
+    assert other.state[fresh]["momentum_buffer"].dtype == torch.float32
